@@ -55,6 +55,16 @@ void swiglu_fwd(const at::Tensor& a, const at::Tensor& b, at::Tensor& o);
 void swiglu_bwd(const at::Tensor& g, const at::Tensor& a, const at::Tensor& b, at::Tensor& ga, at::Tensor& gb);
 void cross_entropy_fwd_bwd(const at::Tensor& logits, const at::Tensor& labels, at::Tensor& grad, at::Tensor& loss,
                            double scale);
+void top_logits(const at::Tensor& logits, at::Tensor& values, at::Tensor& indices, at::Tensor& lse, double tau);
+void distill_fwd_bwd(const at::Tensor& logits, const c10::optional<at::Tensor>& labels, const at::Tensor& top_values,
+                     const at::Tensor& top_indices, const c10::optional<at::Tensor>& top_lse,
+                     const c10::optional<at::Tensor>& grad, at::Tensor& loss, double tau, double alpha, double grad_scale);
+std::tuple<at::Tensor, at::Tensor> window_attention_fwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                                        int64_t window, int64_t sinks);
+std::tuple<at::Tensor, at::Tensor, at::Tensor> window_attention_bwd(const at::Tensor& go, const at::Tensor& q,
+                                                                    const at::Tensor& k, const at::Tensor& v,
+                                                                    const at::Tensor& o, const at::Tensor& lse,
+                                                                    int64_t window, int64_t sinks);
 void dion_momentum_add(const std::vector<at::Tensor>& M, const std::vector<at::Tensor>& G, at::Tensor& nz);
 void dion_fixup(at::Tensor& P, at::Tensor& R, const at::Tensor& Q0, const at::Tensor& nz);
 void col_sumsq(const at::Tensor& R, at::Tensor& out);
@@ -116,6 +126,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("swiglu_fwd", &bdion::swiglu_fwd);
   m.def("swiglu_bwd", &bdion::swiglu_bwd);
   m.def("cross_entropy_fwd_bwd", &bdion::cross_entropy_fwd_bwd);
+  m.def("top_logits", &bdion::top_logits, "k largest logits of each row, their indices and the row's log-sum-exp");
+  m.def("distill_fwd_bwd", &bdion::distill_fwd_bwd, "distillation loss from a teacher's top logits and its gradient");
+  m.def("window_attention_fwd", &bdion::window_attention_fwd, "sliding-window attention with visible first tokens");
+  m.def("window_attention_bwd", &bdion::window_attention_bwd);
   m.def("dion_momentum_add", &bdion::dion_momentum_add);
   m.def("dion_fixup", &bdion::dion_fixup);
   m.def("col_sumsq", &bdion::col_sumsq);

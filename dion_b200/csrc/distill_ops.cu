@@ -1,0 +1,621 @@
+// Distillation from a teacher's top logits: the k largest logits of every row
+// (with the row's log-sum-exp), and the distillation loss with its gradient.
+// Rows are the tokens, columns the vocabulary; logits are bf16, fp16 or fp32,
+// all arithmetic is fp32.
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <cuda_fp16.h>
+#include <torch/extension.h>
+
+#include <cfloat>
+
+#include "common.cuh"
+#include "host_utils.h"
+
+namespace bdion {
+
+namespace {
+
+constexpr int kThreads = 512;
+constexpr int kWarps = kThreads / 32;
+constexpr int kMaxTop = 1024;     // entries kept per row
+constexpr int kMaxCand = 2048;    // candidates collected per row before ranking
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ float as_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float as_f(__half v) { return __half2float(v); }
+__device__ __forceinline__ float as_f(float v) { return v; }
+
+__device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+__device__ __forceinline__ void put(__half* p, float v) { *p = __float2half_rn(v); }
+__device__ __forceinline__ void put(float* p, float v) { *p = v; }
+
+__device__ __forceinline__ void load8(const __half* p, float* v) {
+  uint4 u = *reinterpret_cast<const uint4*>(p);
+  const __half2* h = reinterpret_cast<const __half2*>(&u);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(h[i]);
+    v[2 * i] = f.x;
+    v[2 * i + 1] = f.y;
+  }
+}
+__device__ __forceinline__ void store8(__half* p, const float* v) {
+  uint4 u;
+  __half2* h = reinterpret_cast<__half2*>(&u);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+  *reinterpret_cast<uint4*>(p) = u;
+}
+using bdion::load8;
+using bdion::store8;
+
+__device__ __forceinline__ float warp_sum(float v) {
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffff, v, o);
+  return v;
+}
+__device__ __forceinline__ float warp_max(float v) {
+  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffff, v, o));
+  return v;
+}
+
+// Block-wide sum / maximum; every thread gets the result. `buf` holds kWarps
+// floats and may be used again once every thread has returned.
+__device__ __forceinline__ float block_sum(float v, float* buf) {
+  v = warp_sum(v);
+  __syncthreads();
+  if (threadIdx.x % 32 == 0) buf[threadIdx.x / 32] = v;
+  __syncthreads();
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < kWarps; ++i) s += buf[i];
+  return s;
+}
+__device__ __forceinline__ float block_max(float v, float* buf) {
+  v = warp_max(v);
+  __syncthreads();
+  if (threadIdx.x % 32 == 0) buf[threadIdx.x / 32] = v;
+  __syncthreads();
+  float s = buf[0];
+#pragma unroll
+  for (int i = 1; i < kWarps; ++i) s = fmaxf(s, buf[i]);
+  return s;
+}
+
+// A running sum of 2^(c * (x - m)) under its running maximum m. The maximum
+// starts at the lowest finite float, so a row of -inf sums to 0 and no
+// inf - inf arises.
+struct RunningSum {
+  float m = -FLT_MAX, s = 0.f;
+  __device__ __forceinline__ void raise(float to, float c) {
+    if (to > m) {
+      s *= ex2((m - to) * c);
+      m = to;
+    }
+  }
+  __device__ __forceinline__ void add(float x, float c) {
+    raise(x, c);
+    s += ex2((x - m) * c);
+  }
+  // over the block: the common maximum and the sum under it
+  __device__ __forceinline__ void join(float c, float* buf) {
+    const float all = block_max(m, buf);
+    s = block_sum(s * ex2((m - all) * c), buf);
+    m = all;
+  }
+};
+
+// Whole number whose order is the float's; -0 ranks as 0, a NaN above all.
+__device__ __forceinline__ uint32_t order_key(float x) {
+  if (x != x) return 0xffffffffu;
+  const uint32_t b = __float_as_uint(x + 0.f);
+  return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+}
+
+// Calls f(column, values, count) over the row: 8 elements at a time where the
+// row is 16-byte aligned, single ones at its ends (`lead` elements first), or
+// everywhere when `vec` is false.
+template <typename T, typename F>
+__device__ __forceinline__ void for_row(const T* row, int V, int lead, F f) {
+  for (int c = threadIdx.x; c < lead; c += kThreads) {
+    float v[8] = {as_f(row[c])};
+    f(c, v, std::integral_constant<int, 1>{});
+  }
+  const int n8 = (V - lead) / 8;
+  for (int g = threadIdx.x; g < n8; g += kThreads) {
+    float v[8];
+    load8(row + lead + g * 8, v);
+    f(lead + g * 8, v, std::integral_constant<int, 8>{});
+  }
+  for (int c = lead + n8 * 8 + threadIdx.x; c < V; c += kThreads) {
+    float v[8] = {as_f(row[c])};
+    f(c, v, std::integral_constant<int, 1>{});
+  }
+}
+
+// Elements before the first 8-element boundary of row `row` (all of them when
+// the tensor's base is not aligned to 8 elements).
+__device__ __forceinline__ int row_lead(int64_t row, int64_t ld, int V, bool vec) {
+  return vec ? min(V, (int)((8 - (row * ld) % 8) % 8)) : V;
+}
+
+// ------------------------------------------------------------ top logits
+// One block per row. The first pass over the row takes the log-sum-exp and
+// the maximum of each of kThreads * G groups of columns. The k-th largest of
+// those maxima bounds the k-th largest logit from below (k elements are at
+// least that large), so a second pass collects the few columns above it, and
+// each candidate's rank is the number of larger ones (value, then the lower
+// index). Rows with too many equal values for the candidate buffer take the
+// exact threshold bit by bit and keep the lowest indices of the equal ones.
+template <typename T, int G>
+__global__ void __launch_bounds__(kThreads) top_logits_kernel(const T* __restrict__ logits, int64_t ld, int V, int k,
+                                                              bool vec, float c, float* __restrict__ values,
+                                                              int64_t* __restrict__ indices,
+                                                              float* __restrict__ lse) {
+  __shared__ float red[kWarps];
+  __shared__ uint32_t s_max[kThreads * G];
+  __shared__ uint64_t s_cand[kMaxCand];
+  __shared__ int s_n;
+  __shared__ uint32_t s_thr;
+  const int64_t row = blockIdx.x;
+  const T* x = logits + row * ld;
+  const int lead = row_lead(row, ld, V, vec);
+
+  RunningSum sum;
+  uint32_t best[G];
+#pragma unroll
+  for (int g = 0; g < G; ++g) best[g] = 0;
+  int turn = 0;
+  for_row(x, V, lead, [&](int, const float* v, auto n) {
+    constexpr int N = decltype(n)::value;
+    float vm = v[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) vm = fmaxf(vm, v[i]);
+    sum.raise(vm, c);
+    uint32_t key = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      sum.s += ex2((v[i] - sum.m) * c);
+      key = max(key, order_key(v[i]));
+    }
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+      if (turn == g) best[g] = max(best[g], key);
+    turn = turn + 1 == G ? 0 : turn + 1;
+  });
+#pragma unroll
+  for (int g = 0; g < G; ++g) s_max[threadIdx.x * G + g] = best[g];
+  if (threadIdx.x == 0) s_n = 0;
+  sum.join(c, red);
+  if (threadIdx.x == 0) lse[row] = sum.m * c * kLn2 + logf(sum.s);
+
+  // largest threshold that at least k group maxima reach (0: everything is a candidate)
+  if (threadIdx.x < 32) {
+    uint32_t mine[kThreads * G / 32];
+#pragma unroll
+    for (int i = 0; i < kThreads * G / 32; ++i) mine[i] = s_max[i * 32 + threadIdx.x];
+    uint32_t thr = 0;
+    for (int bit = 31; bit >= 0; --bit) {
+      const uint32_t t = thr | (1u << bit);
+      int cnt = 0;
+#pragma unroll
+      for (int i = 0; i < kThreads * G / 32; ++i) cnt += mine[i] >= t;
+      if (__reduce_add_sync(0xffffffff, cnt) >= k) thr = t;
+    }
+    if (threadIdx.x == 0) s_thr = thr;
+  }
+  __syncthreads();
+  uint32_t thr = s_thr;
+  auto collect = [&]() {
+    for_row(x, V, lead, [&](int col, const float* v, auto n) {
+      constexpr int N = decltype(n)::value;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const uint32_t key = order_key(v[i]);
+        if (key >= thr) {
+          const int at = atomicAdd(&s_n, 1);
+          if (at < kMaxCand) s_cand[at] = ((uint64_t)key << 32) | (uint32_t)~(uint32_t)(col + i);
+        }
+      }
+    });
+    __syncthreads();
+  };
+  collect();
+  int n = s_n;
+  if (n > kMaxCand) {
+    // exact threshold: the largest one that at least k logits reach
+    thr = 0;
+    for (int bit = 31; bit >= 0; --bit) {
+      const uint32_t t = thr | (1u << bit);
+      int cnt = 0;
+      for_row(x, V, lead, [&](int, const float* v, auto n) {
+        constexpr int N = decltype(n)::value;
+#pragma unroll
+        for (int i = 0; i < N; ++i) cnt += order_key(v[i]) >= t;
+      });
+      __syncthreads();
+      if (threadIdx.x == 0) s_n = 0;
+      __syncthreads();
+      cnt = __reduce_add_sync(0xffffffff, cnt);
+      if (threadIdx.x % 32 == 0) atomicAdd(&s_n, cnt);
+      __syncthreads();
+      if (s_n >= k) thr = t;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) s_n = 0;
+    __syncthreads();
+    const uint32_t at_thr = thr;
+    if (at_thr != 0xffffffffu) {  // those above it: fewer than k
+      thr = at_thr + 1;
+      collect();
+    }
+    // the equal ones in the order of their indices, as many as are wanted
+    int have = s_n;
+    __syncthreads();
+    for (int c0 = 0; c0 < V && have < k; c0 += kThreads) {
+      const int col = c0 + threadIdx.x;
+      const bool eq = col < V && order_key(as_f(x[col])) == at_thr;
+      const uint32_t votes = __ballot_sync(0xffffffff, eq);
+      if (threadIdx.x % 32 == 0) s_max[threadIdx.x / 32] = __popc(votes);
+      __syncthreads();
+      int before = have, all = 0;
+      for (int w = 0; w < kWarps; ++w) {
+        if (w < (int)threadIdx.x / 32) before += s_max[w];
+        all += s_max[w];
+      }
+      before += __popc(votes & ((1u << (threadIdx.x % 32)) - 1u));
+      if (eq && before < k) s_cand[before] = ((uint64_t)at_thr << 32) | (uint32_t)~(uint32_t)col;
+      have += all;
+      __syncthreads();
+    }
+    n = min(have, k);
+  }
+  for (int i = threadIdx.x; i < n; i += kThreads) {
+    const uint64_t mine = s_cand[i];
+    int rank = 0;
+    for (int j = 0; j < n; ++j) rank += s_cand[j] > mine;
+    if (rank < k) {
+      const int col = (int)~(uint32_t)mine;
+      values[row * k + rank] = as_f(x[col]);
+      indices[row * k + rank] = col;
+    }
+  }
+}
+
+// ------------------------------------------------------------ distillation loss
+struct DistillArgs {
+  const int64_t* labels;  // may be null
+  const float* top_values;
+  const void* top_indices;
+  bool idx64;
+  const float* top_lse;   // may be null: the teacher's entries alone are normalised
+  float* row_loss;
+  int64_t ld_in, ld_out;
+  int V, k;
+  bool vec;
+  float inv_tau, alpha, tau, grad_scale;
+};
+
+// One block per row:
+//   p_j   teacher's probability of entry j (of the whole vocabulary when its
+//         log-sum-exp is given, p_rest = 1 - sum p; else of the k entries)
+//   q     student's softmax(z / tau); q_rest its sum outside the entries
+//   loss  (1 - alpha) CE(z, label) + alpha tau^2 [sum p_j log(p_j / q_j) + p_rest log(p_rest / q_rest)]
+//   grad  grad_scale * dloss/dz, in the pass that reads the row again
+// The entries' columns are marked in a bitmap, so that the sum over the rest
+// is taken directly (1 - sum q_j would cancel when the student is sure) and
+// keeps a maximum of its own.
+template <typename T, typename TG>
+__global__ void __launch_bounds__(kThreads) distill_kernel(const T* __restrict__ logits, TG* __restrict__ grad,
+                                                           const DistillArgs a) {
+  extern __shared__ uint32_t bitmap[];
+  __shared__ float red[kWarps];
+  __shared__ float s_p[kMaxTop], s_z[kMaxTop];
+  __shared__ int s_i[kMaxTop];
+  __shared__ int s_marked, s_twice;
+  const int64_t row = blockIdx.x;
+  const int V = a.V, tid = threadIdx.x;
+  const T* x = logits + row * a.ld_in;
+  TG* gx = grad + row * a.ld_out;
+  const int lead = row_lead(row, a.ld_in, V, a.vec);
+  const int shift = (8 - lead % 8) % 8;  // bit of column c is c + shift: 8-element groups are whole bytes
+  const int64_t label = a.labels ? a.labels[row] : 0;
+  if (label < 0 || label >= V) {  // takes no part
+    const float zero[8] = {};
+    if (tid == 0) a.row_loss[row] = 0.f;
+    if (grad == nullptr) return;
+    for (int i = tid; i < lead; i += kThreads) put(gx + i, 0.f);
+    const int n8 = (V - lead) / 8;
+    for (int g = tid; g < n8; g += kThreads) store8(gx + lead + g * 8, zero);
+    for (int c = lead + n8 * 8 + tid; c < V; c += kThreads) put(gx + c, 0.f);
+    return;
+  }
+  const bool hard = a.labels != nullptr && a.alpha != 1.f;
+  const bool both = hard && a.inv_tau != 1.f;  // the label's softmax differs from the teacher's
+  const float c = a.inv_tau * kLog2e;
+
+  for (int i = tid; i < (V + 7 + 31) / 32; i += kThreads) bitmap[i] = 0;
+  if (tid == 0) s_marked = s_twice = 0;
+  __syncthreads();
+  // the teacher's entries
+  float tmax = -FLT_MAX;
+  for (int j = tid; j < a.k; j += kThreads) {
+    const int64_t i = a.idx64 ? static_cast<const int64_t*>(a.top_indices)[row * a.k + j]
+                              : static_cast<const int*>(a.top_indices)[row * a.k + j];
+    const bool in = i >= 0 && i < V;
+    const float t = a.top_values[row * a.k + j] * a.inv_tau;
+    s_i[j] = in ? (int)i : -1;
+    s_p[j] = in ? t : -INFINITY;
+    if (in) {
+      s_z[j] = as_f(x[i]);
+      const uint32_t bit = (uint32_t)i + shift, m = 1u << (bit & 31);
+      if (atomicOr(&bitmap[bit >> 5], m) & m)
+        s_twice = 1;
+      else
+        atomicAdd(&s_marked, 1);
+      tmax = fmaxf(tmax, t);
+    }
+  }
+  float tlse;
+  if (a.top_lse != nullptr) {
+    tlse = a.top_lse[row];
+  } else {
+    tmax = block_max(tmax, red);
+    float s = 0.f;
+    for (int j = tid; j < a.k; j += kThreads)
+      if (s_i[j] >= 0) s += ex2((s_p[j] - tmax) * kLog2e);
+    s = block_sum(s, red);
+    tlse = tmax + logf(s);  // -inf without entries; s_p stays -inf there and gives p = 0 below
+  }
+  __syncthreads();
+
+  // the row: sums over the columns outside the set, and over all at temperature 1 where the label needs it
+  RunningSum rest, full;
+  for_row(x, V, lead, [&](int col, const float* v, auto n) {
+    constexpr int N = decltype(n)::value;
+    const uint32_t bit = (uint32_t)(col + shift);
+    const uint32_t marks = (bitmap[bit >> 5] >> (bit & 31)) & ((1u << N) - 1u);
+    float vm = v[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) vm = fmaxf(vm, v[i]);
+    if (both) {
+      full.raise(vm, kLog2e);
+#pragma unroll
+      for (int i = 0; i < N; ++i) full.s += ex2((v[i] - full.m) * kLog2e);
+    }
+    if (marks == 0) {
+      rest.raise(vm, c);
+#pragma unroll
+      for (int i = 0; i < N; ++i) rest.s += ex2((v[i] - rest.m) * c);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (!((marks >> i) & 1u)) rest.add(v[i], c);
+    }
+  });
+  rest.join(c, red);
+  if (both) full.join(kLog2e, red);
+
+  // the set's own part of the student's sum
+  const bool twice = s_twice != 0;
+  auto first_of = [&](int j) {  // whether entry j is the first with its index
+    if (twice)
+      for (int i = 0; i < j; ++i)
+        if (s_i[i] == s_i[j]) return false;
+    return true;
+  };
+  float zmax = -FLT_MAX;
+  for (int j = tid; j < a.k; j += kThreads)
+    if (s_i[j] >= 0) zmax = fmaxf(zmax, s_z[j]);
+  const float m = fmaxf(block_max(zmax, red), rest.m);
+  float set = 0.f, psum = 0.f;
+  for (int j = tid; j < a.k; j += kThreads)
+    if (s_i[j] >= 0) {
+      if (first_of(j)) set += ex2((s_z[j] - m) * c);
+      psum += s_p[j] == -INFINITY ? 0.f : ex2((s_p[j] - tlse) * kLog2e);
+    }
+  set = block_sum(set, red);
+  psum = block_sum(psum, red);
+  const float B = set + rest.s * ex2((rest.m - m) * c);
+  const float logB = logf(B), logz = m * a.inv_tau + logB;  // log of the sum of exp(z / tau)
+  const bool has_rest = a.top_lse != nullptr && s_marked < V;
+  const float p_rest = has_rest ? fmaxf(1.f - psum, 0.f) : 0.f;
+
+  float kl = 0.f;
+  for (int j = tid; j < a.k; j += kThreads)
+    if (s_i[j] >= 0 && s_p[j] != -INFINITY) {
+      const float logp = s_p[j] - tlse, p = ex2(logp * kLog2e);
+      if (p > 0.f) kl += p * (logp - (s_z[j] * a.inv_tau - logz));
+      if (p != p) kl = p;
+    }
+  kl = block_sum(kl, red);
+  if (p_rest > 0.f) kl += p_rest * (logf(p_rest) - (rest.m * a.inv_tau + logf(rest.s) - logz));
+  const float zy = hard ? as_f(x[label]) : 0.f;
+  const float log_full = !hard ? 0.f : both ? full.m + logf(full.s) : logz;
+  if (tid == 0)
+    a.row_loss[row] = (a.alpha > 0.f ? a.alpha * a.tau * a.tau * kl : 0.f) +
+                      (hard ? (1.f - a.alpha) * (log_full - zy) : 0.f);
+
+  if (grad == nullptr) return;
+  // gradient. Outside the set: w_hard softmax(z) + w_soft (q - p_rest q / q_rest)
+  const float w_soft = a.grad_scale * a.alpha * a.tau * (psum + p_rest == 0.f ? 0.f : 1.f);
+  const float w_hard = hard ? a.grad_scale * (1.f - a.alpha) : 0.f;
+  const float inv_B = 1.f / B;
+  float f_rest = 0.f;  // factor of 2^(c (z - rest.m))
+  if (rest.s > 0.f || rest.s != rest.s)
+    f_rest = w_soft * (ex2((rest.m - m) * c) * inv_B - p_rest / rest.s) +
+             (both ? 0.f : w_hard * ex2((rest.m - m) * c) * inv_B);
+  const float f_full = both ? w_hard / full.s : 0.f;
+  __syncthreads();
+  for_row(x, V, lead, [&](int col, const float* v, auto n) {
+    constexpr int N = decltype(n)::value;
+    float g[8];
+#pragma unroll
+    for (int i = 0; i < N; ++i) g[i] = f_rest * ex2((v[i] - rest.m) * c);
+    if (both) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) g[i] += f_full * ex2((v[i] - full.m) * kLog2e);
+    }
+    if (N == 8)
+      store8(gx + col, g);
+    else
+      put(gx + col, g[0]);
+  });
+  __syncthreads();
+  // the set's columns and the label's
+  auto at_label = [&](float z) { return both ? ex2((z - full.m) * kLog2e) / full.s : ex2((z - m) * c) * inv_B; };
+  for (int j = tid; j < a.k; j += kThreads) {
+    const int i = s_i[j];
+    if (i < 0 || !first_of(j)) continue;
+    float p = 0.f;
+    for (int e = j; e < (twice ? a.k : j + 1); ++e)
+      if (s_i[e] == i && s_p[e] != -INFINITY) p += ex2((s_p[e] - tlse) * kLog2e);
+    float g = w_soft * (ex2((s_z[j] - m) * c) * inv_B - p);
+    if (hard) g += w_hard * (at_label(s_z[j]) - (i == label ? 1.f : 0.f));
+    put(gx + i, g);
+  }
+  if (hard && tid == 0) {
+    const uint32_t bit = (uint32_t)label + shift;
+    if (!((bitmap[bit >> 5] >> (bit & 31)) & 1u)) {
+      const float q = ex2((zy - m) * c) * inv_B;
+      const float r = rest.s > 0.f ? p_rest * ex2((zy - rest.m) * c) / rest.s : 0.f;
+      put(gx + label, w_soft * (q - r) + w_hard * (at_label(zy) - 1.f));
+    }
+  }
+}
+
+bool aligned8(const at::Tensor& t) {
+  return reinterpret_cast<uintptr_t>(t.data_ptr()) % (8 * t.element_size()) == 0;
+}
+
+void check_rows(const at::Tensor& t, const char* op) {
+  TORCH_CHECK(t.is_cuda() && t.dim() == 2 && (t.size(1) <= 1 || t.stride(1) == 1),
+              "dion_b200 ", op, ": logits [T, V] on a CUDA device with contiguous rows");
+  TORCH_CHECK(t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf || t.scalar_type() == at::kFloat,
+              "dion_b200 ", op, ": bf16, fp16 or fp32 logits");
+  TORCH_CHECK(t.size(0) < (1ll << 31) && t.size(1) >= 1 && t.size(1) <= (1 << 20), "dion_b200 ", op,
+              ": 1 <= V <= 2^20 and T < 2^31");
+}
+
+void check_out(const at::Tensor& t, const at::Tensor& like, at::ScalarType dtype, at::IntArrayRef shape,
+               const char* what) {
+  TORCH_CHECK(t.is_cuda() && t.device() == like.device() && t.scalar_type() == dtype && t.sizes() == shape &&
+                  t.is_contiguous(),
+              "dion_b200 ", what, ": a contiguous tensor of the stated shape and type on the logits' device");
+}
+
+template <typename F>
+void by_type(at::ScalarType t, F f) {
+  if (t == at::kBFloat16)
+    f(__nv_bfloat16{});
+  else if (t == at::kHalf)
+    f(__half{});
+  else
+    f(float{});
+}
+
+}  // namespace
+
+// values / indices [T, k]: the k largest logits of each row in falling order
+// (equal ones by the lower index); lse [T]: log sum exp(logits / tau)
+void top_logits(const at::Tensor& logits, at::Tensor& values, at::Tensor& indices, at::Tensor& lse, double tau) {
+  check_rows(logits, "top_logits");
+  const int64_t T = logits.size(0);
+  const int V = (int)logits.size(1), k = (int)values.size(1);
+  TORCH_CHECK(k >= 1 && k <= std::min(V, kMaxTop), "dion_b200 top_logits: 1 <= k <= min(V, 1024)");
+  TORCH_CHECK(tau > 0, "dion_b200 top_logits: temperature > 0");
+  check_out(values, logits, at::kFloat, {T, k}, "top_logits values");
+  check_out(indices, logits, at::kLong, {T, k}, "top_logits indices");
+  check_out(lse, logits, at::kFloat, {T}, "top_logits lse");
+  if (T == 0) return;
+  c10::cuda::CUDAGuard guard(logits.device());
+  auto s = at::cuda::getCurrentCUDAStream();
+  by_type(logits.scalar_type(), [&](auto tag) {
+    using E = decltype(tag);
+    auto launch = [&](auto g) {
+      top_logits_kernel<E, decltype(g)::value><<<(unsigned)T, kThreads, 0, s>>>(
+          static_cast<const E*>(logits.data_ptr()), logits.stride(0), V, k, aligned8(logits), (float)(kLog2e / tau),
+          values.data_ptr<float>(), indices.data_ptr<int64_t>(), lse.data_ptr<float>());
+    };
+    // at least twice as many groups as entries keeps the candidates near 1.4 k
+    if (k <= kThreads / 2)
+      launch(std::integral_constant<int, 1>{});
+    else
+      launch(std::integral_constant<int, 4>{});
+  });
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  note_launch();
+}
+
+// loss: the sum of the rows' losses; grad (optional): grad_scale * d loss / d logits
+void distill_fwd_bwd(const at::Tensor& logits, const c10::optional<at::Tensor>& labels, const at::Tensor& top_values,
+                     const at::Tensor& top_indices, const c10::optional<at::Tensor>& top_lse,
+                     const c10::optional<at::Tensor>& grad, at::Tensor& loss, double tau, double alpha, double grad_scale) {
+  check_rows(logits, "distill");
+  const int64_t T = logits.size(0);
+  const int V = (int)logits.size(1), k = (int)top_values.size(1);
+  TORCH_CHECK(k >= 1 && k <= kMaxTop, "dion_b200 distill: 1 to 1024 teacher entries per row");
+  TORCH_CHECK(tau > 0, "dion_b200 distill: temperature > 0");
+  check_out(top_values, logits, at::kFloat, {T, k}, "distill top_values");
+  TORCH_CHECK(top_indices.scalar_type() == at::kLong || top_indices.scalar_type() == at::kInt,
+              "dion_b200 distill: int32 or int64 top_indices");
+  check_out(top_indices, logits, top_indices.scalar_type(), {T, k}, "distill top_indices");
+  if (labels.has_value()) check_out(*labels, logits, at::kLong, {T}, "distill labels");
+  if (top_lse.has_value()) check_out(*top_lse, logits, at::kFloat, {T}, "distill top_lse");
+  const auto gtype = grad.has_value() ? grad->scalar_type() : logits.scalar_type();
+  if (grad.has_value()) {
+    TORCH_CHECK(gtype == logits.scalar_type() ||
+                    (logits.scalar_type() == at::kFloat && (gtype == at::kBFloat16 || gtype == at::kHalf)),
+                "dion_b200 distill: gradient in the logits' type, or bf16 or fp16 of fp32 logits");
+    check_out(*grad, logits, gtype, {T, V}, "distill grad");
+  }
+  c10::cuda::CUDAGuard guard(logits.device());
+  if (T == 0) {
+    loss.zero_();
+    return;
+  }
+  auto rows = at::empty({T}, logits.options().dtype(at::kFloat));
+  DistillArgs a;
+  a.labels = labels.has_value() ? labels->data_ptr<int64_t>() : nullptr;
+  a.top_values = top_values.data_ptr<float>();
+  a.top_indices = top_indices.data_ptr();
+  a.idx64 = top_indices.scalar_type() == at::kLong;
+  a.top_lse = top_lse.has_value() ? top_lse->data_ptr<float>() : nullptr;
+  a.row_loss = rows.data_ptr<float>();
+  a.ld_in = logits.stride(0);
+  a.ld_out = V;
+  a.V = V;
+  a.k = k;
+  // 8-element groups of the logits and of the gradient have to start together
+  a.vec = aligned8(logits) && (!grad.has_value() || (aligned8(*grad) && (T == 1 || a.ld_in % 8 == a.ld_out % 8)));
+  a.inv_tau = (float)(1.0 / tau);
+  a.tau = (float)tau;
+  a.alpha = (float)alpha;
+  a.grad_scale = (float)grad_scale;
+  const size_t smem = ((size_t)V + 7 + 31) / 32 * 4;
+  auto s = at::cuda::getCurrentCUDAStream();
+  by_type(logits.scalar_type(), [&](auto tag) {
+    using E = decltype(tag);
+    by_type(gtype, [&](auto gtag) {
+      using G = decltype(gtag);
+      if constexpr (std::is_same_v<E, G> || std::is_same_v<E, float>) {
+        auto kern = distill_kernel<E, G>;
+        C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        kern<<<(unsigned)T, kThreads, smem, s>>>(static_cast<const E*>(logits.data_ptr()),
+                                                 grad.has_value() ? static_cast<G*>(grad->data_ptr()) : nullptr, a);
+      }
+    });
+  });
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  note_launch();
+  at::sum_out(loss, rows, 0);
+}
+
+}  // namespace bdion

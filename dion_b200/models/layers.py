@@ -1,5 +1,7 @@
 """Building blocks of the Llama model: RMSNorm, rotary embedding, causal
-grouped-query attention, SwiGLU and a memory-lean linear + cross-entropy.
+grouped-query attention (full, or with a sliding window and visible first
+tokens), SwiGLU, a memory-lean linear + cross-entropy, and distillation from a
+teacher's top logits (their selection and the loss, both behind the LM head).
 
 Each op uses the package's fused sm_100a kernel for CUDA bf16 inputs when
 the extension provides it, and plain PyTorch otherwise (CPU runs and
@@ -7,7 +9,7 @@ autograd reference)."""
 from __future__ import annotations
 
 import math
-from typing import Tuple
+from typing import Optional, Tuple
 
 import torch
 import torch.nn as nn
@@ -15,14 +17,20 @@ import torch.nn.functional as F
 
 from .. import ops
 from ..ops import fused as _fused
+from ..ops.fused import TopLogits
 
 __all__ = [
     "RMSNorm",
     "rope_table",
     "apply_rope",
     "causal_attention",
+    "window_attention",
     "swiglu",
     "linear_cross_entropy",
+    "TopLogits",
+    "top_logits",
+    "linear_top_logits",
+    "linear_distillation",
 ]
 
 
@@ -80,6 +88,25 @@ def causal_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> torch
     return o.transpose(1, 2)
 
 
+def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: int, sinks: int = 0) -> torch.Tensor:
+    """Causal attention over the last ``window`` positions and the first
+    ``sinks`` ones: i sees j <= i where i - j < window or j < sinks.
+    q: [b, s, hq, d], k/v: [b, s, hkv, d] -> [b, s, hq, d]."""
+    if _fused.window_enabled(q):
+        return _fused.window_attention(q, k, v, window, sinks)
+    _fused._check_window(q, k, v, window, sinks)
+    return _window_ref(q, k, v, window, sinks)
+
+
+def _window_ref(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: int, sinks: int) -> torch.Tensor:
+    pos = torch.arange(q.shape[1], device=q.device)
+    i, j = pos[:, None], pos[None, :]
+    seen = (j <= i) & ((i - j < window) | (j < sinks))
+    qt, kt, vt = q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2)
+    o = F.scaled_dot_product_attention(qt, kt, vt, attn_mask=seen, enable_gqa=qt.shape[1] != kt.shape[1])
+    return o.transpose(1, 2)
+
+
 def swiglu(a: torch.Tensor, b: torch.Tensor) -> torch.Tensor:
     if _fused.enabled(a):
         return _fused.swiglu(a, b)
@@ -131,3 +158,87 @@ def linear_cross_entropy(h: torch.Tensor, W: torch.Tensor, labels: torch.Tensor,
             total += loss_c
         return total / T
     return _LinearCE.apply(h2, W, lab, chunk)
+
+
+def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0) -> TopLogits:
+    """The k largest logits of every row of [T, V] with their columns, and the
+    row's log-sum-exp at ``temperature`` (see :func:`dion_b200.ops.fused.top_logits`)."""
+    return _fused.top_logits(logits, k, temperature)
+
+
+def _head_logits(h: torch.Tensor, W: torch.Tensor) -> torch.Tensor:
+    """h W^T in fp32. A bf16 logit of 8 is off by up to 2^-6, and a softmax
+    turns that into as large a relative error of its probability."""
+    if h.dtype == torch.float32:
+        return h @ W.t()
+    if h.is_cuda:
+        return torch.mm(h, W.t(), out_dtype=torch.float32)
+    return h.float() @ W.float().t()
+
+
+@torch.no_grad()
+def linear_top_logits(h: torch.Tensor, W: torch.Tensor, k: int, temperature: float = 1.0,
+                      chunk: int = 4096) -> TopLogits:
+    """``top_logits`` of the LM head's h @ W^T, ``chunk`` tokens at a time, so
+    that the [tokens, vocab] logits never exist at once. h: [..., dim]; the
+    results are [..., k] and [...]."""
+    h2 = h.reshape(-1, h.shape[-1])
+    parts = [_fused.top_logits(_head_logits(c, W), k, temperature) for c in h2.split(max(1, chunk))]
+    values, indices, lse = (torch.cat(p) if len(p) > 1 else p[0] for p in zip(*parts))
+    lead = h.shape[:-1]
+    return TopLogits(values.view(*lead, k), indices.view(*lead, k), lse.view(lead))
+
+
+class _LinearDistillation(torch.autograd.Function):
+    """Mean distillation loss behind the LM head, its gradient computed chunk by
+    chunk during forward as in :class:`_LinearCE`. The chunk's gradient of the
+    logits is unscaled (a sum, not a mean) in h's dtype; the division by the
+    number of rows in the loss, known on the device only, is applied with the
+    incoming gradient in backward."""
+
+    @staticmethod
+    def forward(ctx, h, W, labels, top_values, top_indices, top_lse, temperature, alpha, chunk, need_grad):
+        T, V = h.shape[0], W.shape[0]
+        total = torch.zeros((), device=h.device, dtype=torch.float32)
+        grad_h = torch.empty_like(h) if need_grad else None
+        grad_W = torch.zeros(W.shape, device=W.device, dtype=torch.float32) if need_grad else None
+        for s in range(0, T, chunk):
+            e = min(T, s + chunk)
+            hc = h[s:e]
+            loss_c, g = _fused.distillation_fwd_bwd(
+                _head_logits(hc, W), None if labels is None else labels[s:e], top_values[s:e], top_indices[s:e],
+                None if top_lse is None else top_lse[s:e], temperature, alpha, 1.0, h.dtype, need_grad)
+            total += loss_c
+            if need_grad:
+                grad_h[s:e] = g @ W
+                if h.is_cuda and h.dtype == torch.bfloat16:
+                    ops.matmul(g.t(), hc, out=grad_W, C=grad_W, beta=1.0)
+                else:
+                    grad_W += g.t().float() @ hc.float()
+        n = max(T, 1) if labels is None else ((labels >= 0) & (labels < V)).sum().clamp_min(1).float()
+        ctx.n = n
+        ctx.save_for_backward(grad_h, grad_W)
+        ctx.W_dtype = W.dtype
+        return total / n
+
+    @staticmethod
+    def backward(ctx, go):
+        grad_h, grad_W = ctx.saved_tensors
+        f = go / ctx.n
+        return (grad_h * f, (grad_W * f).to(ctx.W_dtype)) + (None,) * 8
+
+
+def linear_distillation(h: torch.Tensor, W: torch.Tensor, labels: Optional[torch.Tensor], top_values: torch.Tensor,
+                        top_indices: torch.Tensor, top_lse: Optional[torch.Tensor] = None, temperature: float = 1.0,
+                        alpha: float = 1.0, chunk: int = 4096) -> torch.Tensor:
+    """Mean distillation loss of the student logits h @ W^T against a teacher's
+    top logits (see :func:`dion_b200.ops.fused.distillation_fwd_bwd` for the
+    loss). h: [..., dim], labels: [...] or None, top_values / top_indices:
+    [..., k], top_lse: [...]. Rows whose label is outside [0, V) are left out
+    of the sum and of the mean; the loss is 0 if that leaves none."""
+    h2 = h.reshape(-1, h.shape[-1])
+    flat = lambda t: None if t is None else t.reshape(-1)  # noqa: E731
+    k = top_values.shape[-1]
+    need = torch.is_grad_enabled() and (h.requires_grad or W.requires_grad)
+    return _LinearDistillation.apply(h2, W, flat(labels), top_values.reshape(-1, k), top_indices.reshape(-1, k),
+                                     flat(top_lse), temperature, alpha, max(1, chunk), need)

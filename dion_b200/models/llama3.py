@@ -8,9 +8,10 @@ hybrid optimizer container see the same names as with the reference's model
 same way).
 
 Compute is bf16 on the tensor cores: cuBLAS for the plain projections,
-torch SDPA (flash/cuDNN) for attention with native grouped-query heads, and
-the package's fused kernels for RMSNorm, rotary embedding, SwiGLU and the
-chunked cross-entropy when they are available on the device.
+torch SDPA (flash/cuDNN) for full attention with native grouped-query heads,
+and the package's fused kernels for RMSNorm, rotary embedding, sliding-window
+attention, SwiGLU, the chunked cross-entropy and the distillation loss when
+they are available on the device.
 """
 from __future__ import annotations
 
@@ -23,6 +24,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from . import layers as L
+from ..ops import has_ext
 from ..parallel.sp import sp_column_linears, sp_row_linear
 
 __all__ = ["Llama3Config", "Transformer", "LLAMA3_CONFIGS", "llama3_config"]
@@ -42,6 +44,10 @@ class Llama3Config:
     rope_theta: float = 500000.0
     max_seq_len: int = 8192
     depth_init: bool = True
+    # sliding-window attention: every position sees the last attn_window ones and
+    # the first attn_sinks ones (None: all earlier positions)
+    attn_window: Optional[int] = None
+    attn_sinks: int = 0
 
     def hidden_dim(self) -> int:
         if self.ffn_dim is not None:
@@ -72,6 +78,8 @@ class Llama3Config:
     def flops_per_token(self, seq_len: int) -> int:
         """Training FLOPs per token: 6 * non-embedding params + attention (12*l*h*q*t)."""
         nparams = self.num_params(include_embedding=False)
+        if self.attn_window is not None:
+            seq_len = min(seq_len, self.attn_window + self.attn_sinks)
         return 6 * nparams + 12 * self.n_layers * self.n_heads * self.head_dim * seq_len
 
 
@@ -104,11 +112,17 @@ class Attention(nn.Module):
         self.n_heads = cfg.n_heads
         self.n_kv_heads = cfg.kv_heads
         self.head_dim = cfg.head_dim
+        self.window, self.sinks = cfg.attn_window, cfg.attn_sinks
         self.wq = nn.Linear(cfg.dim, cfg.n_heads * self.head_dim, bias=False)
         self.wk = nn.Linear(cfg.dim, self.n_kv_heads * self.head_dim, bias=False)
         self.wv = nn.Linear(cfg.dim, self.n_kv_heads * self.head_dim, bias=False)
         self.wo = nn.Linear(cfg.n_heads * self.head_dim, cfg.dim, bias=False)
         self.sp = None  # sequence-parallel TP group (parallel/sp.py), set by apply_tp
+
+    def _attend(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> torch.Tensor:
+        if self.window is None:
+            return L.causal_attention(q, k, v)
+        return L.window_attention(q, k, v, self.window, self.sinks)
 
     def forward(self, x: torch.Tensor, rope: torch.Tensor) -> torch.Tensor:
         if self.sp is not None:
@@ -119,7 +133,7 @@ class Attention(nn.Module):
             k = k.view(bs, seqlen, -1, self.head_dim)
             v = v.view(bs, seqlen, -1, self.head_dim)
             q, k = L.apply_rope(q, k, rope)
-            o = L.causal_attention(q, k, v)
+            o = self._attend(q, k, v)
             return sp_row_linear(self.sp, o.reshape(bs * seqlen, -1), self.wo.weight)
         bs, seqlen, _ = x.shape
         # -1 heads: under tensor parallelism each rank holds n_heads / tp of them
@@ -127,7 +141,7 @@ class Attention(nn.Module):
         k = self.wk(x).view(bs, seqlen, -1, self.head_dim)
         v = self.wv(x).view(bs, seqlen, -1, self.head_dim)
         q, k = L.apply_rope(q, k, rope)
-        o = L.causal_attention(q, k, v)  # [bs, seq, heads, hd]
+        o = self._attend(q, k, v)  # [bs, seq, heads, hd]
         return self.wo(o.reshape(bs, seqlen, -1))
 
 
@@ -160,6 +174,8 @@ def _sac_context():
         names = ("mm", "addmm", "bmm", "_scaled_dot_product_flash_attention", "_scaled_dot_product_cudnn_attention",
                  "_scaled_dot_product_efficient_attention")
         _SAC_SAVE = {getattr(aten, n).default for n in names if hasattr(aten, n)}
+        if has_ext():
+            _SAC_SAVE.add(torch.ops.dion_b200.window_attention_fwd.default)
 
     def policy(ctx, op, *args, **kwargs):
         return CheckpointPolicy.MUST_SAVE if op in _SAC_SAVE else CheckpointPolicy.PREFER_RECOMPUTE
@@ -253,12 +269,21 @@ class Transformer(nn.Module):
         )
 
     def forward(self, tokens: torch.Tensor, labels: Optional[torch.Tensor] = None,
-                return_hidden: bool = False) -> torch.Tensor:
+                return_hidden: bool = False, teacher: Optional[L.TopLogits] = None, temperature: float = 1.0,
+                alpha: float = 1.0, top_k: int = 0):
         """Logits, or with ``labels`` the mean next-token cross-entropy computed
         chunk-wise without materialising fp32 logits. (The loss lives in
-        ``forward`` so FSDP's root hooks unshard the LM head for it.)"""
+        ``forward`` so FSDP's root hooks unshard the LM head for it.)
+
+        With ``teacher`` (a teacher's top logits for these tokens) the mean
+        distillation loss at ``temperature``, ``alpha`` of it against the
+        teacher and the rest against ``labels``; with ``top_k`` this model's
+        own top logits (:class:`~dion_b200.models.layers.TopLogits`)."""
         seqlen = tokens.shape[1]
         sp = self.sp
+        if sp is not None and (teacher is not None or top_k):
+            raise ValueError("distillation has no sequence-parallel path: each rank holds other tokens, so the mean "
+                             "over the rows that take part is not known to it (sequence_parallel=False)")
         if sp is not None:
             # sequence parallelism: this rank embeds and carries its shard of the flattened tokens
             sp.batch_shape = (tokens.shape[0], seqlen)
@@ -269,6 +294,10 @@ class Transformer(nn.Module):
         for layer in self.layers.values():
             h = layer(h, rope)
         h = self.norm(h)
+        if top_k:
+            return L.linear_top_logits(h, self.output.weight, top_k, temperature)
+        if teacher is not None:
+            return L.linear_distillation(h, self.output.weight, labels, *teacher, temperature=temperature, alpha=alpha)
         if labels is not None:
             if sp is not None:
                 # this rank's share of the mean loss over all N tokens (the TP
@@ -282,3 +311,12 @@ class Transformer(nn.Module):
 
     def loss(self, tokens: torch.Tensor, labels: torch.Tensor) -> torch.Tensor:
         return self(tokens, labels)
+
+    @torch.no_grad()
+    def top_logits(self, tokens: torch.Tensor, k: int, temperature: float = 1.0) -> L.TopLogits:
+        """This model's k largest logits at every position ([b, s, k]), as a teacher gives them."""
+        return self(tokens, top_k=k, temperature=temperature)
+
+    def distillation_loss(self, tokens: torch.Tensor, labels: Optional[torch.Tensor], teacher: L.TopLogits,
+                          temperature: float = 1.0, alpha: float = 1.0) -> torch.Tensor:
+        return self(tokens, labels, teacher=teacher, temperature=temperature, alpha=alpha)

@@ -1,4 +1,5 @@
-"""Fused model-side ops (RMSNorm, rotary embedding, SwiGLU, cross-entropy).
+"""Fused model-side ops (RMSNorm, rotary embedding, sliding-window attention,
+SwiGLU, cross-entropy, distillation from a teacher's top logits).
 
 The CUDA versions are sm_100a kernels of the ``dion_b200._C`` extension,
 wrapped in autograd Functions; ``enabled(x)`` says whether a tensor takes the
@@ -7,7 +8,7 @@ fused path (CUDA, bf16, extension present, not disabled through
 from __future__ import annotations
 
 import os
-from typing import Tuple
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 import torch.nn.functional as F
@@ -112,6 +113,63 @@ def rope(q: torch.Tensor, k: torch.Tensor, table: torch.Tensor) -> Tuple[torch.T
     return _Rope.apply(q, k, table)
 
 
+# ---------------------------------------------------------------- sliding-window attention
+def _check_window(q, k, v, window, sinks) -> None:
+    if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape:
+        raise ValueError(f"window_attention: q [b, s, hq, d] and k, v [b, s, hkv, d], got {tuple(q.shape)}, "
+                         f"{tuple(k.shape)}, {tuple(v.shape)}")
+    if q.shape[:2] != k.shape[:2] or q.shape[3] != k.shape[3]:
+        raise ValueError(f"window_attention: q {tuple(q.shape)} and k {tuple(k.shape)} differ in batch, positions or "
+                         "head dimension")
+    if k.shape[2] < 1 or q.shape[2] % k.shape[2]:
+        raise ValueError(f"window_attention: {q.shape[2]} query heads do not divide over {k.shape[2]} key heads")
+    if not (q.dtype == k.dtype == v.dtype) or not (q.device == k.device == v.device):
+        raise ValueError("window_attention: q, k and v of one type on one device")
+    if int(window) < 1 or int(sinks) < 0:
+        raise ValueError(f"window_attention: window >= 1 and sinks >= 0, got {window} and {sinks}")
+
+
+def window_enabled(q: torch.Tensor) -> bool:
+    """Window attention kernels: bf16 or fp16, head dimension a multiple of 8 up to 128."""
+    return ((not _DISABLED) and q.is_cuda and q.dtype in (torch.bfloat16, torch.float16) and q.shape[-1] % 8 == 0
+            and 8 <= q.shape[-1] <= 128 and has_ext() and hasattr(ext(), "window_attention_fwd"))
+
+
+def _tile_rows(x: torch.Tensor) -> torch.Tensor:
+    """x itself where the kernels' tiled copies can read it in place (head dim
+    contiguous, every other stride a positive multiple of 16 bytes, aligned
+    base), a packed copy otherwise."""
+    st = x.stride()
+    ok = x.data_ptr() % 16 == 0 and st[3] == 1 and all(n == 1 or (t > 0 and t % 8 == 0) for n, t in zip(x.shape[:3], st))
+    return x if ok else x.clone(memory_format=torch.contiguous_format)
+
+
+class _WindowAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, window, sinks):
+        q, k, v = _tile_rows(q), _tile_rows(k), _tile_rows(v)
+        o, lse = torch.ops.dion_b200.window_attention_fwd(q, k, v, window, sinks)
+        ctx.save_for_backward(q, k, v, o, lse)
+        ctx.window, ctx.sinks = window, sinks
+        return o
+
+    @staticmethod
+    def backward(ctx, go):
+        q, k, v, o, lse = ctx.saved_tensors
+        dq, dk, dv = ext().window_attention_bwd(_tile_rows(go), q, k, v, o, lse, ctx.window, ctx.sinks)
+        return dq, dk, dv, None, None
+
+
+def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: int, sinks: int = 0) -> torch.Tensor:
+    """Causal attention in which position i sees position j <= i where
+    ``i - j < window`` or ``j < sinks``. q: [b, s, hq, d], k/v: [b, s, hkv, d]
+    (query head h reads key head h // (hq / hkv)) -> [b, s, hq, d]; scores are
+    scaled by 1 / sqrt(d). Inputs are finite: a non-finite key or value also
+    reaches rows up to a tile of 128 beyond those that see it."""
+    _check_window(q, k, v, window, sinks)
+    return _WindowAttention.apply(q, k, v, int(window), int(sinks))
+
+
 # ---------------------------------------------------------------- SwiGLU
 class _SwiGLU(torch.autograd.Function):
     @staticmethod
@@ -150,3 +208,135 @@ def cross_entropy_fwd_bwd(logits: torch.Tensor, labels: torch.Tensor, grad_scale
     p = torch.exp(lf - lse.unsqueeze(1))
     p.scatter_add_(1, labels.view(-1, 1), torch.full_like(picked.view(-1, 1), -1.0))
     return loss, (p * grad_scale).to(logits.dtype)
+
+
+# ---------------------------------------------------------------- distillation
+class TopLogits(NamedTuple):
+    """A teacher's largest logits per row: values (fp32) and indices [T, k] in
+    falling order, and log sum exp(logits / temperature) of the whole row [T]."""
+
+    values: torch.Tensor
+    indices: torch.Tensor
+    lse: Optional[torch.Tensor]
+
+
+MAX_TOP = 1024
+
+
+def _rows_enabled(x: torch.Tensor) -> bool:
+    return ((not _DISABLED) and x.is_cuda and x.dtype in (torch.bfloat16, torch.float16, torch.float32) and has_ext()
+            and hasattr(ext(), "top_logits"))
+
+
+def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0) -> TopLogits:
+    """The k largest logits of every row of [T, V] in falling order (equal ones
+    by the lower index, a NaN above all), with the row's log-sum-exp at
+    ``temperature``. 1 <= k <= min(V, 1024)."""
+    if logits.dim() != 2:
+        raise ValueError(f"top_logits: logits [T, V], got {tuple(logits.shape)}")
+    T, V = logits.shape
+    if not 1 <= k <= min(V, MAX_TOP):
+        raise ValueError(f"top_logits: 1 <= k <= min(V, {MAX_TOP}), got k = {k} with V = {V}")
+    if not temperature > 0:
+        raise ValueError(f"top_logits: temperature > 0, got {temperature}")
+    if _rows_enabled(logits):
+        x = logits if logits.stride(1) == 1 or V == 1 else logits.contiguous()
+        values = torch.empty(T, k, device=x.device, dtype=torch.float32)
+        indices = torch.empty(T, k, device=x.device, dtype=torch.int64)
+        lse = torch.empty(T, device=x.device, dtype=torch.float32)
+        ext().top_logits(x, values, indices, lse, float(temperature))
+        return TopLogits(values, indices, lse)
+    x = logits.float()
+    indices = (x + 0.0).sort(dim=1, descending=True, stable=True).indices[:, :k].contiguous()
+    return TopLogits(x.gather(1, indices), indices, torch.logsumexp(x / temperature, dim=1))
+
+
+def distillation_fwd_bwd(logits: torch.Tensor, labels: Optional[torch.Tensor], top_values: torch.Tensor,
+                         top_indices: torch.Tensor, top_lse: Optional[torch.Tensor] = None, temperature: float = 1.0,
+                         alpha: float = 1.0, grad_scale: float = 1.0, grad_dtype: Optional[torch.dtype] = None,
+                         need_grad: bool = True):
+    """Sum over the rows of
+    ``(1 - alpha) CE(logits, label) + alpha temperature^2 KL(teacher || softmax(logits / temperature))``
+    (fp32 scalar), and grad_scale times its gradient with respect to the logits
+    (in their dtype, or ``grad_dtype`` for fp32 logits; None without ``need_grad``).
+
+    logits: [T, V]; top_values / top_indices: [T, k], k <= 1024, the teacher's
+    logits and their columns (int32 or int64; a column outside [0, V) marks an
+    unused entry, a column may come twice). ``top_lse`` [T] is the teacher's
+    log-sum-exp at the temperature: the teacher's probability outside its
+    entries then counts as one outcome more, held against the student's
+    probability outside them. Without it the entries are normalised among
+    themselves. labels: int64 [T] (a row whose label is outside [0, V) is left
+    out: loss and gradient 0), or None with alpha = 1."""
+    if logits.dim() != 2 or top_values.dim() != 2 or top_values.shape != top_indices.shape:
+        raise ValueError(f"distillation: logits [T, V], top_values and top_indices [T, k], got {tuple(logits.shape)}, "
+                         f"{tuple(top_values.shape)}, {tuple(top_indices.shape)}")
+    T, V = logits.shape
+    k = top_values.shape[1]
+    if top_values.shape[0] != T or not 1 <= k <= MAX_TOP:
+        raise ValueError(f"distillation: {T} rows of 1 to {MAX_TOP} teacher entries, got {tuple(top_values.shape)}")
+    if top_indices.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"distillation: int32 or int64 top_indices, got {top_indices.dtype}")
+    for name, t in (("labels", labels), ("top_lse", top_lse)):
+        if t is not None and t.shape != (T,):
+            raise ValueError(f"distillation: {name} [{T}], got {tuple(t.shape)}")
+    if not temperature > 0 or not 0 <= alpha <= 1:
+        raise ValueError(f"distillation: temperature > 0 and 0 <= alpha <= 1, got {temperature} and {alpha}")
+    if labels is None and alpha != 1:
+        raise ValueError("distillation: alpha < 1 needs labels")
+    if labels is not None and labels.dtype != torch.int64:
+        raise ValueError(f"distillation: int64 labels, got {labels.dtype}")
+    gdt = grad_dtype or logits.dtype
+    if gdt != logits.dtype and (logits.dtype != torch.float32 or gdt not in (torch.bfloat16, torch.float16)):
+        raise ValueError(f"distillation: a {gdt} gradient of {logits.dtype} logits")
+    if _rows_enabled(logits):
+        x = logits if logits.stride(1) == 1 or V == 1 else logits.contiguous()
+        loss = torch.empty((), device=x.device, dtype=torch.float32)
+        grad = torch.empty((T, V), device=x.device, dtype=gdt) if need_grad else None
+        ext().distill_fwd_bwd(x, None if labels is None else labels.contiguous(), top_values.float().contiguous(),
+                              top_indices.contiguous(), None if top_lse is None else top_lse.float().contiguous(), grad,
+                              loss, float(temperature), float(alpha), float(grad_scale))
+        return loss, grad
+    loss, grad = _distillation_ref(logits.float(), labels, top_values.float(), top_indices.long(),
+                                   None if top_lse is None else top_lse.float(), temperature, alpha, need_grad)
+    return loss, (grad * grad_scale).to(gdt) if need_grad else None
+
+
+def _distillation_ref(z, labels, top_values, top_indices, top_lse, tau, alpha, need_grad=True):
+    V = z.shape[1]
+    ninf = float("-inf")
+    valid = (top_indices >= 0) & (top_indices < V)
+    at = top_indices.clamp(0, V - 1)
+    t = torch.where(valid, top_values / tau, ninf)
+    tl = torch.logsumexp(t, 1, keepdim=True) if top_lse is None else top_lse[:, None]
+    logp = t - tl
+    p = torch.where(t == ninf, 0.0, logp.exp())
+    zt = z / tau
+    logz = torch.logsumexp(zt, 1, keepdim=True)
+    kl = torch.where(p == 0, 0.0, p * (logp - (zt.gather(1, at) - logz))).sum(1)
+    q = (zt - logz).exp() if need_grad else None
+    mass = p.sum(1, keepdim=True)
+    soft = q
+    if top_lse is not None:
+        inside = torch.zeros_like(z).scatter_add(1, at, valid.to(z.dtype)) > 0
+        p_rest = torch.where(inside.all(1, keepdim=True), 0.0, (1 - mass).clamp_min(0))
+        rest = torch.logsumexp(zt.masked_fill(inside, ninf), 1, keepdim=True)
+        kl = kl + torch.where(p_rest > 0, p_rest * (p_rest.log() - (rest - logz)), 0.0)[:, 0]
+        mass = mass + p_rest
+        if need_grad:
+            soft = soft - torch.where(inside | (rest == ninf), 0.0, p_rest * (zt - rest).exp())
+    loss = alpha * tau * tau * kl if alpha > 0 else torch.zeros_like(kl)
+    grad = None
+    if need_grad:
+        grad = torch.where(mass == 0, 0.0, soft.scatter_add(1, at, -p)) * (alpha * tau)
+    if labels is not None:
+        live = (labels >= 0) & (labels < V)
+        y = labels.clamp(0, V - 1)[:, None]
+        if alpha != 1:
+            logs = torch.log_softmax(z, 1)
+            loss = loss - (1 - alpha) * logs.gather(1, y)[:, 0]
+            if need_grad:
+                grad = grad + (1 - alpha) * logs.exp().scatter_add(1, y, -torch.ones_like(y, dtype=z.dtype))
+        loss = torch.where(live, loss, 0.0)
+        grad = torch.where(live[:, None], grad, 0.0) if need_grad else None
+    return loss.sum(), grad
