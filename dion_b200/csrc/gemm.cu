@@ -8,14 +8,9 @@
 #include <mutex>
 
 #include "gemm_launch.cuh"
+#include "tensor_map.h"
 
 namespace bdion {
-
-namespace {
-
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
 EncodeTiledFn encode_fn() {
   static EncodeTiledFn fn = nullptr;
@@ -30,6 +25,8 @@ EncodeTiledFn encode_fn() {
   });
   return fn;
 }
+
+namespace {
 
 // 3-D tensor map over storage [batch][rows][cols] (cols contiguous), box =
 // {one 128-byte row of elements, box_rows, 1}, 128-byte swizzle, zero fill

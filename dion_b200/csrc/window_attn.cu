@@ -13,134 +13,13 @@
 #include <torch/extension.h>
 #include <torch/library.h>
 
-#include "common.cuh"
 #include "host_utils.h"
+#include "tensor_map.h"
+#include "window_tc.cuh"
 
 namespace bdion {
 
 namespace {
-
-struct WinArgs {
-  int b, s, hq, hkv, d, window, sinks;
-  float scale;
-  // strides in elements over (batch, position, head); the head dim is contiguous
-  int64_t q[3], k[3], v[3], g[3];
-};
-
-__device__ __forceinline__ float as_f(__nv_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ float as_f(__half v) { return __half2float(v); }
-__device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
-__device__ __forceinline__ void put(__half* p, float v) { *p = __float2half_rn(v); }
-
-__device__ __forceinline__ float warp_sum(float v) {
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffff, v, o);
-  return v;
-}
-
-template <typename T>
-__device__ __forceinline__ void load_row(const T* p, int d, float (&x)[4]) {
-#pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    const int c = r * 32 + threadIdx.x % 32;
-    x[r] = c < d ? as_f(p[c]) : 0.f;
-  }
-}
-__device__ __forceinline__ float dot(const float (&x)[4], const float (&y)[4]) {
-  return warp_sum(x[0] * y[0] + x[1] * y[1] + x[2] * y[2] + x[3] * y[3]);
-}
-
-// Calls f(j) for every key that query i sees.
-template <typename F>
-__device__ __forceinline__ void for_keys(const WinArgs& a, int i, F f) {
-  const int lo = max(0, i - a.window + 1);
-  for (int j = 0; j < min(a.sinks, lo); ++j) f(j);
-  for (int j = lo; j <= i; ++j) f(j);
-}
-
-// One warp per query: o and the row's log-sum-exp (natural logarithm).
-template <typename T>
-__global__ void __launch_bounds__(128) window_fwd_kernel(const T* q, const T* k, const T* v, T* o, float* lse,
-                                                         const WinArgs a) {
-  const int64_t w = (int64_t)blockIdx.x * 4 + threadIdx.x / 32;  // (b, i, h)
-  if (w >= (int64_t)a.b * a.s * a.hq) return;
-  const int h = w % a.hq, i = (w / a.hq) % a.s, b = w / a.hq / a.s, hk = h / (a.hq / a.hkv);
-  float x[4], acc[4] = {}, m = -INFINITY, sum = 0.f;
-  load_row(q + b * a.q[0] + i * a.q[1] + h * a.q[2], a.d, x);
-  for_keys(a, i, [&](int j) {
-    float y[4];
-    load_row(k + b * a.k[0] + j * a.k[1] + hk * a.k[2], a.d, y);
-    const float sc = dot(x, y) * a.scale, mn = fmaxf(m, sc), f = __expf(m - mn), p = __expf(sc - mn);
-    load_row(v + b * a.v[0] + j * a.v[1] + hk * a.v[2], a.d, y);
-    for (int r = 0; r < 4; ++r) acc[r] = acc[r] * f + p * y[r];
-    sum = sum * f + p;
-    m = mn;
-  });
-  for (int r = 0; r < 4; ++r) {
-    const int c = r * 32 + threadIdx.x % 32;
-    if (c < a.d) put(o + w * a.d + c, acc[r] / sum);
-  }
-  if (threadIdx.x % 32 == 0) lse[((int64_t)b * a.hq + h) * a.s + i] = m + logf(sum);
-}
-
-// One warp per query: dq and delta.
-template <typename T>
-__global__ void __launch_bounds__(128) window_dq_kernel(const T* q, const T* k, const T* v, const T* o, const T* g,
-                                                        const float* lse, T* dq, float* delta, const WinArgs a) {
-  const int64_t w = (int64_t)blockIdx.x * 4 + threadIdx.x / 32;
-  if (w >= (int64_t)a.b * a.s * a.hq) return;
-  const int h = w % a.hq, i = (w / a.hq) % a.s, b = w / a.hq / a.s, hk = h / (a.hq / a.hkv);
-  const int64_t at = ((int64_t)b * a.hq + h) * a.s + i;
-  float x[4], y[4], go[4], acc[4] = {};
-  load_row(q + b * a.q[0] + i * a.q[1] + h * a.q[2], a.d, x);
-  load_row(g + b * a.g[0] + i * a.g[1] + h * a.g[2], a.d, go);
-  load_row(o + w * a.d, a.d, y);
-  const float dl = dot(go, y), L = lse[at];
-  if (threadIdx.x % 32 == 0) delta[at] = dl;
-  for_keys(a, i, [&](int j) {
-    load_row(v + b * a.v[0] + j * a.v[1] + hk * a.v[2], a.d, y);
-    const float dp = dot(go, y);
-    load_row(k + b * a.k[0] + j * a.k[1] + hk * a.k[2], a.d, y);
-    const float ds = __expf(dot(x, y) * a.scale - L) * (dp - dl) * a.scale;
-    for (int r = 0; r < 4; ++r) acc[r] += ds * y[r];
-  });
-  for (int r = 0; r < 4; ++r) {
-    const int c = r * 32 + threadIdx.x % 32;
-    if (c < a.d) put(dq + w * a.d + c, acc[r]);
-  }
-}
-
-// One warp per key: dk and dv over the queries that see it and the heads of the group.
-template <typename T>
-__global__ void __launch_bounds__(128) window_dkv_kernel(const T* q, const T* k, const T* v, const T* g,
-                                                         const float* lse, const float* delta, T* dk, T* dv,
-                                                         const WinArgs a) {
-  const int64_t w = (int64_t)blockIdx.x * 4 + threadIdx.x / 32;
-  if (w >= (int64_t)a.b * a.s * a.hkv) return;
-  const int hk = w % a.hkv, j = (w / a.hkv) % a.s, b = w / a.hkv / a.s, group = a.hq / a.hkv;
-  float kx[4], vx[4], x[4], go[4], ak[4] = {}, av[4] = {};
-  load_row(k + b * a.k[0] + j * a.k[1] + hk * a.k[2], a.d, kx);
-  load_row(v + b * a.v[0] + j * a.v[1] + hk * a.v[2], a.d, vx);
-  const int last = j < a.sinks ? a.s : (int)min((int64_t)a.s, (int64_t)j + a.window);
-  for (int h = hk * group; h < (hk + 1) * group; ++h)
-    for (int i = j; i < last; ++i) {
-      const int64_t at = ((int64_t)b * a.hq + h) * a.s + i;
-      load_row(q + b * a.q[0] + i * a.q[1] + h * a.q[2], a.d, x);
-      load_row(g + b * a.g[0] + i * a.g[1] + h * a.g[2], a.d, go);
-      const float p = __expf(dot(x, kx) * a.scale - lse[at]);
-      const float ds = p * (dot(go, vx) - delta[at]) * a.scale;
-      for (int r = 0; r < 4; ++r) {
-        ak[r] += ds * x[r];
-        av[r] += p * go[r];
-      }
-    }
-  for (int r = 0; r < 4; ++r) {
-    const int c = r * 32 + threadIdx.x % 32;
-    if (c < a.d) {
-      put(dk + w * a.d + c, ak[r]);
-      put(dv + w * a.d + c, av[r]);
-    }
-  }
-}
 
 void check_heads(const at::Tensor& t, const at::Tensor& like, const char* what) {
   TORCH_CHECK(t.is_cuda() && t.device() == like.device() && t.scalar_type() == like.scalar_type() && t.dim() == 4 &&
@@ -170,47 +49,108 @@ WinArgs make_args(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
   a.d = (int)q.size(3);
   a.window = (int)std::min<int64_t>(window, a.s);
   a.sinks = (int)std::min<int64_t>(sinks, a.s);
+  a.s_pad = (a.s + kTile - 1) / kTile * kTile;
   a.scale = 1.f / std::sqrt((float)a.d);
-  for (int i = 0; i < 3; ++i) {
-    a.q[i] = q.stride(i);
-    a.k[i] = k.stride(i);
-    a.v[i] = v.stride(i);
-    a.g[i] = 0;
-  }
+  a.scale_log2 = a.scale * 1.4426950408889634f;
+  a.status = status_device_ptr();
+  a.limit_ns = wait_limit_ns();
   return a;
 }
 
-template <typename F>
-void by_type(at::ScalarType t, F f) {
-  if (t == at::kBFloat16)
-    f(__nv_bfloat16{});
-  else
-    f(__half{});
+// [b, s, heads, d] as a 4-D map (d, s, heads, b): boxes of 64 elements (one
+// swizzled 128-byte row) by `rows` positions of one head; elements beyond d
+// and rows beyond s read as zero.
+CUtensorMap head_map(const at::Tensor& t, int rows, const char* what) {
+  CUtensorMap m;
+  const cuuint64_t dims[4] = {(cuuint64_t)t.size(3), (cuuint64_t)t.size(1), (cuuint64_t)t.size(2),
+                              (cuuint64_t)t.size(0)};
+  cuuint64_t strides[3];
+  const int axis[3] = {1, 2, 0};
+  for (int i = 0; i < 3; ++i) {
+    const int64_t st = t.size(axis[i]) > 1 ? t.stride(axis[i]) * 2 : 16;
+    TORCH_CHECK(st > 0 && st % 16 == 0, "dion_b200 window_attention: ", what,
+                ": strides that are positive multiples of 16 bytes");
+    strides[i] = (cuuint64_t)st;
+  }
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0, "dion_b200 window_attention: ", what,
+              ": a base aligned to 16 bytes");
+  const cuuint32_t box[4] = {64u, (cuuint32_t)rows, 1u, 1u}, step[4] = {1u, 1u, 1u, 1u};
+  const CUresult r =
+      encode_fn()(&m, t.scalar_type() == at::kHalf ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                  4, t.data_ptr(), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  TORCH_CHECK(r == CUDA_SUCCESS, "dion_b200 window_attention: cuTensorMapEncodeTiled failed with ", (int)r);
+  return m;
 }
 
-unsigned warps_grid(int64_t rows) {
-  TORCH_CHECK((rows + 3) / 4 < (1ll << 31), "dion_b200 window_attention: too many rows");
-  return (unsigned)((rows + 3) / 4);
+// The tensor-map encoder wants a current context, which a thread that has made
+// no runtime call yet (autograd's backward threads) lacks.
+void bind_context(const at::Tensor& t) { C10_CUDA_CHECK(cudaSetDevice(t.get_device())); }
+
+// Launches with the kernel's shared memory allowed on the current device.
+template <typename K, typename... Args>
+void launch(K kern, int64_t grid, int threads, int smem, cudaStream_t st, Args... args) {
+  TORCH_CHECK(grid < (1ll << 31), "dion_b200 window_attention: too many tiles");
+  C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  kern<<<(unsigned)grid, threads, smem, st>>>(args...);
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  note_launch();
+}
+
+// f(element type, padded head dimension)
+template <typename F>
+void by_case(at::ScalarType t, int d, F f) {
+  auto with = [&](auto tag) {
+    if (d <= 64)
+      f(tag, std::integral_constant<int, 64>{});
+    else
+      f(tag, std::integral_constant<int, 128>{});
+  };
+  if (t == at::kBFloat16)
+    with(__nv_bfloat16{});
+  else
+    with(__half{});
+}
+
+// Parts of the dK / dV kernel. A tile is cut where the whole tiles would not
+// give every SM two parts; a tile with first tokens where its steps would
+// outlast the others'. A part has 8 steps at least: fewer cost more in its
+// start and its sums' way through memory than they bring.
+KeySplit split_keys(const WinArgs& a) {
+  KeySplit p;
+  const int64_t group = a.hq / a.hkv, sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
+  p.n_tiles = a.s_pad / kTile;
+  p.n_first = std::min(p.n_tiles, (a.sinks + kTile - 1) / kTile);
+  const int64_t heads = (int64_t)a.b * a.hkv, per_head = a.s_pad / kHalfTile;
+  const int64_t band = group * std::min<int64_t>(per_head, ((int64_t)kTile + a.window - 2) / kHalfTile + 1);
+  const int64_t first = group * per_head;
+  auto cut = [](int64_t parts, int64_t steps) { return (int)std::max<int64_t>(1, std::min(parts, steps / 8)); };
+  p.c_band = cut((2 * sms + heads * p.n_tiles - 1) / (heads * p.n_tiles), band);
+  const int64_t total = heads * (p.n_first * first + (p.n_tiles - p.n_first) * band);
+  const int64_t longest = std::max((band + p.c_band - 1) / p.c_band, total / (4 * sms));
+  p.c_first = cut((first + longest - 1) / longest, first);
+  return p;
 }
 
 }  // namespace
 
-// o [b, s, hq, d] and the rows' log-sum-exp [b, hq, s]
+// o [b, s, hq, d], and log2 of each row's sum of exponentials [b, hq, s
+// rounded up to 128] (+inf behind the last position) for the backward pass
 std::tuple<at::Tensor, at::Tensor> window_attention_fwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
                                                         int64_t window, int64_t sinks) {
   const WinArgs a = make_args(q, k, v, window, sinks);
   c10::cuda::CUDAGuard guard(q.device());
+  bind_context(q);
   auto o = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
-  auto lse = at::empty({a.b, a.hq, a.s}, q.options().dtype(at::kFloat));
+  auto lse = at::empty({a.b, a.hq, a.s_pad}, q.options().dtype(at::kFloat));
   if (o.numel() == 0) return {o, lse};
-  by_type(q.scalar_type(), [&](auto tag) {
+  const CUtensorMap mq = head_map(q, kTile, "q"), mk = head_map(k, kTile, "k"), mv = head_map(v, kTile, "v");
+  by_case(q.scalar_type(), a.d, [&](auto tag, auto dp) {
     using E = decltype(tag);
-    window_fwd_kernel<E><<<warps_grid((int64_t)a.b * a.s * a.hq), 128, 0, at::cuda::getCurrentCUDAStream()>>>(
-        (const E*)q.data_ptr(), (const E*)k.data_ptr(), (const E*)v.data_ptr(), (E*)o.data_ptr(),
-        lse.data_ptr<float>(), a);
+    constexpr int DP = decltype(dp)::value;
+    launch(window_fwd_tc<E, DP>, (int64_t)a.b * a.hq * (a.s_pad / kTile), 192, FwdCfg<E, DP>::kSmemBytes,
+           at::cuda::getCurrentCUDAStream(), mq, mk, mv, (E*)o.data_ptr(), lse.data_ptr<float>(), a);
   });
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
-  note_launch();
   return {o, lse};
 }
 
@@ -218,13 +158,14 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> window_attention_bwd(const at::Te
                                                                     const at::Tensor& k, const at::Tensor& v,
                                                                     const at::Tensor& o, const at::Tensor& lse,
                                                                     int64_t window, int64_t sinks) {
-  WinArgs a = make_args(q, k, v, window, sinks);
+  const WinArgs a = make_args(q, k, v, window, sinks);
   check_heads(go, q, "the output's gradient");
-  TORCH_CHECK(go.sizes() == q.sizes() && o.sizes() == q.sizes() && o.is_contiguous() && lse.is_contiguous() &&
-                  lse.scalar_type() == at::kFloat && lse.numel() == (int64_t)a.b * a.hq * a.s,
+  TORCH_CHECK(go.sizes() == q.sizes() && o.sizes() == q.sizes() && o.is_contiguous() && o.device() == q.device() &&
+                  o.scalar_type() == q.scalar_type() && lse.is_contiguous() && lse.device() == q.device() &&
+                  lse.scalar_type() == at::kFloat && lse.numel() == (int64_t)a.b * a.hq * a.s_pad,
               "dion_b200 window_attention: o and lse as the forward pass gave them");
-  for (int i = 0; i < 3; ++i) a.g[i] = go.stride(i);
   c10::cuda::CUDAGuard guard(q.device());
+  bind_context(q);
   auto st = at::cuda::getCurrentCUDAStream();
   auto like = [](const at::Tensor& t) {
     return at::empty(t.sizes(), t.options().memory_format(at::MemoryFormat::Contiguous));
@@ -232,18 +173,30 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> window_attention_bwd(const at::Te
   auto dq = like(q), dk = like(k), dv = like(v);
   if (q.numel() == 0) return {dq, dk.zero_(), dv.zero_()};
   auto delta = at::empty_like(lse);
-  by_type(q.scalar_type(), [&](auto tag) {
+  const KeySplit split = split_keys(a);
+  const CUtensorMap q128 = head_map(q, kTile, "q"), k128 = head_map(k, kTile, "k"), v128 = head_map(v, kTile, "v"),
+                    g128 = head_map(go, kTile, "the output's gradient"), q64 = head_map(q, kHalfTile, "q"),
+                    k64 = head_map(k, kHalfTile, "k"), v64 = head_map(v, kHalfTile, "v"),
+                    g64 = head_map(go, kHalfTile, "the output's gradient");
+  by_case(q.scalar_type(), a.d, [&](auto tag, auto dp) {
     using E = decltype(tag);
-    window_dq_kernel<E><<<warps_grid((int64_t)a.b * a.s * a.hq), 128, 0, st>>>(
-        (const E*)q.data_ptr(), (const E*)k.data_ptr(), (const E*)v.data_ptr(), (const E*)o.data_ptr(),
-        (const E*)go.data_ptr(), lse.data_ptr<float>(), (E*)dq.data_ptr(), delta.data_ptr<float>(), a);
-    C10_CUDA_KERNEL_LAUNCH_CHECK();
-    window_dkv_kernel<E><<<warps_grid((int64_t)a.b * a.s * a.hkv), 128, 0, st>>>(
-        (const E*)q.data_ptr(), (const E*)k.data_ptr(), (const E*)v.data_ptr(), (const E*)go.data_ptr(),
-        lse.data_ptr<float>(), delta.data_ptr<float>(), (E*)dk.data_ptr(), (E*)dv.data_ptr(), a);
-    C10_CUDA_KERNEL_LAUNCH_CHECK();
+    constexpr int DP = decltype(dp)::value;
+    launch(window_dq_tc<E, DP>, (int64_t)a.b * a.hq * (a.s_pad / kTile), 192, DqCfg<E, DP>::kSmemBytes, st, q128, k64,
+           v64, g128, (const E*)o.data_ptr(), (const E*)go.data_ptr(), go.stride(0), go.stride(1), go.stride(2),
+           lse.data_ptr<float>(), delta.data_ptr<float>(), (E*)dq.data_ptr(), a);
+    at::Tensor work;
+    const int64_t slots = (int64_t)a.b * a.hkv * split.slots();
+    if (slots > 0) work = at::empty({slots, 2, kTile, DP}, lse.options());
+    launch(window_dkv_tc<E, DP>, (int64_t)a.b * a.hkv * split.parts(), 320, DkvCfg<E, DP>::kSmemBytes, st, q64, k128,
+           v128, g64, lse.data_ptr<float>(), delta.data_ptr<float>(), (E*)dk.data_ptr(), (E*)dv.data_ptr(),
+           slots > 0 ? work.data_ptr<float>() : nullptr, split, a);
+    if (slots > 0) {
+      const int tile0 = split.c_first > 1 ? 0 : split.n_first;
+      const int tile1 = split.c_band > 1 ? split.n_tiles : split.n_first;
+      launch(window_dkv_join<E, DP>, (int64_t)(tile1 - tile0) * a.b * a.hkv * 2 * (kTile / 16), 16 * DP / 8, 0, st,
+             work.data_ptr<float>(), (E*)dk.data_ptr(), (E*)dv.data_ptr(), split, tile0, a);
+    }
   });
-  note_launch(2);
   return {dq, dk, dv};
 }
 

@@ -1,0 +1,877 @@
+// Tensor-core kernels of the sliding-window attention (see window_attn.cu for
+// the mathematics and the host side).
+#pragma once
+#include "ptx_attn.cuh"
+
+namespace bdion {
+
+struct WinArgs {
+  int b, s, hq, hkv, d, window, sinks;
+  int s_pad;        // positions rounded up to 128: row length of lse and delta
+  float scale;      // 1 / sqrt(d)
+  float scale_log2; // scale * log2(e)
+  int* status;
+  uint64_t limit_ns;
+};
+
+template <typename T>
+struct AttnType;
+template <>
+struct AttnType<__nv_bfloat16> {
+  static constexpr uint32_t kFmt = 1;
+};
+template <>
+struct AttnType<__half> {
+  static constexpr uint32_t kFmt = 0;
+};
+
+constexpr int kTile = 128;         // query rows of a CTA, and keys of a step
+constexpr int kPanel = kTile * 128;  // bytes of 128 rows of one 128-byte swizzle row (64 elements)
+
+// The key tiles that a tile of queries sees, in the order of their positions:
+// those with first tokens that lie before the band, then the band's.
+template <int NK>
+struct KeyTiles {
+  int n_first, band, n;
+  __device__ __forceinline__ KeyTiles(const WinArgs& a, int q0) {
+    band = max(0, q0 - a.window + 1) / NK;
+    n_first = min((a.sinks + NK - 1) / NK, band);
+    const int last = min(q0 + kTile, a.s) - 1;
+    n = n_first + last / NK - band + 1;
+  }
+  __device__ __forceinline__ int k0(int t) const { return (t < n_first ? t : band + t - n_first) * NK; }
+  // whether each of the 128 queries from q0 on sees each key of the tile at k0
+  static __device__ __forceinline__ bool whole(const WinArgs& a, int q0, int k0) {
+    return k0 + NK - 1 <= q0 && (q0 + kTile - 1 - k0 < a.window || k0 + NK <= a.sinks);
+  }
+};
+
+// Which of 32 keys k0 .. k0 + 31 query i sees, as a bit mask.
+__device__ __forceinline__ uint32_t seen_mask(const WinArgs& a, int i, int k0) {
+  const int hi = i - k0;                       // last visible column
+  const int lo = max(0, i - a.window + 1 - k0);  // first column of the band
+  const int first = a.sinks - k0;              // columns before this one are first tokens
+  uint32_t m = 0xffffffffu;
+  if (lo > 0) m = lo >= 32 ? 0u : 0xffffffffu << lo;
+  if (first > 0) m |= first >= 32 ? 0xffffffffu : (1u << first) - 1u;
+  if (hi < 31) m &= hi < 0 ? 0u : 0xffffffffu >> (31 - hi);
+  return m;
+}
+
+template <typename T, int DP>
+struct FwdCfg {
+  static constexpr int kPanels = DP / 64;
+  static constexpr int kTileBytes = kPanels * kPanel;
+  // keys and values: two stages where two CTAs still share an SM
+  static constexpr int kStages = DP == 64 ? 2 : 1;
+  static constexpr int kSmemBytes = kTileBytes * (1 + 2 * kStages) + 1024 + 256;
+  static constexpr int kTmemCols = 256;
+  // columns: S [0, 128), P after it where there is room (else P lies on S), O at the end
+  static constexpr bool kOverlay = DP == 128;
+  static constexpr int kP = kOverlay ? 0 : 128;
+  static constexpr int kO = 256 - DP;
+};
+
+// One CTA per (128 queries, head, sequence); two CTAs share an SM, so that one's
+// products run under the other's exponentials. Warp 0 loads (TMA), warp 1 issues
+// the products, warps 2-5 hold one query row per thread.
+//
+// A row's running maximum is the reference of its exponentials. It is moved
+// only when a tile exceeds it by more than 2^8, so O in TMEM is rarely rescaled;
+// P <= 2^8 loses nothing in 16 bits (its rounding is relative) and the sum is
+// kept in fp32 from the unrounded values.
+template <typename T, int DP>
+__global__ void __launch_bounds__(192, 2)
+    window_fwd_tc(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
+                  const __grid_constant__ CUtensorMap tv, T* __restrict__ o, float* __restrict__ lse, const WinArgs a) {
+  using Cfg = FwdCfg<T, DP>;
+  constexpr int ST = Cfg::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sQ = smem;
+  uint8_t* sK = sQ + Cfg::kTileBytes;
+  uint8_t* sV = sK + ST * Cfg::kTileBytes;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sV + ST * Cfg::kTileBytes);
+  uint64_t *q_full = bars, *k_full = bars + 1, *k_empty = bars + 3, *v_full = bars + 5, *v_empty = bars + 7,
+           *s_full = bars + 9, *p_full = bars + 10, *o_full = bars + 11, *drain = bars + 12;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 13);
+  volatile int* abort = reinterpret_cast<volatile int*>(bars + 14);
+
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int h = blockIdx.x % a.hq;
+  const int n_q = a.s_pad / kTile;
+  const int q0 = (blockIdx.x / a.hq) % n_q * kTile;
+  const int b = blockIdx.x / a.hq / n_q;
+  const int hk = h / (a.hq / a.hkv);
+  const KeyTiles<kTile> tiles(a, q0);
+
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&k_full[i], 1);
+      mbar_init(&k_empty[i], 1);
+      mbar_init(&v_full[i], 1);
+      mbar_init(&v_empty[i], 1);
+    }
+    mbar_init(s_full, 1);
+    mbar_init(p_full, 4);
+    mbar_init(o_full, 1);
+    mbar_init(drain, 1);
+    *abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, Cfg::kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const uint64_t limit = a.limit_ns;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      mbar_arrive_expect_tx(q_full, Cfg::kTileBytes);
+      for (int p = 0; p < Cfg::kPanels; ++p) tma_load_4d(&tq, q_full, sQ + p * kPanel, p * 64, q0, h, b);
+      int t = 0;
+      bool ok = true;
+      for (; t < tiles.n; ++t) {
+        const int st = t % ST, k0 = tiles.k0(t);
+        const uint32_t ph = (t / ST) & 1;
+        if (!mbar_wait_bounded(&k_empty[st], ph ^ 1, abort, limit)) { ok = false; break; }
+        mbar_arrive_expect_tx(&k_full[st], Cfg::kTileBytes);
+        for (int p = 0; p < Cfg::kPanels; ++p)
+          tma_load_4d(&tk, &k_full[st], sK + st * Cfg::kTileBytes + p * kPanel, p * 64, k0, hk, b);
+        if (!mbar_wait_bounded(&v_empty[st], ph ^ 1, abort, limit)) { ok = false; break; }
+        mbar_arrive_expect_tx(&v_full[st], Cfg::kTileBytes);
+        for (int p = 0; p < Cfg::kPanels; ++p)
+          tma_load_4d(&tv, &v_full[st], sV + st * Cfg::kTileBytes + p * kPanel, p * 64, k0, hk, b);
+      }
+      if (!ok) {
+        report_status(a.status, kStatusWindowProducerTimeout);
+        // copies in flight land before the shared memory is given up (bounded)
+        const uint64_t t0 = globaltimer_ns();
+        while (!mbar_try_wait(q_full, 0) && globaltimer_ns() - t0 < 100000000ull) {
+        }
+        for (int i = max(0, t - ST); i <= t; ++i) {
+          while (!mbar_try_wait(&k_full[i % ST], (i / ST) & 1) && globaltimer_ns() - t0 < 100000000ull) {
+          }
+          while (!mbar_try_wait(&v_full[i % ST], (i / ST) & 1) && globaltimer_ns() - t0 < 100000000ull) {
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      constexpr uint32_t kS = make_idesc(kTile, kTile, false, false, AttnType<T>::kFmt);
+      constexpr uint32_t kPV = make_idesc(kTile, DP, false, true, AttnType<T>::kFmt);
+      const uint32_t q_base = smem_u32(sQ);
+      bool ok = mbar_wait_bounded(q_full, 0, abort, limit);
+      auto scores = [&](int t) {
+        const int st = t % ST;
+        if (!mbar_wait_bounded(&k_full[st], (t / ST) & 1, abort, limit)) return false;
+        tc_fence_after();
+        const uint32_t k_base = smem_u32(sK + st * Cfg::kTileBytes);
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k) {
+          const uint32_t off = (k / 4) * kPanel + (k % 4) * 32;
+          umma_f16(tmem, make_sdesc_sw128(q_base + off, 16, 1024), make_sdesc_sw128(k_base + off, 16, 1024), kS, k != 0);
+        }
+        umma_commit(&k_empty[st]);
+        umma_commit(s_full);
+        return true;
+      };
+      if (ok) ok = scores(0);
+      for (int t = 0; t < tiles.n && ok; ++t) {
+        const int st = t % ST;
+        ok = mbar_wait_bounded(p_full, t & 1, abort, limit);
+        if (!ok) break;
+        tc_fence_after();
+        // the rows have read S; their next scores may start before this tile's P V
+        if (!Cfg::kOverlay && t + 1 < tiles.n && !scores(t + 1)) { ok = false; break; }
+        if (!mbar_wait_bounded(&v_full[st], (t / ST) & 1, abort, limit)) { ok = false; break; }
+        tc_fence_after();
+        const uint32_t v_base = smem_u32(sV + st * Cfg::kTileBytes);
+#pragma unroll
+        for (int k = 0; k < kTile / 16; ++k)
+          umma_f16_ts(tmem + Cfg::kO, tmem + Cfg::kP + k * 8, make_sdesc_sw128(v_base + k * 2048, kPanel, 1024), kPV,
+                      (t | k) != 0);
+        umma_commit(&v_empty[st]);
+        umma_commit(o_full);
+        if (Cfg::kOverlay && t + 1 < tiles.n) {
+          ok = mbar_wait_bounded(o_full, t & 1, abort, limit) && scores(t + 1);
+        }
+      }
+      if (!ok) {
+        report_status(a.status, kStatusWindowMmaTimeout);
+        umma_commit(drain);
+        const uint64_t t0 = globaltimer_ns();
+        while (!mbar_try_wait(drain, 0) && globaltimer_ns() - t0 < 100000000ull) {
+        }
+      }
+    }
+  } else {
+    const int quarter = warp & 3;
+    const int r = quarter * 32 + lane, i = q0 + r;
+    const uint32_t row = tmem + ((uint32_t)(quarter * 32) << 16);
+    const float c = a.scale_log2;
+    float m = -INFINITY, l = 0.f;  // reference of the exponentials (in score units), sum under it
+    bool ok = true;
+    for (int t = 0; t < tiles.n; ++t) {
+      const int k0 = tiles.k0(t);
+      if (!mbar_wait_bounded(s_full, t & 1, abort, limit)) { ok = false; break; }
+      tc_fence_after();
+      uint32_t x[128];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) tmem_ld_32x32b_x32(row + j * 32, reinterpret_cast<uint32_t(&)[32]>(x[j * 32]));
+      tmem_wait_ld();
+      if (!tiles.whole(a, q0, k0)) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t seen = seen_mask(a, i, k0 + j * 32);
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (!((seen >> e) & 1u)) x[j * 32 + e] = 0xff800000u;  // -inf
+        }
+      }
+      float mt[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int e = 0; e < 128; ++e) mt[e % 4] = fmaxf(mt[e % 4], __uint_as_float(x[e]));
+      const float top = fmaxf(fmaxf(mt[0], mt[1]), fmaxf(mt[2], mt[3]));
+      // move the reference where this tile exceeds it by more than 8 powers of two
+      float f = 1.f;
+      if ((top - m) * c > 8.f) {  // also the first visible tile (m = -inf); never while nothing is visible
+        f = ex2((m - top) * c);
+        m = top;
+        l *= f;
+      }
+      const float mc = m == -INFINITY ? 0.f : m * c;
+      float sum[4] = {};
+#pragma unroll
+      for (int e = 0; e < 128; e += 2) {
+        const float p0 = ex2(__uint_as_float(x[e]) * c - mc), p1 = ex2(__uint_as_float(x[e + 1]) * c - mc);
+        sum[(e / 2) % 2 * 2] += p0;
+        sum[(e / 2) % 2 * 2 + 1] += p1;
+        x[e / 2] = pack2(p0, p1, T{});
+      }
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      if (t > 0) {
+        // P's place and O are free once the tile before is done
+        if (!mbar_wait_bounded(o_full, (t - 1) & 1, abort, limit)) { ok = false; break; }
+        tc_fence_after();
+        if (__any_sync(0xffffffffu, f != 1.f)) {
+#pragma unroll
+          for (int j = 0; j < DP / 32; ++j) {
+            uint32_t y[32];
+            tmem_ld_32x32b_x32(row + Cfg::kO + j * 32, y);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) y[e] = __float_as_uint(__uint_as_float(y[e]) * f);
+            tmem_st_32x32b_x32(row + Cfg::kO + j * 32, y);
+          }
+        }
+      }
+      tmem_st_32x32b_x32(row + Cfg::kP, x);
+      tmem_st_32x32b_x32(row + Cfg::kP + 32, x + 32);
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(p_full);
+    }
+    if (ok) ok = mbar_wait_bounded(o_full, (tiles.n - 1) & 1, abort, limit);
+    if (!ok) {
+      if (lane == 0) report_status(a.status, kStatusWindowSoftmaxTimeout);
+    } else {
+      tc_fence_after();
+      const bool real = i < a.s;
+      lse[((int64_t)b * a.hq + h) * a.s_pad + i] = real ? m * c + log2f(l) : INFINITY;
+      const float inv = 1.f / l;
+      T* orow = o + (((int64_t)b * a.s + i) * a.hq + h) * a.d;
+#pragma unroll
+      for (int j = 0; j < DP / 32; ++j) {
+        uint32_t y[32];
+        tmem_ld_32x32b_x32(row + Cfg::kO + j * 32, y);
+        tmem_wait_ld();
+#pragma unroll
+        for (int e = 0; e < 32; e += 8) {
+          if (real && j * 32 + e < a.d) {
+            uint4 u;
+            uint32_t* w = reinterpret_cast<uint32_t*>(&u);
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+              w[n] = pack2(__uint_as_float(y[e + 2 * n]) * inv, __uint_as_float(y[e + 2 * n + 1]) * inv, T{});
+            *reinterpret_cast<uint4*>(orow + j * 32 + e) = u;
+          }
+        }
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc(tmem, Cfg::kTmemCols);
+}
+
+// ------------------------------------------------------------ backward: dQ
+constexpr int kHalfTile = 64;               // keys (dQ) or queries (dK, dV) of a step
+constexpr int kHalfPanel = kHalfTile * 128;
+
+template <typename T, int DP>
+struct DqCfg {
+  static constexpr int kPanels = DP / 64;
+  static constexpr int kRowBytes = kPanels * kPanel;       // Q, dO
+  static constexpr int kStepBytes = kPanels * kHalfPanel;  // K, V
+  static constexpr int kStages = DP == 64 ? 2 : 1;
+  static constexpr int kSmemBytes = 2 * kRowBytes + 2 * kStages * kStepBytes + 1024 + 256;
+  static constexpr int kTmemCols = 256;
+  // columns: S [0, 64), dP [64, 128), dS behind them where there is room (else on S), dQ at the end
+  static constexpr bool kOverlay = DP == 128;
+  static constexpr int kDS = kOverlay ? 0 : 128;
+  static constexpr int kDQ = 256 - DP;
+};
+
+// One CTA per (128 queries, head, sequence), two to an SM: S and dP by the
+// tensor cores, dS = P o (dP - delta) by one thread per query row, dQ += dS K
+// with dS read from TMEM. delta is taken here from O and dO and kept for the
+// dK / dV kernel (0 behind the last position).
+template <typename T, int DP>
+__global__ void __launch_bounds__(192, 2)
+    window_dq_tc(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
+                 const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap tg,
+                 const T* __restrict__ o, const T* __restrict__ go, int64_t go_b, int64_t go_s, int64_t go_h,
+                 const float* __restrict__ lse, float* __restrict__ delta, T* __restrict__ dq, const WinArgs a) {
+  using Cfg = DqCfg<T, DP>;
+  constexpr int ST = Cfg::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sQ = smem;
+  uint8_t* sG = sQ + Cfg::kRowBytes;
+  uint8_t* sK = sG + Cfg::kRowBytes;
+  uint8_t* sV = sK + ST * Cfg::kStepBytes;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sV + ST * Cfg::kStepBytes);
+  uint64_t *q_full = bars, *k_full = bars + 1, *k_empty = bars + 3, *v_full = bars + 5, *v_empty = bars + 7,
+           *s_full = bars + 9, *p_full = bars + 10, *o_full = bars + 11, *drain = bars + 12;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 13);
+  volatile int* abort = reinterpret_cast<volatile int*>(bars + 14);
+
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int h = blockIdx.x % a.hq;
+  const int n_q = a.s_pad / kTile;
+  const int q0 = (blockIdx.x / a.hq) % n_q * kTile;
+  const int b = blockIdx.x / a.hq / n_q;
+  const int hk = h / (a.hq / a.hkv);
+  const KeyTiles<kHalfTile> tiles(a, q0);
+
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&k_full[i], 1);
+      mbar_init(&k_empty[i], 1);
+      mbar_init(&v_full[i], 1);
+      mbar_init(&v_empty[i], 1);
+    }
+    mbar_init(s_full, 1);
+    mbar_init(p_full, 4);
+    mbar_init(o_full, 1);
+    mbar_init(drain, 1);
+    *abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, Cfg::kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const uint64_t limit = a.limit_ns;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      mbar_arrive_expect_tx(q_full, 2 * Cfg::kRowBytes);
+      for (int p = 0; p < Cfg::kPanels; ++p) {
+        tma_load_4d(&tq, q_full, sQ + p * kPanel, p * 64, q0, h, b);
+        tma_load_4d(&tg, q_full, sG + p * kPanel, p * 64, q0, h, b);
+      }
+      int t = 0;
+      bool ok = true;
+      for (; t < tiles.n; ++t) {
+        const int st = t % ST, k0 = tiles.k0(t);
+        const uint32_t ph = (t / ST) & 1;
+        // V is free once dP is done, K only after dQ
+        if (!mbar_wait_bounded(&v_empty[st], ph ^ 1, abort, limit)) { ok = false; break; }
+        mbar_arrive_expect_tx(&v_full[st], Cfg::kStepBytes);
+        for (int p = 0; p < Cfg::kPanels; ++p)
+          tma_load_4d(&tv, &v_full[st], sV + st * Cfg::kStepBytes + p * kHalfPanel, p * 64, k0, hk, b);
+        if (!mbar_wait_bounded(&k_empty[st], ph ^ 1, abort, limit)) { ok = false; break; }
+        mbar_arrive_expect_tx(&k_full[st], Cfg::kStepBytes);
+        for (int p = 0; p < Cfg::kPanels; ++p)
+          tma_load_4d(&tk, &k_full[st], sK + st * Cfg::kStepBytes + p * kHalfPanel, p * 64, k0, hk, b);
+      }
+      if (!ok) {
+        report_status(a.status, kStatusWindowProducerTimeout);
+        const uint64_t t0 = globaltimer_ns();
+        while (!mbar_try_wait(q_full, 0) && globaltimer_ns() - t0 < 100000000ull) {
+        }
+        for (int i = max(0, t - ST); i <= t; ++i) {
+          while (!mbar_try_wait(&k_full[i % ST], (i / ST) & 1) && globaltimer_ns() - t0 < 100000000ull) {
+          }
+          while (!mbar_try_wait(&v_full[i % ST], (i / ST) & 1) && globaltimer_ns() - t0 < 100000000ull) {
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      constexpr uint32_t kS = make_idesc(kTile, kHalfTile, false, false, AttnType<T>::kFmt);
+      constexpr uint32_t kD = make_idesc(kTile, DP, false, true, AttnType<T>::kFmt);
+      const uint32_t q_base = smem_u32(sQ), g_base = smem_u32(sG);
+      bool ok = mbar_wait_bounded(q_full, 0, abort, limit);
+      auto scores = [&](int t) {
+        const int st = t % ST;
+        const uint32_t ph = (t / ST) & 1;
+        if (!mbar_wait_bounded(&v_full[st], ph, abort, limit) || !mbar_wait_bounded(&k_full[st], ph, abort, limit))
+          return false;
+        tc_fence_after();
+        const uint32_t k_base = smem_u32(sK + st * Cfg::kStepBytes), v_base = smem_u32(sV + st * Cfg::kStepBytes);
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k) {
+          const uint32_t qo = (k / 4) * kPanel + (k % 4) * 32, ko = (k / 4) * kHalfPanel + (k % 4) * 32;
+          umma_f16(tmem, make_sdesc_sw128(q_base + qo, 16, 1024), make_sdesc_sw128(k_base + ko, 16, 1024), kS, k != 0);
+        }
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k) {
+          const uint32_t qo = (k / 4) * kPanel + (k % 4) * 32, ko = (k / 4) * kHalfPanel + (k % 4) * 32;
+          umma_f16(tmem + 64, make_sdesc_sw128(g_base + qo, 16, 1024), make_sdesc_sw128(v_base + ko, 16, 1024), kS,
+                   k != 0);
+        }
+        umma_commit(&v_empty[st]);
+        umma_commit(s_full);
+        return true;
+      };
+      if (ok) ok = scores(0);
+      for (int t = 0; t < tiles.n && ok; ++t) {
+        const int st = t % ST;
+        ok = mbar_wait_bounded(p_full, t & 1, abort, limit);
+        if (!ok) break;
+        tc_fence_after();
+        if (!Cfg::kOverlay && t + 1 < tiles.n && !scores(t + 1)) { ok = false; break; }
+        const uint32_t k_base = smem_u32(sK + st * Cfg::kStepBytes);
+#pragma unroll
+        for (int k = 0; k < kHalfTile / 16; ++k)
+          umma_f16_ts(tmem + Cfg::kDQ, tmem + Cfg::kDS + k * 8, make_sdesc_sw128(k_base + k * 2048, kHalfPanel, 1024), kD,
+                      (t | k) != 0);
+        umma_commit(&k_empty[st]);
+        umma_commit(o_full);
+        if (Cfg::kOverlay && t + 1 < tiles.n) ok = mbar_wait_bounded(o_full, t & 1, abort, limit) && scores(t + 1);
+      }
+      if (!ok) {
+        report_status(a.status, kStatusWindowMmaTimeout);
+        umma_commit(drain);
+        const uint64_t t0 = globaltimer_ns();
+        while (!mbar_try_wait(drain, 0) && globaltimer_ns() - t0 < 100000000ull) {
+        }
+      }
+    }
+  } else {
+    const int quarter = warp & 3;
+    const int i = q0 + quarter * 32 + lane;
+    const uint32_t row = tmem + ((uint32_t)(quarter * 32) << 16);
+    const float c = a.scale_log2;
+    const int64_t at = ((int64_t)b * a.hq + h) * a.s_pad + i;
+    const float L = lse[at];
+    float dl = 0.f;
+    if (i < a.s) {
+      const T* orow = o + (((int64_t)b * a.s + i) * a.hq + h) * a.d;
+      const T* grow = go + b * go_b + i * go_s + h * go_h;
+      for (int e = 0; e < a.d; e += 8) {
+        const uint4 ou = *reinterpret_cast<const uint4*>(orow + e), gu = *reinterpret_cast<const uint4*>(grow + e);
+        const T *op = reinterpret_cast<const T*>(&ou), *gp = reinterpret_cast<const T*>(&gu);
+#pragma unroll
+        for (int n = 0; n < 8; ++n) dl += (float)op[n] * (float)gp[n];
+      }
+    }
+    delta[at] = dl;
+    bool ok = true;
+    for (int t = 0; t < tiles.n; ++t) {
+      const int k0 = tiles.k0(t);
+      if (!mbar_wait_bounded(s_full, t & 1, abort, limit)) { ok = false; break; }
+      tc_fence_after();
+      uint32_t x[64], y[64];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        tmem_ld_32x32b_x32(row + j * 32, reinterpret_cast<uint32_t(&)[32]>(x[j * 32]));
+        tmem_ld_32x32b_x32(row + 64 + j * 32, reinterpret_cast<uint32_t(&)[32]>(y[j * 32]));
+      }
+      tmem_wait_ld();
+      if (!tiles.whole(a, q0, k0)) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const uint32_t seen = seen_mask(a, i, k0 + j * 32);
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (!((seen >> e) & 1u)) x[j * 32 + e] = 0xff800000u;
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 64; e += 2) {
+        const float p0 = ex2(__uint_as_float(x[e]) * c - L), p1 = ex2(__uint_as_float(x[e + 1]) * c - L);
+        x[e / 2] = pack2(p0 * (__uint_as_float(y[e]) - dl), p1 * (__uint_as_float(y[e + 1]) - dl), T{});
+      }
+      if (!Cfg::kOverlay && t > 0) {  // dS's place is free once the step before is done
+        if (!mbar_wait_bounded(o_full, (t - 1) & 1, abort, limit)) { ok = false; break; }
+        tc_fence_after();
+      }
+      tmem_st_32x32b_x32(row + Cfg::kDS, x);
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(p_full);
+    }
+    if (ok) ok = mbar_wait_bounded(o_full, (tiles.n - 1) & 1, abort, limit);
+    if (!ok) {
+      if (lane == 0) report_status(a.status, kStatusWindowSoftmaxTimeout);
+    } else {
+      tc_fence_after();
+      T* out = dq + (((int64_t)b * a.s + i) * a.hq + h) * a.d;
+#pragma unroll
+      for (int j = 0; j < DP / 32; ++j) {
+        uint32_t y[32];
+        tmem_ld_32x32b_x32(row + Cfg::kDQ + j * 32, y);
+        tmem_wait_ld();
+#pragma unroll
+        for (int e = 0; e < 32; e += 8) {
+          if (i < a.s && j * 32 + e < a.d) {
+            uint4 u;
+            uint32_t* w = reinterpret_cast<uint32_t*>(&u);
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+              w[n] = pack2(__uint_as_float(y[e + 2 * n]) * a.scale, __uint_as_float(y[e + 2 * n + 1]) * a.scale, T{});
+            *reinterpret_cast<uint4*>(out + j * 32 + e) = u;
+          }
+        }
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc(tmem, Cfg::kTmemCols);
+}
+
+// ------------------------------------------------------------ backward: dK, dV
+// How the key tiles' steps (a step: 64 queries of one head) are split over
+// CTAs. The queries that see first tokens reach to the end of the sequence,
+// those of every other tile only as far as the window: the tiles with first
+// tokens are cut into `c_first` parts, the others into `c_band`. A part of a
+// cut tile writes fp32 sums to its slot of the workspace, and a second kernel
+// adds the slots in order.
+struct KeySplit {
+  int n_tiles, n_first;   // key tiles, and those that hold first tokens
+  int c_first, c_band;
+  __host__ __device__ __forceinline__ int parts() const { return n_first * c_first + (n_tiles - n_first) * c_band; }
+  // parts of tile `tile`, and the number of the first of them
+  __host__ __device__ __forceinline__ int of(int tile) const { return tile < n_first ? c_first : c_band; }
+  __host__ __device__ __forceinline__ int first_part(int tile) const {
+    return tile < n_first ? tile * c_first : n_first * c_first + (tile - n_first) * c_band;
+  }
+  // workspace slots: parts of cut tiles only
+  __host__ __device__ __forceinline__ int slots() const {
+    return (c_first > 1 ? n_first * c_first : 0) + (c_band > 1 ? (n_tiles - n_first) * c_band : 0);
+  }
+  __host__ __device__ __forceinline__ int slot(int tile) const {
+    return tile < n_first ? tile * c_first : (c_first > 1 ? n_first * c_first : 0) + (tile - n_first) * c_band;
+  }
+};
+
+template <typename T, int DP>
+struct DkvCfg {
+  static constexpr int kPanels = DP / 64;
+  static constexpr int kRowBytes = kPanels * kPanel;       // K, V
+  static constexpr int kStepBytes = kPanels * kHalfPanel;  // Q, dO
+  static constexpr int kStages = DP == 64 ? 4 : 3;
+  static constexpr int kStatBytes = kHalfTile * 4;
+  static constexpr int kSmemBytes = 2 * kRowBytes + kStages * (2 * kStepBytes + 2 * kStatBytes) + 1024 + 512;
+  static constexpr int kTmemCols = 512;
+  // columns: two buffers of (S^T, dP^T) with P^T and dS^T on them, then dV and dK
+  static constexpr int kDV = 256, kDK = 256 + DP;
+};
+
+// One CTA per (128 keys, key head, sequence, part). With the keys as rows, P^T
+// and dS^T come out of TMEM in the place where dV += P^T dO and dK += dS^T Q
+// want their A operand, so neither passes through shared memory. Two groups of
+// four warps take the steps in turn, each with its own buffer.
+template <typename T, int DP>
+__global__ void __launch_bounds__(320, 1)
+    window_dkv_tc(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
+                  const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap tg,
+                  const float* __restrict__ lse, const float* __restrict__ delta, T* __restrict__ dk,
+                  T* __restrict__ dv, float* __restrict__ work, const KeySplit split, const WinArgs a) {
+  using Cfg = DkvCfg<T, DP>;
+  constexpr int ST = Cfg::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sK = smem;
+  uint8_t* sV = sK + Cfg::kRowBytes;
+  uint8_t* sQ = sV + Cfg::kRowBytes;
+  uint8_t* sG = sQ + ST * Cfg::kStepBytes;
+  float* sL = reinterpret_cast<float*>(sG + ST * Cfg::kStepBytes);
+  float* sD = sL + ST * kHalfTile;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sD + ST * kHalfTile);
+  uint64_t *k_full = bars, *q_full = bars + 1, *q_empty = bars + 5, *s_full = bars + 9, *p_full = bars + 11,
+           *acc_done = bars + 13, *all_done = bars + 15, *drain = bars + 16;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 17);
+  volatile int* abort = reinterpret_cast<volatile int*>(bars + 18);
+
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int hk = blockIdx.x % a.hkv, group = a.hq / a.hkv;
+  const int part = (blockIdx.x / a.hkv) % split.parts();
+  const int b = blockIdx.x / a.hkv / split.parts();
+  const int in_first = split.n_first * split.c_first;
+  const int tile = part < in_first ? part / split.c_first : split.n_first + (part - in_first) / split.c_band;
+  const int parts = split.of(tile), mine = part - split.first_part(tile);
+  const int k0 = tile * kTile;
+  // steps of the whole tile, and this part's
+  const int q_first = k0 / kHalfTile;
+  const int last_key = min(k0 + kTile, a.s) - 1;
+  const int q_last = (k0 < a.sinks ? a.s - 1 : (int)min((int64_t)a.s - 1, (int64_t)last_key + a.window - 1)) / kHalfTile;
+  const int nq = q_last - q_first + 1;
+  const int64_t all = (int64_t)nq * group;
+  const int lo = (int)(all * mine / parts), n = (int)(all * (mine + 1) / parts) - lo;
+
+  if (threadIdx.x == 0) {
+    mbar_init(k_full, 1);
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(&q_full[i], 1);
+      mbar_init(&q_empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 4);
+      mbar_init(&acc_done[i], 1);
+    }
+    mbar_init(all_done, 1);
+    mbar_init(drain, 1);
+    *abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, Cfg::kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const uint64_t limit = a.limit_ns;
+
+  if (warp == 0) {
+    if (lane == 0 && n > 0) {
+      mbar_arrive_expect_tx(k_full, 2 * Cfg::kRowBytes);
+      for (int p = 0; p < Cfg::kPanels; ++p) {
+        tma_load_4d(&tk, k_full, sK + p * kPanel, p * 64, k0, hk, b);
+        tma_load_4d(&tv, k_full, sV + p * kPanel, p * 64, k0, hk, b);
+      }
+      bool ok = true;
+      int t = 0;
+      for (; t < n; ++t) {
+        const int st = t % ST;
+        const int h = hk * group + (lo + t) / nq, q0 = (q_first + (lo + t) % nq) * kHalfTile;
+        if (!mbar_wait_bounded(&q_empty[st], ((t / ST) & 1) ^ 1, abort, limit)) { ok = false; break; }
+        mbar_arrive_expect_tx(&q_full[st], 2 * Cfg::kStepBytes + 2 * Cfg::kStatBytes);
+        for (int p = 0; p < Cfg::kPanels; ++p) {
+          tma_load_4d(&tq, &q_full[st], sQ + st * Cfg::kStepBytes + p * kHalfPanel, p * 64, q0, h, b);
+          tma_load_4d(&tg, &q_full[st], sG + st * Cfg::kStepBytes + p * kHalfPanel, p * 64, q0, h, b);
+        }
+        const int64_t at = ((int64_t)b * a.hq + h) * a.s_pad + q0;
+        bulk_load(sL + st * kHalfTile, lse + at, Cfg::kStatBytes, &q_full[st]);
+        bulk_load(sD + st * kHalfTile, delta + at, Cfg::kStatBytes, &q_full[st]);
+      }
+      if (!ok) {
+        report_status(a.status, kStatusWindowProducerTimeout);
+        const uint64_t t0 = globaltimer_ns();
+        while (!mbar_try_wait(k_full, 0) && globaltimer_ns() - t0 < 100000000ull) {
+        }
+        for (int i = max(0, t - ST); i < t; ++i)
+          while (!mbar_try_wait(&q_full[i % ST], (i / ST) & 1) && globaltimer_ns() - t0 < 100000000ull) {
+          }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && n > 0) {
+      constexpr uint32_t kS = make_idesc(kTile, kHalfTile, false, false, AttnType<T>::kFmt);
+      constexpr uint32_t kD = make_idesc(kTile, DP, false, true, AttnType<T>::kFmt);
+      const uint32_t k_base = smem_u32(sK), v_base = smem_u32(sV);
+      bool ok = mbar_wait_bounded(k_full, 0, abort, limit);
+      auto scores = [&](int t) {
+        const int st = t % ST, buf = t & 1;
+        if (!mbar_wait_bounded(&q_full[st], (t / ST) & 1, abort, limit)) return false;
+        // the buffer's P^T and dS^T of two steps ago have been read
+        if (t >= 2 && !mbar_wait_bounded(&acc_done[buf], ((t >> 1) - 1) & 1, abort, limit)) return false;
+        tc_fence_after();
+        const uint32_t q_base = smem_u32(sQ + st * Cfg::kStepBytes), g_base = smem_u32(sG + st * Cfg::kStepBytes);
+        const uint32_t d = tmem + buf * 128;
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k) {
+          const uint32_t ko = (k / 4) * kPanel + (k % 4) * 32, qo = (k / 4) * kHalfPanel + (k % 4) * 32;
+          umma_f16(d, make_sdesc_sw128(k_base + ko, 16, 1024), make_sdesc_sw128(q_base + qo, 16, 1024), kS, k != 0);
+        }
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k) {
+          const uint32_t ko = (k / 4) * kPanel + (k % 4) * 32, qo = (k / 4) * kHalfPanel + (k % 4) * 32;
+          umma_f16(d + 64, make_sdesc_sw128(v_base + ko, 16, 1024), make_sdesc_sw128(g_base + qo, 16, 1024), kS, k != 0);
+        }
+        umma_commit(&s_full[buf]);
+        return true;
+      };
+      if (ok) ok = scores(0);
+      for (int t = 0; t < n && ok; ++t) {
+        const int st = t % ST, buf = t & 1;
+        if (t + 1 < n && !scores(t + 1)) { ok = false; break; }
+        if (!mbar_wait_bounded(&p_full[buf], (t >> 1) & 1, abort, limit)) { ok = false; break; }
+        tc_fence_after();
+        const uint32_t q_base = smem_u32(sQ + st * Cfg::kStepBytes), g_base = smem_u32(sG + st * Cfg::kStepBytes);
+        const uint32_t d = tmem + buf * 128;
+#pragma unroll
+        for (int k = 0; k < kHalfTile / 16; ++k)
+          umma_f16_ts(tmem + Cfg::kDV, d + k * 8, make_sdesc_sw128(g_base + k * 2048, kHalfPanel, 1024), kD, (t | k) != 0);
+#pragma unroll
+        for (int k = 0; k < kHalfTile / 16; ++k)
+          umma_f16_ts(tmem + Cfg::kDK, d + 64 + k * 8, make_sdesc_sw128(q_base + k * 2048, kHalfPanel, 1024), kD,
+                      (t | k) != 0);
+        umma_commit(&q_empty[st]);
+        umma_commit(&acc_done[buf]);
+      }
+      if (ok) {
+        umma_commit(all_done);
+      } else {
+        report_status(a.status, kStatusWindowMmaTimeout);
+        umma_commit(drain);
+        const uint64_t t0 = globaltimer_ns();
+        while (!mbar_try_wait(drain, 0) && globaltimer_ns() - t0 < 100000000ull) {
+        }
+      }
+    }
+  } else {
+    const int quarter = warp & 3, which = (warp - 2) / 4;
+    const int r = quarter * 32 + lane, j = k0 + r;
+    const uint32_t row = tmem + ((uint32_t)(quarter * 32) << 16);
+    const uint32_t buf = row + which * 128;
+    const float c = a.scale_log2;
+    bool ok = true;
+    for (int t = which; t < n; t += 2) {
+      const int st = t % ST, q0 = (q_first + (lo + t) % nq) * kHalfTile;
+      if (!mbar_wait_bounded(&s_full[which], (t >> 1) & 1, abort, limit)) { ok = false; break; }
+      tc_fence_after();
+      uint32_t x[64], y[64];
+#pragma unroll
+      for (int n2 = 0; n2 < 2; ++n2) {
+        tmem_ld_32x32b_x32(buf + n2 * 32, reinterpret_cast<uint32_t(&)[32]>(x[n2 * 32]));
+        tmem_ld_32x32b_x32(buf + 64 + n2 * 32, reinterpret_cast<uint32_t(&)[32]>(y[n2 * 32]));
+      }
+      tmem_wait_ld();
+      // queries q0 + e that see key j: e in [j - q0, j + window - q0), without an end for first tokens
+      if (!(q0 >= k0 + kTile - 1 && (q0 + kHalfTile - 1 - k0 < a.window || k0 + kTile <= a.sinks))) {
+        const int e0 = j - q0, e1 = j < a.sinks ? kHalfTile : (int)min((int64_t)kHalfTile, (int64_t)j + a.window - q0);
+#pragma unroll
+        for (int e = 0; e < 64; ++e)
+          if (e < e0 || e >= e1) x[e] = 0xff800000u;
+      }
+      const float *pl = sL + st * kHalfTile, *pd = sD + st * kHalfTile;
+#pragma unroll
+      for (int e = 0; e < 64; e += 4) {
+        const float4 L = *reinterpret_cast<const float4*>(pl + e), D = *reinterpret_cast<const float4*>(pd + e);
+        const float p0 = ex2(__uint_as_float(x[e]) * c - L.x), p1 = ex2(__uint_as_float(x[e + 1]) * c - L.y);
+        const float p2 = ex2(__uint_as_float(x[e + 2]) * c - L.z), p3 = ex2(__uint_as_float(x[e + 3]) * c - L.w);
+        x[e / 2] = pack2(p0, p1, T{});
+        x[e / 2 + 1] = pack2(p2, p3, T{});
+        y[e / 2] = pack2(p0 * (__uint_as_float(y[e]) - D.x), p1 * (__uint_as_float(y[e + 1]) - D.y), T{});
+        y[e / 2 + 1] = pack2(p2 * (__uint_as_float(y[e + 2]) - D.z), p3 * (__uint_as_float(y[e + 3]) - D.w), T{});
+      }
+      tmem_st_32x32b_x32(buf, x);
+      tmem_st_32x32b_x32(buf + 64, y);
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_full[which]);
+    }
+    if (ok && n > 0) ok = mbar_wait_bounded(all_done, 0, abort, limit);
+    if (!ok) {
+      if (lane == 0) report_status(a.status, kStatusWindowSoftmaxTimeout);
+    } else {
+      tc_fence_after();
+      // the first group stores dV, the second dK
+      const uint32_t acc = row + (which == 0 ? Cfg::kDV : Cfg::kDK);
+      const float f = which == 0 ? 1.f : a.scale;
+      T* out = (which == 0 ? dv : dk) + (((int64_t)b * a.s + j) * a.hkv + hk) * a.d;
+      float* slot = nullptr;
+      if (parts > 1)
+        slot = work + ((((int64_t)b * a.hkv + hk) * split.slots() + split.slot(tile) + mine) * 2 + which) * kTile * DP +
+               (int64_t)r * DP;
+#pragma unroll
+      for (int j2 = 0; j2 < DP / 32; ++j2) {
+        uint32_t y[32];
+        if (n > 0) {
+          tmem_ld_32x32b_x32(acc + j2 * 32, y);
+          tmem_wait_ld();
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) y[e] = 0u;
+        }
+#pragma unroll
+        for (int e = 0; e < 32; e += 8) {
+          float v[8];
+#pragma unroll
+          for (int n2 = 0; n2 < 8; ++n2) v[n2] = __uint_as_float(y[e + n2]) * f;
+          if (slot != nullptr) {
+            store8(slot + j2 * 32 + e, v);
+          } else if (j < a.s && j2 * 32 + e < a.d) {
+            uint4 u;
+            uint32_t* w = reinterpret_cast<uint32_t*>(&u);
+#pragma unroll
+            for (int n2 = 0; n2 < 4; ++n2) w[n2] = pack2(v[2 * n2], v[2 * n2 + 1], T{});
+            *reinterpret_cast<uint4*>(out + j2 * 32 + e) = u;
+          }
+        }
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc(tmem, Cfg::kTmemCols);
+}
+
+// dK / dV of the cut tiles: the sum of their parts' slots, in order. One block
+// per 16 rows of (tile, key head, sequence, dK or dV).
+template <typename T, int DP>
+__global__ void __launch_bounds__(16 * DP / 8)
+    window_dkv_join(const float* __restrict__ work, T* __restrict__ dk, T* __restrict__ dv, const KeySplit split,
+                    int tile0, const WinArgs a) {
+  const int which = blockIdx.x % 2, r = blockIdx.x / 2 % (kTile / 16) * 16 + threadIdx.x / (DP / 8);
+  const int rest = blockIdx.x / (2 * kTile / 16);
+  const int hk = rest % a.hkv, b = rest / a.hkv % a.b, tile = tile0 + rest / a.hkv / a.b;
+  const int col = threadIdx.x % (DP / 8) * 8, j = tile * kTile + r;
+  if (j >= a.s || col >= a.d) return;
+  const float* p = work + (((int64_t)b * a.hkv + hk) * split.slots() + split.slot(tile)) * 2 * kTile * DP +
+                   (int64_t)which * kTile * DP + (int64_t)r * DP + col;
+  float s[8] = {};
+  for (int i = 0; i < split.of(tile); ++i) {
+    float v[8];
+    load8(p + (int64_t)i * 2 * kTile * DP, v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s[e] += v[e];
+  }
+  uint4 u;
+  uint32_t* w = reinterpret_cast<uint32_t*>(&u);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) w[e] = pack2(s[2 * e], s[2 * e + 1], T{});
+  *reinterpret_cast<uint4*>((which == 0 ? dv : dk) + (((int64_t)b * a.s + j) * a.hkv + hk) * a.d + col) = u;
+}
+
+}  // namespace bdion

@@ -166,14 +166,16 @@ def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0) -> TopLog
     return _fused.top_logits(logits, k, temperature)
 
 
-def _head_logits(h: torch.Tensor, W: torch.Tensor) -> torch.Tensor:
-    """h W^T in fp32. A bf16 logit of 8 is off by up to 2^-6, and a softmax
-    turns that into as large a relative error of its probability."""
-    if h.dtype == torch.float32:
-        return h @ W.t()
-    if h.is_cuda:
-        return torch.mm(h, W.t(), out_dtype=torch.float32)
-    return h.float() @ W.float().t()
+def _mm_fp32(a: torch.Tensor, b: torch.Tensor) -> torch.Tensor:
+    """a @ b with the sum and the result in fp32. (A bf16 logit of 8 is off by
+    up to 2^-6, and a softmax turns that into as large a relative error of its
+    probability; a bf16 result also lets the library add parts of a long sum
+    in bf16.)"""
+    if a.dtype == torch.float32:
+        return a @ b
+    if a.is_cuda:
+        return torch.mm(a, b, out_dtype=torch.float32)
+    return a.float() @ b.float()
 
 
 @torch.no_grad()
@@ -183,7 +185,7 @@ def linear_top_logits(h: torch.Tensor, W: torch.Tensor, k: int, temperature: flo
     that the [tokens, vocab] logits never exist at once. h: [..., dim]; the
     results are [..., k] and [...]."""
     h2 = h.reshape(-1, h.shape[-1])
-    parts = [_fused.top_logits(_head_logits(c, W), k, temperature) for c in h2.split(max(1, chunk))]
+    parts = [_fused.top_logits(_mm_fp32(c, W.t()), k, temperature) for c in h2.split(max(1, chunk))]
     values, indices, lse = (torch.cat(p) if len(p) > 1 else p[0] for p in zip(*parts))
     lead = h.shape[:-1]
     return TopLogits(values.view(*lead, k), indices.view(*lead, k), lse.view(lead))
@@ -194,23 +196,23 @@ class _LinearDistillation(torch.autograd.Function):
     chunk during forward as in :class:`_LinearCE`. The chunk's gradient of the
     logits is unscaled (a sum, not a mean) in h's dtype; the division by the
     number of rows in the loss, known on the device only, is applied with the
-    incoming gradient in backward."""
+    incoming gradient in backward, before the one rounding of each result."""
 
     @staticmethod
     def forward(ctx, h, W, labels, top_values, top_indices, top_lse, temperature, alpha, chunk, need_grad):
         T, V = h.shape[0], W.shape[0]
         total = torch.zeros((), device=h.device, dtype=torch.float32)
-        grad_h = torch.empty_like(h) if need_grad else None
+        grad_h = torch.empty(h.shape, device=h.device, dtype=torch.float32) if need_grad else None
         grad_W = torch.zeros(W.shape, device=W.device, dtype=torch.float32) if need_grad else None
         for s in range(0, T, chunk):
             e = min(T, s + chunk)
             hc = h[s:e]
             loss_c, g = _fused.distillation_fwd_bwd(
-                _head_logits(hc, W), None if labels is None else labels[s:e], top_values[s:e], top_indices[s:e],
+                _mm_fp32(hc, W.t()), None if labels is None else labels[s:e], top_values[s:e], top_indices[s:e],
                 None if top_lse is None else top_lse[s:e], temperature, alpha, 1.0, h.dtype, need_grad)
             total += loss_c
             if need_grad:
-                grad_h[s:e] = g @ W
+                grad_h[s:e] = _mm_fp32(g, W)
                 if h.is_cuda and h.dtype == torch.bfloat16:
                     ops.matmul(g.t(), hc, out=grad_W, C=grad_W, beta=1.0)
                 else:
@@ -218,14 +220,14 @@ class _LinearDistillation(torch.autograd.Function):
         n = max(T, 1) if labels is None else ((labels >= 0) & (labels < V)).sum().clamp_min(1).float()
         ctx.n = n
         ctx.save_for_backward(grad_h, grad_W)
-        ctx.W_dtype = W.dtype
+        ctx.dtypes = h.dtype, W.dtype
         return total / n
 
     @staticmethod
     def backward(ctx, go):
         grad_h, grad_W = ctx.saved_tensors
         f = go / ctx.n
-        return (grad_h * f, (grad_W * f).to(ctx.W_dtype)) + (None,) * 8
+        return ((grad_h * f).to(ctx.dtypes[0]), (grad_W * f).to(ctx.dtypes[1])) + (None,) * 8
 
 
 def linear_distillation(h: torch.Tensor, W: torch.Tensor, labels: Optional[torch.Tensor], top_values: torch.Tensor,
