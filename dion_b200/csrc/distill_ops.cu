@@ -4,10 +4,14 @@
 // all arithmetic is fp32.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <cooperative_groups.h>
 #include <cuda_fp16.h>
 #include <torch/extension.h>
 
 #include <cfloat>
+#include <map>
+#include <mutex>
+#include <tuple>
 
 #include "common.cuh"
 #include "host_utils.h"
@@ -297,7 +301,7 @@ struct DistillArgs {
   bool idx64;
   const float* top_lse;   // may be null: the teacher's entries alone are normalised
   float* row_loss;
-  int64_t ld_in, ld_out;
+  int64_t T, ld_in, ld_out;
   int V, k;
   bool vec;
   float inv_tau, alpha, tau, grad_scale;
@@ -491,6 +495,393 @@ __global__ void __launch_bounds__(kThreads) distill_kernel(const T* __restrict__
   }
 }
 
+// ------------------------------------------------------------ distillation loss, row held in registers
+// Eight elements as they lie in memory.
+template <typename T>
+struct Raw8 {
+  uint4 u[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) u[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
+  }
+  __device__ __forceinline__ void get(float* v) const { load8(reinterpret_cast<const T*>(u), v); }
+};
+
+constexpr int kEnds = 16;          // elements before the first and after the last 8-element group
+constexpr int kMaxCluster = 8;
+
+// Sums (or maxima) of N values over the block in two barriers; `buf` holds
+// N * (kWarps + 1) floats, which the next call may use at once.
+template <int N, bool MAX>
+__device__ __forceinline__ void block_all(float (&v)[N], float* buf) {
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = MAX ? warp_max(v[i]) : warp_sum(v[i]);
+  if (lane == 0) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) buf[N + i * kWarps + warp] = v[i];
+  }
+  __syncthreads();
+  if (warp < N) {
+    float x = lane < kWarps ? buf[N + warp * kWarps + lane] : (MAX ? -FLT_MAX : 0.f);
+    x = MAX ? warp_max(x) : warp_sum(x);
+    if (lane == 0) buf[warp] = x;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = buf[i];
+}
+
+// How the label's softmax (temperature 1) is taken beside the teacher's.
+enum HardMode { kHardNone, kHardSquare, kHardOther };
+
+// A cluster of `C` blocks holds one row in registers: each thread up to NV
+// groups of 8 elements, so the row is read once. The blocks exchange eight
+// partial results (one cluster barrier) and each writes its own part of the
+// gradient. The entries belong to the block that holds their column. Clusters
+// stay on their SMs and take rows in turn; the next row's elements are loaded
+// into the registers that the gradient has just been computed from, its label
+// and entries before that, so memory is busy through the row's reductions.
+//
+// Where the label's softmax differs from the teacher's, temperature 2 gives it
+// as the square of the teacher's exponentials, 2^(x log2e) = (2^(x log2e / 2))^2
+// (kHardSquare): at two exponentials per element and pass the SFU would take
+// longer than memory. Temperatures 3 and 4 take powers likewise (kHardOther
+// with `power`), others an exponential of their own.
+template <typename T, typename TG, int NV, int MODE>
+__global__ void __launch_bounds__(kThreads, 2)
+    distill_row_kernel(const T* __restrict__ logits, TG* __restrict__ grad, const DistillArgs a, int C, int power) {
+  namespace cg = cooperative_groups;
+  constexpr bool both = MODE != kHardNone;
+  __shared__ uint32_t s_marks[kThreads * NV / 4];  // one byte per group: which of its columns are in the set
+  __shared__ uint32_t s_end_marks;
+  __shared__ float red_max[2 * (kWarps + 1)], red_sum[6 * (kWarps + 1)];
+  __shared__ float s_p[kMaxTop], s_z[kMaxTop];
+  __shared__ int s_i[kMaxTop];
+  __shared__ int s_marked, s_twice;
+  enum { kM, kZ, kS, kF, kSet, kSetF, kCross, kCount, kParts };
+  __shared__ float s_parts[2][kMaxCluster][kParts];  // two turns: a block may be one row ahead of another
+  auto cluster = cg::this_cluster();
+  const int rank = blockIdx.x % C;
+  const int64_t stride = gridDim.x / C;
+  const int V = a.V, tid = threadIdx.x;
+  const bool hard = a.labels != nullptr && a.alpha != 1.f;
+  const float c = a.inv_tau * kLog2e;
+
+  // which columns this block holds of a row
+  struct Part {
+    int lead, g0, n, tail0;  // columns before the groups, first group, groups, columns behind all groups
+  };
+  auto part_of = [&](int64_t row) {
+    Part p;
+    p.lead = row_lead(row, a.ld_in, V, true);
+    const int n8 = (V - p.lead) / 8, per = (n8 + C - 1) / C;
+    p.g0 = min(n8, rank * per);
+    p.n = min(n8, p.g0 + per) - p.g0;
+    p.tail0 = p.lead + n8 * 8;
+    return p;
+  };
+  auto owner_bit = [&](const Part& p, int col, uint32_t*& word) -> int {  // bit of this block's marks, -1 if another's
+    if (col < p.lead || col >= p.tail0) {
+      word = &s_end_marks;
+      return rank == 0 ? (col < p.lead ? col : 8 + col - p.tail0) : -1;
+    }
+    const int g = (col - p.lead) / 8 - p.g0;
+    if (g < 0 || g >= p.n) return -1;
+    word = &s_marks[g / 4];
+    return g % 4 * 8 + (col - p.lead) % 8;
+  };
+  auto label_of = [&](int64_t row) -> int {  // -1: takes no part
+    if (row >= a.T) return -1;
+    const int64_t y = a.labels ? a.labels[row] : 0;
+    return y >= 0 && y < V ? (int)y : -1;
+  };
+  auto index_of = [&](int64_t row, int j) -> int {  // -1: unused entry
+    const int64_t i = a.idx64 ? static_cast<const int64_t*>(a.top_indices)[row * a.k + j]
+                              : static_cast<const int*>(a.top_indices)[row * a.k + j];
+    return i >= 0 && i < V ? (int)i : -1;
+  };
+  auto clear_marks = [&] {
+    for (int i = tid; i < kThreads * NV / 4; i += kThreads) s_marks[i] = 0;
+    if (tid == 0) s_marked = s_twice = 0, s_end_marks = 0;
+  };
+
+  cluster.barrier_arrive();  // waited for before the first store into another block
+  bool arrived = true;
+  int turn = 0;
+  int64_t row = blockIdx.x / C;
+  int label = label_of(row);
+  Raw8<T> raw[NV];
+  if (label >= 0) {
+    const Part p = part_of(row);
+    const T* xg = logits + row * a.ld_in + p.lead + (int64_t)p.g0 * 8;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (i * kThreads + tid < p.n) raw[i].load(xg + (i * kThreads + tid) * 8);
+  }
+  int ahead_i = -1;       // this thread's first entry of the next row
+  float ahead_t = 0.f;
+  if (label >= 0 && tid < a.k) {
+    ahead_i = index_of(row, tid);
+    ahead_t = a.top_values[row * a.k + tid];
+  }
+  clear_marks();
+  __syncthreads();
+
+  for (; row < a.T; row += stride) {
+  const Part mine_of = part_of(row);
+  const int lead = mine_of.lead, g0 = mine_of.g0, n_mine = mine_of.n, tail0 = mine_of.tail0;
+  const T* x = logits + row * a.ld_in;
+  TG* gx = grad + row * a.ld_out;
+  const int next_label = label_of(row + stride);
+  const Part next = part_of(row + stride);
+  const T* next_x = logits + (row + stride) * a.ld_in + next.lead + (int64_t)next.g0 * 8;
+  // the next row's group i into the place of this row's
+  auto load_next = [&](int i) {
+    if (next_label >= 0 && i * kThreads + tid < next.n) raw[i].load(next_x + (i * kThreads + tid) * 8);
+  };
+  const int now_i = ahead_i;
+  const float now_t = ahead_t;
+  if (next_label >= 0 && tid < a.k) {
+    ahead_i = index_of(row + stride, tid);
+    ahead_t = a.top_values[(row + stride) * a.k + tid];
+  }
+  if (label < 0) {  // takes no part: the whole cluster alike
+    const float zero[8] = {};
+    if (tid == 0 && rank == 0) a.row_loss[row] = 0.f;
+    if (grad != nullptr) {
+      for (int g = tid; g < n_mine; g += kThreads) store8(gx + lead + (g0 + g) * 8, zero);
+      if (rank == 0 && tid < lead) put(gx + tid, 0.f);
+      if (rank == 0 && tail0 + tid < V) put(gx + tail0 + tid, 0.f);
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) load_next(i);
+    label = next_label;
+    continue;
+  }
+  // ends of the row: columns [0, lead) and [tail0, V), one per thread of block 0
+  int end_col = -1;
+  if (rank == 0 && tid < 8 && tid < lead) end_col = tid;
+  if (rank == 0 && tid >= 8 && tid < kEnds && tail0 + tid - 8 < V) end_col = tail0 + tid - 8;
+  const float end_z = end_col >= 0 ? as_f(x[end_col]) : -INFINITY;
+  const float zy = hard ? as_f(x[label]) : 0.f;
+
+  float mx[2] = {-FLT_MAX, -FLT_MAX};  // outside the set, in it
+  float tmax = -FLT_MAX;
+  for (int j = tid; j < a.k; j += kThreads) {
+    const int i = j == tid ? now_i : index_of(row, j);
+    const float t = (j == tid ? now_t : a.top_values[row * a.k + j]) * a.inv_tau;
+    int mine = -1;  // this block's column, or -1
+    if (i >= 0) {
+      uint32_t* word;
+      const int bit = owner_bit(mine_of, i, word);
+      if (bit >= 0) {
+        mine = i;
+        const float z = as_f(x[i]);
+        s_z[j] = z;
+        mx[1] = fmaxf(mx[1], z);
+        if (atomicOr(word, 1u << bit) & (1u << bit))
+          s_twice = 1;
+        else
+          atomicAdd(&s_marked, 1);
+      }
+      tmax = fmaxf(tmax, t);
+    }
+    s_i[j] = mine;
+    s_p[j] = i >= 0 ? t : -INFINITY;
+  }
+  float tlse;
+  if (a.top_lse != nullptr) {
+    tlse = a.top_lse[row];
+  } else {
+    tmax = block_max(tmax, red_max);
+    float s = 0.f;
+    for (int j = tid; j < a.k; j += kThreads) s += s_p[j] == -INFINITY ? 0.f : ex2((s_p[j] - tmax) * kLog2e);
+    s = block_sum(s, red_max);
+    tlse = tmax + logf(s);
+  }
+  __syncthreads();
+
+  // maximum outside the set, then the sums under it; columns in the set count as -inf
+  auto get = [&](int i, float* v) {
+    raw[i].get(v);
+    const uint32_t marks = reinterpret_cast<const uint8_t*>(s_marks)[i * kThreads + tid];
+    if (marks) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if ((marks >> e) & 1u) v[e] = -INFINITY;
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    if (i * kThreads + tid < n_mine) {
+      float v[8];
+      get(i, v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) mx[0] = fmaxf(mx[0], v[e]);
+    }
+  const bool end_rest = end_col >= 0 && !((s_end_marks >> tid) & 1u);
+  if (end_rest) mx[0] = fmaxf(mx[0], end_z);
+  block_all<2, true>(mx, red_max);
+  const float m = mx[0], zmax = mx[1];
+  // y = 2^(c (z - ref)) of the teacher's softmax -> the label's
+  auto full_of = [&](float y, float z, float ref) {
+    if (MODE == kHardSquare) return y * y;
+    return power == 3 ? y * y * y : power == 4 ? (y * y) * (y * y) : ex2((z - ref) * kLog2e);
+  };
+  float sum[6] = {};  // rest; rest at temperature 1; set; set at temperature 1; teacher's mass; sum p (log p - z / tau)
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    if (i * kThreads + tid < n_mine) {
+      float v[8];
+      get(i, v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float y = ex2((v[e] - m) * c);
+        sum[0] += y;
+        if (both) sum[1] += full_of(y, v[e], m);
+      }
+    }
+  if (end_rest) {
+    const float y = ex2((end_z - m) * c);
+    sum[0] += y;
+    if (both) sum[1] += full_of(y, end_z, m);
+  }
+  const bool twice = s_twice != 0;
+  auto first_of = [&](int j) {
+    if (twice)
+      for (int i = 0; i < j; ++i)
+        if (s_i[i] == s_i[j]) return false;
+    return true;
+  };
+  for (int j = tid; j < a.k; j += kThreads) {
+    const float logp = s_p[j] - tlse, p = s_p[j] == -INFINITY ? 0.f : ex2(logp * kLog2e);
+    sum[4] += p;
+    if (s_i[j] >= 0) {
+      if (p != 0.f) sum[5] += p * (logp - s_z[j] * a.inv_tau);
+      if (first_of(j)) {
+        const float y = ex2((s_z[j] - zmax) * c);
+        sum[2] += y;
+        if (both) sum[3] += full_of(y, s_z[j], zmax);
+      }
+    }
+  }
+  block_all<6, false>(sum, red_sum);
+  const float psum = sum[4];
+  auto s_part = s_parts[turn];
+  turn ^= 1;
+  if (arrived) cluster.barrier_wait();
+  arrived = false;
+  if (tid < C * kParts) {
+    const int to = tid / kParts, what = tid % kParts;
+    const float mine[kParts] = {m, zmax, sum[0], sum[1], sum[2], sum[3], sum[5], (float)s_marked};
+    float v = mine[0];
+#pragma unroll
+    for (int i = 1; i < kParts; ++i) v = what == i ? mine[i] : v;
+    *cluster.map_shared_rank(&s_part[rank][what], to) = v;
+  }
+  cluster.sync();
+  float rm = -FLT_MAX, zm = -FLT_MAX;  // over the row
+  for (int r = 0; r < C; ++r) {
+    rm = fmaxf(rm, s_part[r][kM]);
+    zm = fmaxf(zm, s_part[r][kZ]);
+  }
+  const float top = fmaxf(rm, zm);
+  float rest_s = 0.f, rest_f = 0.f, B = 0.f, F = 0.f, cross = 0.f, marked = 0.f;
+  for (int r = 0; r < C; ++r) {
+    const float* q = s_part[r];
+    rest_s += q[kS] * ex2((q[kM] - rm) * c);
+    B += q[kSet] * ex2((q[kZ] - top) * c);
+    if (both) {
+      rest_f += q[kF] * ex2((q[kM] - rm) * kLog2e);
+      F += q[kSetF] * ex2((q[kZ] - top) * kLog2e);
+    }
+    cross += q[kCross];
+    marked += q[kCount];
+  }
+  const float to_top = ex2((rm - top) * c);
+  B += rest_s * to_top;
+  if (both) F += rest_f * ex2((rm - top) * kLog2e);
+  const float logz = top * a.inv_tau + logf(B);
+  const bool has_rest = a.top_lse != nullptr && marked < (float)V;
+  const float p_rest = has_rest ? fmaxf(1.f - psum, 0.f) : 0.f;
+  if (rank == 0 && tid == 0) {
+    float kl = psum != 0.f ? cross + psum * logz : 0.f;
+    if (p_rest > 0.f) kl += p_rest * (logf(p_rest) - (rm * a.inv_tau + logf(rest_s) - logz));
+    const float log_full = both ? top + logf(F) : logz;
+    a.row_loss[row] = (a.alpha > 0.f ? a.alpha * a.tau * a.tau * kl : 0.f) +
+                      (hard ? (1.f - a.alpha) * (log_full - zy) : 0.f);
+  }
+  if (grad == nullptr) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) load_next(i);
+    __syncthreads();
+    clear_marks();
+    __syncthreads();
+    label = next_label;
+    continue;
+  }
+
+  const float w_soft = a.grad_scale * a.alpha * a.tau * (psum + p_rest == 0.f ? 0.f : 1.f);
+  const float w_hard = hard ? a.grad_scale * (1.f - a.alpha) : 0.f;
+  const float inv_B = 1.f / B, inv_F = both ? 1.f / F : inv_B;
+  float f_rest = 0.f, f_full = 0.f;
+  if (rest_s > 0.f || rest_s != rest_s) {
+    f_rest = w_soft * (to_top * inv_B - p_rest / rest_s) + (both ? 0.f : w_hard * to_top * inv_B);
+    f_full = both ? w_hard * ex2((rm - top) * kLog2e) * inv_F : 0.f;
+  }
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    float v[8];
+    raw[i].get(v);
+    load_next(i);
+    if (i * kThreads + tid < n_mine) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float y = ex2((v[e] - rm) * c);
+        if (MODE == kHardNone)
+          v[e] = f_rest * y;
+        else if (MODE == kHardSquare)
+          v[e] = y * (f_rest + f_full * y);
+        else
+          v[e] = f_rest * y + f_full * full_of(y, v[e], rm);
+      }
+      store8(gx + lead + (g0 + i * kThreads + tid) * 8, v);
+    }
+  }
+  if (end_col >= 0) {
+    const float y = ex2((end_z - rm) * c);
+    put(gx + end_col, both ? f_rest * y + f_full * full_of(y, end_z, rm) : f_rest * y);
+  }
+  __syncthreads();
+  auto soft_at = [&](float z) { return ex2((z - top) * c) * inv_B; };
+  auto hard_at = [&](float z) { return both ? ex2((z - top) * kLog2e) * inv_F : soft_at(z); };
+  for (int j = tid; j < a.k; j += kThreads) {
+    const int i = s_i[j];
+    if (i < 0 || !first_of(j)) continue;
+    float p = 0.f;
+    for (int e = j; e < (twice ? a.k : j + 1); ++e)
+      if (s_i[e] == i && s_p[e] != -INFINITY) p += ex2((s_p[e] - tlse) * kLog2e);
+    float g = w_soft * (soft_at(s_z[j]) - p);
+    if (hard) g += w_hard * (hard_at(s_z[j]) - (i == label ? 1.f : 0.f));
+    put(gx + i, g);
+  }
+  if (hard && tid == 0) {
+    uint32_t* word;
+    const int bit = owner_bit(mine_of, label, word);
+    if (bit >= 0 && !((*word >> bit) & 1u)) {
+      const float r = rest_s > 0.f ? p_rest * ex2((zy - rm) * c) / rest_s : 0.f;
+      put(gx + label, w_soft * (soft_at(zy) - r) + w_hard * (hard_at(zy) - 1.f));
+    }
+  }
+  __syncthreads();
+  clear_marks();
+  __syncthreads();
+  label = next_label;
+  }
+  if (arrived) cluster.barrier_wait();
+}
+
 bool aligned8(const at::Tensor& t) {
   return reinterpret_cast<uintptr_t>(t.data_ptr()) % (8 * t.element_size()) == 0;
 }
@@ -500,8 +891,8 @@ void check_rows(const at::Tensor& t, const char* op) {
               "dion_b200 ", op, ": logits [T, V] on a CUDA device with contiguous rows");
   TORCH_CHECK(t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf || t.scalar_type() == at::kFloat,
               "dion_b200 ", op, ": bf16, fp16 or fp32 logits");
-  TORCH_CHECK(t.size(0) < (1ll << 31) && t.size(1) >= 1 && t.size(1) <= (1 << 20), "dion_b200 ", op,
-              ": 1 <= V <= 2^20 and T < 2^31");
+  TORCH_CHECK(t.size(0) < (1ll << 28) && t.size(1) >= 1 && t.size(1) <= (1 << 20), "dion_b200 ", op,
+              ": 1 <= V <= 2^20 and T < 2^28");
 }
 
 void check_out(const at::Tensor& t, const at::Tensor& like, at::ScalarType dtype, at::IntArrayRef shape,
@@ -509,6 +900,20 @@ void check_out(const at::Tensor& t, const at::Tensor& like, at::ScalarType dtype
   TORCH_CHECK(t.is_cuda() && t.device() == like.device() && t.scalar_type() == dtype && t.sizes() == shape &&
                   t.is_contiguous(),
               "dion_b200 ", what, ": a contiguous tensor of the stated shape and type on the logits' device");
+}
+
+// Clusters of C blocks that the device holds at once (asked once per kernel, device and C).
+template <typename K>
+int resident_clusters(K kern, const cudaLaunchConfig_t& cfg, int device, int C) {
+  static std::mutex lock;
+  static std::map<std::tuple<K, int, int>, int> known;
+  std::lock_guard<std::mutex> hold(lock);
+  int& n = known[{kern, device, C}];
+  if (n == 0) {
+    C10_CUDA_CHECK(cudaOccupancyMaxActiveClusters(&n, kern, &cfg));
+    n = std::max(n, 1);
+  }
+  return n;
 }
 
 template <typename F>
@@ -591,6 +996,7 @@ void distill_fwd_bwd(const at::Tensor& logits, const c10::optional<at::Tensor>& 
   a.row_loss = rows.data_ptr<float>();
   a.ld_in = logits.stride(0);
   a.ld_out = V;
+  a.T = T;
   a.V = V;
   a.k = k;
   // 8-element groups of the logits and of the gradient have to start together
@@ -606,6 +1012,48 @@ void distill_fwd_bwd(const at::Tensor& logits, const c10::optional<at::Tensor>& 
     by_type(gtype, [&](auto gtag) {
       using G = decltype(gtag);
       if constexpr (std::is_same_v<E, G> || std::is_same_v<E, float>) {
+        // Rows of up to kMaxCluster blocks' registers are read once; longer ones, and
+        // those whose logits and gradient are not aligned alike, twice.
+        constexpr int kMost = sizeof(E) == 2 ? 8 : 4;  // 32 registers of logits per thread
+        const int64_t groups = V / 8;
+        if (a.vec && groups <= (int64_t)kMaxCluster * kThreads * kMost) {
+          int C = 1;
+          while (groups > (int64_t)C * kThreads * kMost) C *= 2;
+          const int64_t per_thread = (groups + C * kThreads - 1) / (C * kThreads);
+          const int power = tau == 3 || tau == 4 ? (int)tau : 0;
+          auto run = [&](auto nv, auto mode) {
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = dim3((unsigned)C);
+            cfg.blockDim = dim3(kThreads);
+            cfg.stream = s;
+            cudaLaunchAttribute attr[1];
+            attr[0].id = cudaLaunchAttributeClusterDimension;
+            attr[0].val.clusterDim = {(unsigned)C, 1u, 1u};
+            cfg.attrs = attr;
+            cfg.numAttrs = 1;
+            auto kern = distill_row_kernel<E, G, decltype(nv)::value, decltype(mode)::value>;
+            cfg.gridDim.x = (unsigned)(C * std::min<int64_t>(T, resident_clusters(kern, cfg, logits.get_device(), C)));
+            C10_CUDA_CHECK(cudaLaunchKernelEx(
+                &cfg, kern,
+                static_cast<const E*>(logits.data_ptr()),
+                grad.has_value() ? static_cast<G*>(grad->data_ptr()) : nullptr, a, C, power));
+          };
+          auto by_mode = [&](auto nv) {
+            if (!a.labels || a.alpha == 1.f || a.inv_tau == 1.f)
+              run(nv, std::integral_constant<int, kHardNone>{});
+            else if (tau == 2)
+              run(nv, std::integral_constant<int, kHardSquare>{});
+            else
+              run(nv, std::integral_constant<int, kHardOther>{});
+          };
+          if (per_thread <= 1)
+            by_mode(std::integral_constant<int, 1>{});
+          else if (per_thread <= 4 || kMost == 4)
+            by_mode(std::integral_constant<int, 4>{});
+          else
+            by_mode(std::integral_constant<int, kMost>{});
+          return;
+        }
         auto kern = distill_kernel<E, G>;
         C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
         kern<<<(unsigned)T, kThreads, smem, s>>>(static_cast<const E*>(logits.data_ptr()),
