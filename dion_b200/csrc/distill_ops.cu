@@ -150,145 +150,246 @@ __device__ __forceinline__ int row_lead(int64_t row, int64_t ld, int V, bool vec
   return vec ? min(V, (int)((8 - (row * ld) % 8) % 8)) : V;
 }
 
+__device__ __forceinline__ float pair_max(uint32_t a, uint32_t b, uint32_t c, uint32_t d, __nv_bfloat16) {
+  auto h = [](uint32_t x) { return *reinterpret_cast<const __nv_bfloat162*>(&x); };
+  const float2 f = __bfloat1622float2(__hmax2(__hmax2(h(a), h(b)), __hmax2(h(c), h(d))));
+  return fmaxf(f.x, f.y);
+}
+__device__ __forceinline__ float pair_max(uint32_t a, uint32_t b, uint32_t c, uint32_t d, __half) {
+  auto h = [](uint32_t x) { return *reinterpret_cast<const __half2*>(&x); };
+  const float2 f = __half22float2(__hmax2(__hmax2(h(a), h(b)), __hmax2(h(c), h(d))));
+  return fmaxf(f.x, f.y);
+}
+
+// Eight elements as they lie in memory.
+template <typename T>
+struct Raw8 {
+  uint4 u[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) u[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
+  }
+  // eight elements at any alignment
+  __device__ __forceinline__ void load_single(const T* p) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) reinterpret_cast<T*>(u)[i] = p[i];
+  }
+  __device__ __forceinline__ float max() const {  // NaN are left out
+    if constexpr (sizeof(T) == 2) {
+      return pair_max(u[0].x, u[0].y, u[0].z, u[0].w, T{});
+    } else {
+      const float* v = reinterpret_cast<const float*>(u);
+      return fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7])));
+    }
+  }
+  __device__ __forceinline__ void get(float* v) const { load8(reinterpret_cast<const T*>(u), v); }
+};
+
+
 // ------------------------------------------------------------ top logits
-// One block per row. The first pass over the row takes the log-sum-exp and
-// the maximum of each of kThreads * G groups of columns. The k-th largest of
-// those maxima bounds the k-th largest logit from below (k elements are at
-// least that large), so a second pass collects the few columns above it, and
-// each candidate's rank is the number of larger ones (value, then the lower
-// index). Rows with too many equal values for the candidate buffer take the
-// exact threshold bit by bit and keep the lowest indices of the equal ones.
+__device__ __forceinline__ float key_float(uint32_t key) {  // the float that order_key took (not for NaN)
+  return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
+}
+
+// Largest threshold that at least k of the n keys reach, bit by bit (one warp);
+// stops early where exactly k do. key(i) may be called for i < n only.
+template <typename F>
+__device__ __forceinline__ uint32_t kth_key(int n, int k, F key) {
+  uint32_t thr = 0;
+  for (int bit = 31; bit >= 0; --bit) {
+    const uint32_t t = thr | (1u << bit);
+    int cnt = 0;
+    for (int i = threadIdx.x % 32; i < n; i += 32) cnt += key(i) >= t;
+    cnt = __reduce_add_sync(0xffffffffu, cnt);
+    if (cnt >= k) thr = t;
+    if (cnt == k) break;
+  }
+  return thr;
+}
+
+// One block per row, in one pass over it and a sample. The sample (`ns` of the
+// row's rounds of kThreads groups, spread evenly) gives the maximum of each of
+// kThreads * G sets of columns; the k-th largest of those bounds the row's k-th
+// largest logit from below. The pass then takes the log-sum-exp and collects
+// the columns above that bound: a group's maximum decides for eight columns at
+// once. The host takes ns so that about 512 come together. A candidate's rank
+// is the number of larger ones (value, then the lower index), counted after a
+// second bound has thinned them out. Rows with too many candidates (equal
+// values), and rows with a NaN or +inf, take the exact threshold over the whole
+// row bit by bit and keep the lowest indices of the equal ones.
 template <typename T, int G>
 __global__ void __launch_bounds__(kThreads) top_logits_kernel(const T* __restrict__ logits, int64_t ld, int V, int k,
-                                                              bool vec, float c, float* __restrict__ values,
+                                                              bool vec, int ns, float c, float* __restrict__ values,
                                                               int64_t* __restrict__ indices,
                                                               float* __restrict__ lse) {
   __shared__ float red[kWarps];
   __shared__ uint32_t s_max[kThreads * G];
-  __shared__ uint64_t s_cand[kMaxCand];
+  __shared__ uint64_t s_cand[2][kMaxCand];
   __shared__ int s_n;
   __shared__ uint32_t s_thr;
   const int64_t row = blockIdx.x;
   const T* x = logits + row * ld;
-  const int lead = row_lead(row, ld, V, vec);
+  const int tid = threadIdx.x;
+  const int lead = vec ? row_lead(row, ld, V, true) : 0;
+  const int n8 = (V - lead) / 8, tail0 = lead + n8 * 8, rounds = (n8 + kThreads - 1) / kThreads;
+  auto load = [&](int g, Raw8<T>& r) {
+    if (vec)
+      r.load(x + lead + g * 8);
+    else
+      r.load_single(x + g * 8);
+  };
+  // columns outside the groups, one per thread
+  const int end_col = tid < 8 ? (tid < lead ? tid : -1) : (tid < 16 && tail0 + tid - 8 < V ? tail0 + tid - 8 : -1);
+  const float end_z = end_col >= 0 ? as_f(x[end_col]) : -INFINITY;
 
-  RunningSum sum;
-  uint32_t best[G];
+  // the sample's bound
+  float best[G];
 #pragma unroll
-  for (int g = 0; g < G; ++g) best[g] = 0;
-  int turn = 0;
-  for_row(x, V, lead, [&](int, const float* v, auto n) {
-    constexpr int N = decltype(n)::value;
-    float vm = v[0];
+  for (int i = 0; i < G; ++i) best[i] = -INFINITY;
+  for (int j = 0; j < ns; j += 4) {
+    Raw8<T> r[4];
 #pragma unroll
-    for (int i = 1; i < N; ++i) vm = fmaxf(vm, v[i]);
-    sum.raise(vm, c);
-    uint32_t key = 0;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      sum.s += ex2((v[i] - sum.m) * c);
-      key = max(key, order_key(v[i]));
+    for (int i = 0; i < 4; ++i) {
+      const int g = (j + i) * rounds / ns * kThreads + tid;
+      if (j + i < ns && g < n8) load(g, r[i]);
     }
 #pragma unroll
-    for (int g = 0; g < G; ++g)
-      if (turn == g) best[g] = max(best[g], key);
-    turn = turn + 1 == G ? 0 : turn + 1;
-  });
-#pragma unroll
-  for (int g = 0; g < G; ++g) s_max[threadIdx.x * G + g] = best[g];
-  if (threadIdx.x == 0) s_n = 0;
-  sum.join(c, red);
-  if (threadIdx.x == 0) lse[row] = sum.m * c * kLn2 + logf(sum.s);
-
-  // largest threshold that at least k group maxima reach (0: everything is a candidate)
-  if (threadIdx.x < 32) {
-    uint32_t mine[kThreads * G / 32];
-#pragma unroll
-    for (int i = 0; i < kThreads * G / 32; ++i) mine[i] = s_max[i * 32 + threadIdx.x];
-    uint32_t thr = 0;
-    for (int bit = 31; bit >= 0; --bit) {
-      const uint32_t t = thr | (1u << bit);
-      int cnt = 0;
-#pragma unroll
-      for (int i = 0; i < kThreads * G / 32; ++i) cnt += mine[i] >= t;
-      if (__reduce_add_sync(0xffffffff, cnt) >= k) thr = t;
+    for (int i = 0; i < 4; ++i) {
+      const int g = (j + i) * rounds / ns * kThreads + tid;
+      if (j + i < ns && g < n8) best[i % G] = fmaxf(best[i % G], r[i].max());
     }
-    if (threadIdx.x == 0) s_thr = thr;
+  }
+#pragma unroll
+  for (int i = 0; i < G; ++i) s_max[tid * G + i] = best[i] == -INFINITY ? 0u : order_key(best[i]);
+  if (tid == 0) s_n = 0;
+  __syncthreads();
+  if (tid < 32) {
+    const uint32_t t = kth_key(kThreads * G, k, [&](int i) { return s_max[i]; });
+    if (tid == 0) s_thr = t;
   }
   __syncthreads();
   uint32_t thr = s_thr;
-  auto collect = [&]() {
-    for_row(x, V, lead, [&](int col, const float* v, auto n) {
-      constexpr int N = decltype(n)::value;
+  const float thr_f = thr == 0 ? -INFINITY : key_float(thr);
+  auto collect_one = [&](float v, int col) {
+    const int at = atomicAdd(&s_n, 1);
+    if (at < kMaxCand) s_cand[0][at] = ((uint64_t)order_key(v) << 32) | (uint32_t)~(uint32_t)col;
+  };
+
+  // the pass
+  RunningSum sum;
+  for (int j = 0; j < rounds; j += 4) {
+    Raw8<T> r[4];
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const uint32_t key = order_key(v[i]);
-        if (key >= thr) {
-          const int at = atomicAdd(&s_n, 1);
-          if (at < kMaxCand) s_cand[at] = ((uint64_t)key << 32) | (uint32_t)~(uint32_t)(col + i);
+    for (int i = 0; i < 4; ++i) {
+      const int g = (j + i) * kThreads + tid;
+      if (g < n8) load(g, r[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int g = (j + i) * kThreads + tid;
+      if (g < n8) {
+        float v[8];
+        r[i].get(v);
+        const float vm = r[i].max();
+        sum.raise(vm, c);
+        float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+          s0 += ex2((v[e] - sum.m) * c);
+          s1 += ex2((v[e + 1] - sum.m) * c);
+        }
+        sum.s += s0 + s1;
+        if (vm >= thr_f) {
+#pragma unroll 1
+          for (int e = 0; e < 8; ++e) {
+            const float z = as_f(x[lead + g * 8 + e]);
+            if (z >= thr_f) collect_one(z, lead + g * 8 + e);
+          }
         }
       }
-    });
-    __syncthreads();
-  };
-  collect();
+    }
+  }
+  if (end_col >= 0) {
+    sum.add(end_z, c);
+    if (end_z >= thr_f) collect_one(end_z, end_col);
+  }
+  sum.join(c, red);  // its barriers also end the collection
   int n = s_n;
-  if (n > kMaxCand) {
+  int from = 0;
+  const bool special = !(sum.s <= FLT_MAX) || !(sum.m <= FLT_MAX);  // a NaN or +inf somewhere
+  if (!special && tid == 0) lse[row] = sum.m * c * kLn2 + logf(sum.s);
+  if (n > kMaxCand || special) {
+    auto for_all = [&](auto f) {
+      for (int col = tid; col < V; col += kThreads) f(col, order_key(as_f(x[col])));
+    };
     // exact threshold: the largest one that at least k logits reach
     thr = 0;
     for (int bit = 31; bit >= 0; --bit) {
       const uint32_t t = thr | (1u << bit);
       int cnt = 0;
-      for_row(x, V, lead, [&](int, const float* v, auto n) {
-        constexpr int N = decltype(n)::value;
-#pragma unroll
-        for (int i = 0; i < N; ++i) cnt += order_key(v[i]) >= t;
-      });
+      for_all([&](int, uint32_t key) { cnt += key >= t; });
       __syncthreads();
-      if (threadIdx.x == 0) s_n = 0;
+      if (tid == 0) s_n = 0;
       __syncthreads();
-      cnt = __reduce_add_sync(0xffffffff, cnt);
-      if (threadIdx.x % 32 == 0) atomicAdd(&s_n, cnt);
+      cnt = __reduce_add_sync(0xffffffffu, cnt);
+      if (tid % 32 == 0) atomicAdd(&s_n, cnt);
       __syncthreads();
       if (s_n >= k) thr = t;
     }
     __syncthreads();
-    if (threadIdx.x == 0) s_n = 0;
+    if (tid == 0) s_n = 0;
     __syncthreads();
-    const uint32_t at_thr = thr;
-    if (at_thr != 0xffffffffu) {  // those above it: fewer than k
-      thr = at_thr + 1;
-      collect();
-    }
+    // those above it, fewer than k
+    for_all([&](int col, uint32_t key) {
+      if (key > thr) s_cand[0][atomicAdd(&s_n, 1)] = ((uint64_t)key << 32) | (uint32_t)~(uint32_t)col;
+    });
+    __syncthreads();
     // the equal ones in the order of their indices, as many as are wanted
     int have = s_n;
     __syncthreads();
     for (int c0 = 0; c0 < V && have < k; c0 += kThreads) {
-      const int col = c0 + threadIdx.x;
-      const bool eq = col < V && order_key(as_f(x[col])) == at_thr;
-      const uint32_t votes = __ballot_sync(0xffffffff, eq);
-      if (threadIdx.x % 32 == 0) s_max[threadIdx.x / 32] = __popc(votes);
+      const int col = c0 + tid;
+      const bool eq = col < V && order_key(as_f(x[col])) == thr;
+      const uint32_t votes = __ballot_sync(0xffffffffu, eq);
+      if (tid % 32 == 0) s_max[tid / 32] = __popc(votes);
       __syncthreads();
       int before = have, all = 0;
       for (int w = 0; w < kWarps; ++w) {
-        if (w < (int)threadIdx.x / 32) before += s_max[w];
+        if (w < tid / 32) before += s_max[w];
         all += s_max[w];
       }
-      before += __popc(votes & ((1u << (threadIdx.x % 32)) - 1u));
-      if (eq && before < k) s_cand[before] = ((uint64_t)at_thr << 32) | (uint32_t)~(uint32_t)col;
+      before += __popc(votes & ((1u << (tid % 32)) - 1u));
+      if (eq && before < k) s_cand[0][before] = ((uint64_t)thr << 32) | (uint32_t)~(uint32_t)col;
       have += all;
       __syncthreads();
     }
     n = min(have, k);
+  } else if (n > 2 * k && n > 128) {
+    // a second bound, now over the candidates
+    if (tid < 32) {
+      const uint32_t t = kth_key(n, k, [&](int i) { return (uint32_t)(s_cand[0][i] >> 32); });
+      if (tid == 0) s_thr = t, s_n = 0;
+    }
+    __syncthreads();
+    thr = s_thr;
+    for (int i = tid; i < n; i += kThreads) {
+      const uint64_t cand = s_cand[0][i];
+      if ((uint32_t)(cand >> 32) >= thr) s_cand[1][atomicAdd(&s_n, 1)] = cand;
+    }
+    __syncthreads();
+    n = s_n;
+    from = 1;
   }
-  for (int i = threadIdx.x; i < n; i += kThreads) {
-    const uint64_t mine = s_cand[i];
+  for (int i = tid; i < n; i += kThreads) {
+    const uint64_t mine = s_cand[from][i];
     int rank = 0;
-    for (int j = 0; j < n; ++j) rank += s_cand[j] > mine;
+    for (int j = 0; j < n; ++j) rank += s_cand[from][j] > mine;
     if (rank < k) {
       const int col = (int)~(uint32_t)mine;
       values[row * k + rank] = as_f(x[col]);
       indices[row * k + rank] = col;
+      // a NaN makes the sum one, +inf without a NaN makes it +inf
+      if (special && rank == 0) lse[row] = (uint32_t)(mine >> 32) == 0xffffffffu ? NAN : as_f(x[col]);
     }
   }
 }
@@ -496,17 +597,6 @@ __global__ void __launch_bounds__(kThreads) distill_kernel(const T* __restrict__
 }
 
 // ------------------------------------------------------------ distillation loss, row held in registers
-// Eight elements as they lie in memory.
-template <typename T>
-struct Raw8 {
-  uint4 u[sizeof(T) / 2];
-  __device__ __forceinline__ void load(const T* p) {
-#pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i) u[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
-  }
-  __device__ __forceinline__ void get(float* v) const { load8(reinterpret_cast<const T*>(u), v); }
-};
-
 constexpr int kEnds = 16;          // elements before the first and after the last 8-element group
 constexpr int kMaxCluster = 8;
 
@@ -944,9 +1034,12 @@ void top_logits(const at::Tensor& logits, at::Tensor& values, at::Tensor& indice
   auto s = at::cuda::getCurrentCUDAStream();
   by_type(logits.scalar_type(), [&](auto tag) {
     using E = decltype(tag);
+    // rounds in the sample: about 512 columns reach its bound
+    const int rounds = (V / 8 + kThreads - 1) / kThreads;
+    const int ns = std::max(1, std::min(rounds, (rounds * k + 511) / 512));
     auto launch = [&](auto g) {
       top_logits_kernel<E, decltype(g)::value><<<(unsigned)T, kThreads, 0, s>>>(
-          static_cast<const E*>(logits.data_ptr()), logits.stride(0), V, k, aligned8(logits), (float)(kLog2e / tau),
+          static_cast<const E*>(logits.data_ptr()), logits.stride(0), V, k, aligned8(logits), ns, (float)(kLog2e / tau),
           values.data_ptr<float>(), indices.data_ptr<int64_t>(), lse.data_ptr<float>());
     };
     // at least twice as many groups as entries keeps the candidates near 1.4 k

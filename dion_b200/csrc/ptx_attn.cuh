@@ -31,16 +31,57 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
                : "memory");
 }
 
-// D[tmem] (+)= A[tmem] * B[smem]^T, A as packed 16-bit pairs, one per 32-bit column.
-__device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
-                                            uint32_t accumulate) {
+// Shared-memory operands of the 128-byte swizzle by the low word of their
+// descriptor (make_sdesc_sw128: address and leading-dimension offset); the high
+// word (8-row stride 1024, version, layout) is the same for all of them.
+constexpr uint32_t kSdescHigh = 64u | (1u << 14) | (2u << 29);
+__device__ __forceinline__ constexpr uint32_t sdesc_low(uint32_t saddr, uint32_t lbo) {
+  return (saddr >> 4) | ((lbo >> 4) << 16);
+}
+
+// tcgen05.mma issued by the one lane whose `leader` is set, without a branch: in
+// code that one lane has branched into, the operands took their own way to
+// uniform registers and every product some 90 cycles to issue.
+//   umma_ss: D[tmem] (+)= A[smem] * B[smem]^T
+//   umma_ts: D[tmem] (+)= A[tmem] * B[smem]^T, A as packed 16-bit pairs, one per 32-bit column
+__device__ __forceinline__ void umma_ss(bool leader, uint32_t d_tmem, uint32_t a_low, uint32_t b_low, uint32_t idesc,
+                                        bool accumulate) {
   asm volatile(
       "{\n"
-      ".reg .pred P;\n"
+      ".reg .pred P, Q;\n"
+      ".reg .b64 A, B;\n"
       "setp.ne.b32 P, %4, 0;\n"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, P;\n"
+      "setp.ne.b32 Q, %5, 0;\n"
+      "mov.b64 A, {%1, %6};\n"
+      "mov.b64 B, {%2, %6};\n"
+      "@Q tcgen05.mma.cta_group::1.kind::f16 [%0], A, B, %3, P;\n"
       "}\n" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      "r"(a_low), "r"(b_low), "r"(idesc), "r"((uint32_t)accumulate), "r"((uint32_t)leader), "n"(kSdescHigh)
+      : "memory");
+}
+__device__ __forceinline__ void umma_ts(bool leader, uint32_t d_tmem, uint32_t a_tmem, uint32_t b_low, uint32_t idesc,
+                                        bool accumulate) {
+  asm volatile(
+      "{\n"
+      ".reg .pred P, Q;\n"
+      ".reg .b64 B;\n"
+      "setp.ne.b32 P, %4, 0;\n"
+      "setp.ne.b32 Q, %5, 0;\n"
+      "mov.b64 B, {%2, %6};\n"
+      "@Q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], B, %3, P;\n"
+      "}\n" ::"r"(d_tmem),
+      "r"(a_tmem), "r"(b_low), "r"(idesc), "r"((uint32_t)accumulate), "r"((uint32_t)leader), "n"(kSdescHigh)
+      : "memory");
+}
+// Arrive on `bar` once every product that this lane has issued is done.
+__device__ __forceinline__ void umma_commit_by(bool leader, uint64_t* bar) {
+  asm volatile(
+      "{\n"
+      ".reg .pred Q;\n"
+      "setp.ne.b32 Q, %1, 0;\n"
+      "@Q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n"
+      "}\n" ::"r"(smem_u32(bar)),
+      "r"((uint32_t)leader)
       : "memory");
 }
 

@@ -144,7 +144,7 @@ std::tuple<at::Tensor, at::Tensor> window_attention_fwd(const at::Tensor& q, con
   auto o = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
   auto lse = at::empty({a.b, a.hq, a.s_pad}, q.options().dtype(at::kFloat));
   if (o.numel() == 0) return {o, lse};
-  const CUtensorMap mq = head_map(q, kTile, "q"), mk = head_map(k, kTile, "k"), mv = head_map(v, kTile, "v");
+  const CUtensorMap mq = head_map(q, kTile, "q"), mk = head_map(k, kHalfTile, "k"), mv = head_map(v, kHalfTile, "v");
   by_case(q.scalar_type(), a.d, [&](auto tag, auto dp) {
     using E = decltype(tag);
     constexpr int DP = decltype(dp)::value;
@@ -181,13 +181,13 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> window_attention_bwd(const at::Te
   by_case(q.scalar_type(), a.d, [&](auto tag, auto dp) {
     using E = decltype(tag);
     constexpr int DP = decltype(dp)::value;
-    launch(window_dq_tc<E, DP>, (int64_t)a.b * a.hq * (a.s_pad / kTile), 192, DqCfg<E, DP>::kSmemBytes, st, q128, k64,
+    launch(window_dq_tc<E, DP>, (int64_t)a.b * a.hq * (a.s_pad / kTile), 576, DqCfg<E, DP>::kSmemBytes, st, q128, k64,
            v64, g128, (const E*)o.data_ptr(), (const E*)go.data_ptr(), go.stride(0), go.stride(1), go.stride(2),
            lse.data_ptr<float>(), delta.data_ptr<float>(), (E*)dq.data_ptr(), a);
     at::Tensor work;
     const int64_t slots = (int64_t)a.b * a.hkv * split.slots();
     if (slots > 0) work = at::empty({slots, 2, kTile, DP}, lse.options());
-    launch(window_dkv_tc<E, DP>, (int64_t)a.b * a.hkv * split.parts(), 320, DkvCfg<E, DP>::kSmemBytes, st, q64, k128,
+    launch(window_dkv_tc<E, DP>, (int64_t)a.b * a.hkv * split.parts(), 576, DkvCfg<E, DP>::kSmemBytes, st, q64, k128,
            v128, g64, lse.data_ptr<float>(), delta.data_ptr<float>(), (E*)dk.data_ptr(), (E*)dv.data_ptr(),
            slots > 0 ? work.data_ptr<float>() : nullptr, split, a);
     if (slots > 0) {

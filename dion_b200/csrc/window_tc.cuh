@@ -25,6 +25,12 @@ struct AttnType<__half> {
   static constexpr uint32_t kFmt = 0;
 };
 
+// The warps that issue products or hold rows run as a whole (see umma_ss; TMEM is
+// read and written by whole warps), so they wait, and give up, as a whole.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort, uint64_t limit_ns) {
+  return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, abort, limit_ns));
+}
+
 constexpr int kTile = 128;         // query rows of a CTA, and keys of a step
 constexpr int kPanel = kTile * 128;  // bytes of 128 rows of one 128-byte swizzle row (64 elements)
 
@@ -58,26 +64,27 @@ __device__ __forceinline__ uint32_t seen_mask(const WinArgs& a, int i, int k0) {
   return m;
 }
 
+constexpr int kHalfTile = 64;               // keys (forward, dQ) or queries (dK, dV) of a step
+constexpr int kHalfPanel = kHalfTile * 128;
+
 template <typename T, int DP>
 struct FwdCfg {
   static constexpr int kPanels = DP / 64;
-  static constexpr int kTileBytes = kPanels * kPanel;
-  // keys and values: two stages where two CTAs still share an SM
-  static constexpr int kStages = DP == 64 ? 2 : 1;
-  static constexpr int kSmemBytes = kTileBytes * (1 + 2 * kStages) + 1024 + 256;
+  static constexpr int kRowBytes = kPanels * kPanel;       // Q
+  static constexpr int kStepBytes = kPanels * kHalfPanel;  // K, V
+  static constexpr int kStages = DP == 64 ? 3 : 2;
+  static constexpr int kSmemBytes = kRowBytes + 2 * kStages * kStepBytes + 1024 + 256;
   static constexpr int kTmemCols = 256;
-  // columns: S [0, 128), P after it where there is room (else P lies on S), O at the end
-  static constexpr bool kOverlay = DP == 128;
-  static constexpr int kP = kOverlay ? 0 : 128;
-  static constexpr int kO = 256 - DP;
+  static constexpr int kO = 256 - DP;  // columns: two buffers of S with P on it at 0 and 64, O at the end
 };
 
-// One CTA per (128 queries, head, sequence); two CTAs share an SM, so that one's
-// products run under the other's exponentials. Warp 0 loads (TMA), warp 1 issues
-// the products, warps 2-5 hold one query row per thread.
+// One CTA per (128 queries, head, sequence), steps of 64 keys; two CTAs share an
+// SM. Warp 0 loads (TMA), warp 1 issues the products, warps 2-5 hold one query
+// row per thread. S has two buffers, so the next step's scores are there when a
+// row is done with this one's, and P V runs under the next step's exponentials.
 //
 // A row's running maximum is the reference of its exponentials. It is moved
-// only when a tile exceeds it by more than 2^8, so O in TMEM is rarely rescaled;
+// only when a step exceeds it by more than 2^8, so O in TMEM is rarely rescaled;
 // P <= 2^8 loses nothing in 16 bits (its rounding is relative) and the sum is
 // kept in fp32 from the unrounded values.
 template <typename T, int DP>
@@ -89,33 +96,35 @@ __global__ void __launch_bounds__(192, 2)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sQ = smem;
-  uint8_t* sK = sQ + Cfg::kTileBytes;
-  uint8_t* sV = sK + ST * Cfg::kTileBytes;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sV + ST * Cfg::kTileBytes);
-  uint64_t *q_full = bars, *k_full = bars + 1, *k_empty = bars + 3, *v_full = bars + 5, *v_empty = bars + 7,
-           *s_full = bars + 9, *p_full = bars + 10, *o_full = bars + 11, *drain = bars + 12;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 13);
-  volatile int* abort = reinterpret_cast<volatile int*>(bars + 14);
+  uint8_t* sK = sQ + Cfg::kRowBytes;
+  uint8_t* sV = sK + ST * Cfg::kStepBytes;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sV + ST * Cfg::kStepBytes);
+  uint64_t *q_full = bars, *k_full = bars + 1, *k_empty = bars + 4, *v_full = bars + 7, *v_empty = bars + 10,
+           *s_full = bars + 13, *p_full = bars + 15, *o_done = bars + 17, *drain = bars + 19;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 20);
+  volatile int* abort = reinterpret_cast<volatile int*>(bars + 21);
 
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
   const int h = blockIdx.x % a.hq;
   const int n_q = a.s_pad / kTile;
   const int q0 = (blockIdx.x / a.hq) % n_q * kTile;
   const int b = blockIdx.x / a.hq / n_q;
   const int hk = h / (a.hq / a.hkv);
-  const KeyTiles<kTile> tiles(a, q0);
+  const KeyTiles<kHalfTile> tiles(a, q0);
 
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < 3; ++i) {
       mbar_init(&k_full[i], 1);
       mbar_init(&k_empty[i], 1);
       mbar_init(&v_full[i], 1);
       mbar_init(&v_empty[i], 1);
     }
-    mbar_init(s_full, 1);
-    mbar_init(p_full, 4);
-    mbar_init(o_full, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 4);
+      mbar_init(&o_done[i], 1);
+    }
     mbar_init(drain, 1);
     *abort = 0;
     fence_mbar_init();
@@ -132,7 +141,7 @@ __global__ void __launch_bounds__(192, 2)
 
   if (warp == 0) {
     if (lane == 0) {
-      mbar_arrive_expect_tx(q_full, Cfg::kTileBytes);
+      mbar_arrive_expect_tx(q_full, Cfg::kRowBytes);
       for (int p = 0; p < Cfg::kPanels; ++p) tma_load_4d(&tq, q_full, sQ + p * kPanel, p * 64, q0, h, b);
       int t = 0;
       bool ok = true;
@@ -140,13 +149,13 @@ __global__ void __launch_bounds__(192, 2)
         const int st = t % ST, k0 = tiles.k0(t);
         const uint32_t ph = (t / ST) & 1;
         if (!mbar_wait_bounded(&k_empty[st], ph ^ 1, abort, limit)) { ok = false; break; }
-        mbar_arrive_expect_tx(&k_full[st], Cfg::kTileBytes);
+        mbar_arrive_expect_tx(&k_full[st], Cfg::kStepBytes);
         for (int p = 0; p < Cfg::kPanels; ++p)
-          tma_load_4d(&tk, &k_full[st], sK + st * Cfg::kTileBytes + p * kPanel, p * 64, k0, hk, b);
+          tma_load_4d(&tk, &k_full[st], sK + st * Cfg::kStepBytes + p * kHalfPanel, p * 64, k0, hk, b);
         if (!mbar_wait_bounded(&v_empty[st], ph ^ 1, abort, limit)) { ok = false; break; }
-        mbar_arrive_expect_tx(&v_full[st], Cfg::kTileBytes);
+        mbar_arrive_expect_tx(&v_full[st], Cfg::kStepBytes);
         for (int p = 0; p < Cfg::kPanels; ++p)
-          tma_load_4d(&tv, &v_full[st], sV + st * Cfg::kTileBytes + p * kPanel, p * 64, k0, hk, b);
+          tma_load_4d(&tv, &v_full[st], sV + st * Cfg::kStepBytes + p * kHalfPanel, p * 64, k0, hk, b);
       }
       if (!ok) {
         report_status(a.status, kStatusWindowProducerTimeout);
@@ -163,52 +172,47 @@ __global__ void __launch_bounds__(192, 2)
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      constexpr uint32_t kS = make_idesc(kTile, kTile, false, false, AttnType<T>::kFmt);
-      constexpr uint32_t kPV = make_idesc(kTile, DP, false, true, AttnType<T>::kFmt);
-      const uint32_t q_base = smem_u32(sQ);
-      bool ok = mbar_wait_bounded(q_full, 0, abort, limit);
-      auto scores = [&](int t) {
-        const int st = t % ST;
-        if (!mbar_wait_bounded(&k_full[st], (t / ST) & 1, abort, limit)) return false;
-        tc_fence_after();
-        const uint32_t k_base = smem_u32(sK + st * Cfg::kTileBytes);
+    const bool leader = elect_one();
+    constexpr uint32_t kS = make_idesc(kTile, kHalfTile, false, false, AttnType<T>::kFmt);
+    constexpr uint32_t kPV = make_idesc(kTile, DP, false, true, AttnType<T>::kFmt);
+    const uint32_t q_base = smem_u32(sQ);
+    bool ok = warp_wait(q_full, 0, abort, limit);
+    auto scores = [&](int t) {
+      const int st = t % ST, buf = t & 1;
+      if (!warp_wait(&k_full[st], (t / ST) & 1, abort, limit)) return false;
+      // the buffer's P of two steps ago has been read
+      if (t >= 2 && !warp_wait(&o_done[buf], ((t >> 1) - 1) & 1, abort, limit)) return false;
+      tc_fence_after();
+      const uint32_t k_base = smem_u32(sK + st * Cfg::kStepBytes);
 #pragma unroll
-        for (int k = 0; k < DP / 16; ++k) {
-          const uint32_t off = (k / 4) * kPanel + (k % 4) * 32;
-          umma_f16(tmem, make_sdesc_sw128(q_base + off, 16, 1024), make_sdesc_sw128(k_base + off, 16, 1024), kS, k != 0);
-        }
-        umma_commit(&k_empty[st]);
-        umma_commit(s_full);
-        return true;
-      };
-      if (ok) ok = scores(0);
-      for (int t = 0; t < tiles.n && ok; ++t) {
-        const int st = t % ST;
-        ok = mbar_wait_bounded(p_full, t & 1, abort, limit);
-        if (!ok) break;
-        tc_fence_after();
-        // the rows have read S; their next scores may start before this tile's P V
-        if (!Cfg::kOverlay && t + 1 < tiles.n && !scores(t + 1)) { ok = false; break; }
-        if (!mbar_wait_bounded(&v_full[st], (t / ST) & 1, abort, limit)) { ok = false; break; }
-        tc_fence_after();
-        const uint32_t v_base = smem_u32(sV + st * Cfg::kTileBytes);
-#pragma unroll
-        for (int k = 0; k < kTile / 16; ++k)
-          umma_f16_ts(tmem + Cfg::kO, tmem + Cfg::kP + k * 8, make_sdesc_sw128(v_base + k * 2048, kPanel, 1024), kPV,
-                      (t | k) != 0);
-        umma_commit(&v_empty[st]);
-        umma_commit(o_full);
-        if (Cfg::kOverlay && t + 1 < tiles.n) {
-          ok = mbar_wait_bounded(o_full, t & 1, abort, limit) && scores(t + 1);
-        }
+      for (int k = 0; k < DP / 16; ++k) {
+        const uint32_t qo = (k / 4) * kPanel + (k % 4) * 32, ko = (k / 4) * kHalfPanel + (k % 4) * 32;
+        umma_ss(leader, tmem + buf * 64, sdesc_low(q_base + qo, 16), sdesc_low(k_base + ko, 16), kS, k != 0);
       }
-      if (!ok) {
-        report_status(a.status, kStatusWindowMmaTimeout);
-        umma_commit(drain);
-        const uint64_t t0 = globaltimer_ns();
-        while (!mbar_try_wait(drain, 0) && globaltimer_ns() - t0 < 100000000ull) {
-        }
+      umma_commit_by(leader, &k_empty[st]);
+      umma_commit_by(leader, &s_full[buf]);
+      return true;
+    };
+    if (ok) ok = scores(0);
+    for (int t = 0; t < tiles.n && ok; ++t) {
+      const int st = t % ST, buf = t & 1;
+      if (t + 1 < tiles.n && !scores(t + 1)) { ok = false; break; }
+      if (!warp_wait(&p_full[buf], (t >> 1) & 1, abort, limit)) { ok = false; break; }
+      if (!warp_wait(&v_full[st], (t / ST) & 1, abort, limit)) { ok = false; break; }
+      tc_fence_after();
+      const uint32_t v_base = smem_u32(sV + st * Cfg::kStepBytes);
+#pragma unroll
+      for (int k = 0; k < kHalfTile / 16; ++k)
+        umma_ts(leader, tmem + Cfg::kO, tmem + buf * 64 + k * 8, sdesc_low(v_base + k * 2048, kHalfPanel), kPV,
+                (t | k) != 0);
+      umma_commit_by(leader, &v_empty[st]);
+      umma_commit_by(leader, &o_done[buf]);
+    }
+    if (!ok) {
+      if (lane == 0) report_status(a.status, kStatusWindowMmaTimeout);
+      umma_commit_by(leader, drain);
+      const uint64_t t0 = globaltimer_ns();
+      while (!mbar_try_wait(drain, 0) && globaltimer_ns() - t0 < 100000000ull) {
       }
     }
   } else {
@@ -219,29 +223,32 @@ __global__ void __launch_bounds__(192, 2)
     float m = -INFINITY, l = 0.f;  // reference of the exponentials (in score units), sum under it
     bool ok = true;
     for (int t = 0; t < tiles.n; ++t) {
-      const int k0 = tiles.k0(t);
-      if (!mbar_wait_bounded(s_full, t & 1, abort, limit)) { ok = false; break; }
+      const int k0 = tiles.k0(t), buf = t & 1;
+      if (!warp_wait(&s_full[buf], (t >> 1) & 1, abort, limit)) { ok = false; break; }
       tc_fence_after();
-      uint32_t x[128];
+      uint32_t x[64], pk[32];
+      auto load = [&] {
+        tmem_ld_32x32b_x32(row + buf * 64, reinterpret_cast<uint32_t(&)[32]>(x[0]));
+        tmem_ld_32x32b_x32(row + buf * 64 + 32, reinterpret_cast<uint32_t(&)[32]>(x[32]));
+        tmem_wait_ld();
+        if (!tiles.whole(a, q0, k0)) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) tmem_ld_32x32b_x32(row + j * 32, reinterpret_cast<uint32_t(&)[32]>(x[j * 32]));
-      tmem_wait_ld();
-      if (!tiles.whole(a, q0, k0)) {
+          for (int j = 0; j < 2; ++j) {
+            const uint32_t seen = seen_mask(a, i, k0 + j * 32);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t seen = seen_mask(a, i, k0 + j * 32);
-#pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (!((seen >> e) & 1u)) x[j * 32 + e] = 0xff800000u;  // -inf
+            for (int e = 0; e < 32; ++e)
+              if (!((seen >> e) & 1u)) x[j * 32 + e] = 0xff800000u;  // -inf
+          }
         }
-      }
+      };
+      load();
       float mt[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int e = 0; e < 128; ++e) mt[e % 4] = fmaxf(mt[e % 4], __uint_as_float(x[e]));
+      for (int e = 0; e < 64; ++e) mt[e % 4] = fmaxf(mt[e % 4], __uint_as_float(x[e]));
       const float top = fmaxf(fmaxf(mt[0], mt[1]), fmaxf(mt[2], mt[3]));
-      // move the reference where this tile exceeds it by more than 8 powers of two
+      // move the reference where this step exceeds it by more than 8 powers of two
       float f = 1.f;
-      if ((top - m) * c > 8.f) {  // also the first visible tile (m = -inf); never while nothing is visible
+      if ((top - m) * c > 8.f) {  // also the first visible step (m = -inf); never while nothing is visible
         f = ex2((m - top) * c);
         m = top;
         l *= f;
@@ -249,37 +256,35 @@ __global__ void __launch_bounds__(192, 2)
       const float mc = m == -INFINITY ? 0.f : m * c;
       float sum[4] = {};
 #pragma unroll
-      for (int e = 0; e < 128; e += 2) {
+      for (int e = 0; e < 64; e += 2) {
         const float p0 = ex2(__uint_as_float(x[e]) * c - mc), p1 = ex2(__uint_as_float(x[e + 1]) * c - mc);
-        sum[(e / 2) % 2 * 2] += p0;
-        sum[(e / 2) % 2 * 2 + 1] += p1;
-        x[e / 2] = pack2(p0, p1, T{});
+        sum[e % 4] += p0;
+        sum[e % 4 + 1] += p1;
+        pk[e / 2] = pack2(p0, p1, T{});
       }
       l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-      if (t > 0) {
-        // P's place and O are free once the tile before is done
-        if (!mbar_wait_bounded(o_full, (t - 1) & 1, abort, limit)) { ok = false; break; }
+      if (t > 0 && __any_sync(0xffffffffu, f != 1.f)) {
+        // O is free once the step before is done
+        if (!warp_wait(&o_done[buf ^ 1], ((t - 1) >> 1) & 1, abort, limit)) { ok = false; break; }
         tc_fence_after();
-        if (__any_sync(0xffffffffu, f != 1.f)) {
 #pragma unroll
-          for (int j = 0; j < DP / 32; ++j) {
-            uint32_t y[32];
-            tmem_ld_32x32b_x32(row + Cfg::kO + j * 32, y);
-            tmem_wait_ld();
+        for (int j = 0; j < DP / 32; ++j) {
+          uint32_t y[32];
+          tmem_ld_32x32b_x32(row + Cfg::kO + j * 32, y);
+          tmem_wait_ld();
 #pragma unroll
-            for (int e = 0; e < 32; ++e) y[e] = __float_as_uint(__uint_as_float(y[e]) * f);
-            tmem_st_32x32b_x32(row + Cfg::kO + j * 32, y);
-          }
+          for (int e = 0; e < 32; ++e) y[e] = __float_as_uint(__uint_as_float(y[e]) * f);
+          tmem_st_32x32b_x32(row + Cfg::kO + j * 32, y);
         }
       }
-      tmem_st_32x32b_x32(row + Cfg::kP, x);
-      tmem_st_32x32b_x32(row + Cfg::kP + 32, x + 32);
+      tmem_st_32x32b_x32(row + buf * 64, pk);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(p_full);
+      if (lane == 0) mbar_arrive(&p_full[buf]);
     }
-    if (ok) ok = mbar_wait_bounded(o_full, (tiles.n - 1) & 1, abort, limit);
+    // the last step's products stand for all before them
+    if (ok) ok = warp_wait(&o_done[(tiles.n - 1) & 1], ((tiles.n - 1) >> 1) & 1, abort, limit);
     if (!ok) {
       if (lane == 0) report_status(a.status, kStatusWindowSoftmaxTimeout);
     } else {
@@ -315,29 +320,31 @@ __global__ void __launch_bounds__(192, 2)
 }
 
 // ------------------------------------------------------------ backward: dQ
-constexpr int kHalfTile = 64;               // keys (dQ) or queries (dK, dV) of a step
-constexpr int kHalfPanel = kHalfTile * 128;
+// Column of the 16 elements that product k of a step reads. Each of the two
+// threads of a row packs its 32 elements into the first 16 of the 32 columns
+// that it has read itself, so neither waits for the other.
+__device__ constexpr int half_col(int k) { return k / 2 * 32 + k % 2 * 8; }
 
 template <typename T, int DP>
 struct DqCfg {
   static constexpr int kPanels = DP / 64;
   static constexpr int kRowBytes = kPanels * kPanel;       // Q, dO
   static constexpr int kStepBytes = kPanels * kHalfPanel;  // K, V
-  static constexpr int kStages = DP == 64 ? 2 : 1;
-  static constexpr int kSmemBytes = 2 * kRowBytes + 2 * kStages * kStepBytes + 1024 + 256;
-  static constexpr int kTmemCols = 256;
-  // columns: S [0, 64), dP [64, 128), dS behind them where there is room (else on S), dQ at the end
-  static constexpr bool kOverlay = DP == 128;
-  static constexpr int kDS = kOverlay ? 0 : 128;
-  static constexpr int kDQ = 256 - DP;
+  static constexpr int kStages = 4;
+  static constexpr int kSmemBytes = 2 * kRowBytes + 2 * kStages * kStepBytes + 1024 + 256 + kTile * 4;
+  static constexpr int kTmemCols = 512;
+  static constexpr int kBufs = 3;    // columns: three buffers of (S, dP) with dS on S, dQ behind them
+  static constexpr int kDQ = 384;
 };
 
-// One CTA per (128 queries, head, sequence), two to an SM: S and dP by the
-// tensor cores, dS = P o (dP - delta) by one thread per query row, dQ += dS K
-// with dS read from TMEM. delta is taken here from O and dO and kept for the
+// One CTA per (128 queries, head, sequence), one to an SM: S and dP by the
+// tensor cores, dS = P o (dP - delta), dQ += dS K with dS read from TMEM. Two
+// groups of eight warps take the steps of 64 keys in turn, two threads to a row
+// with half of the keys each; with three buffers the scores of two more steps
+// are under way meanwhile. delta is taken here from O and dO and kept for the
 // dK / dV kernel (0 behind the last position).
 template <typename T, int DP>
-__global__ void __launch_bounds__(192, 2)
+__global__ void __launch_bounds__(576, 1)
     window_dq_tc(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                  const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap tg,
                  const T* __restrict__ o, const T* __restrict__ go, int64_t go_b, int64_t go_s, int64_t go_h,
@@ -351,12 +358,13 @@ __global__ void __launch_bounds__(192, 2)
   uint8_t* sK = sG + Cfg::kRowBytes;
   uint8_t* sV = sK + ST * Cfg::kStepBytes;
   uint64_t* bars = reinterpret_cast<uint64_t*>(sV + ST * Cfg::kStepBytes);
-  uint64_t *q_full = bars, *k_full = bars + 1, *k_empty = bars + 3, *v_full = bars + 5, *v_empty = bars + 7,
-           *s_full = bars + 9, *p_full = bars + 10, *o_full = bars + 11, *drain = bars + 12;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 13);
-  volatile int* abort = reinterpret_cast<volatile int*>(bars + 14);
+  uint64_t *q_full = bars, *k_full = bars + 1, *k_empty = bars + 5, *s_full = bars + 9, *p_full = bars + 12,
+           *acc_done = bars + 15, *all_done = bars + 18, *drain = bars + 19;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 20);
+  volatile int* abort = reinterpret_cast<volatile int*>(bars + 21);
+  float* s_delta = reinterpret_cast<float*>(bars + 24);
 
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
   const int h = blockIdx.x % a.hq;
   const int n_q = a.s_pad / kTile;
   const int q0 = (blockIdx.x / a.hq) % n_q * kTile;
@@ -366,15 +374,16 @@ __global__ void __launch_bounds__(192, 2)
 
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < ST; ++i) {
       mbar_init(&k_full[i], 1);
       mbar_init(&k_empty[i], 1);
-      mbar_init(&v_full[i], 1);
-      mbar_init(&v_empty[i], 1);
     }
-    mbar_init(s_full, 1);
-    mbar_init(p_full, 4);
-    mbar_init(o_full, 1);
+    for (int i = 0; i < Cfg::kBufs; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 8);
+      mbar_init(&acc_done[i], 1);
+    }
+    mbar_init(all_done, 1);
     mbar_init(drain, 1);
     *abort = 0;
     fence_mbar_init();
@@ -401,144 +410,144 @@ __global__ void __launch_bounds__(192, 2)
       for (; t < tiles.n; ++t) {
         const int st = t % ST, k0 = tiles.k0(t);
         const uint32_t ph = (t / ST) & 1;
-        // V is free once dP is done, K only after dQ
-        if (!mbar_wait_bounded(&v_empty[st], ph ^ 1, abort, limit)) { ok = false; break; }
-        mbar_arrive_expect_tx(&v_full[st], Cfg::kStepBytes);
-        for (int p = 0; p < Cfg::kPanels; ++p)
-          tma_load_4d(&tv, &v_full[st], sV + st * Cfg::kStepBytes + p * kHalfPanel, p * 64, k0, hk, b);
         if (!mbar_wait_bounded(&k_empty[st], ph ^ 1, abort, limit)) { ok = false; break; }
-        mbar_arrive_expect_tx(&k_full[st], Cfg::kStepBytes);
-        for (int p = 0; p < Cfg::kPanels; ++p)
+        mbar_arrive_expect_tx(&k_full[st], 2 * Cfg::kStepBytes);
+        for (int p = 0; p < Cfg::kPanels; ++p) {
           tma_load_4d(&tk, &k_full[st], sK + st * Cfg::kStepBytes + p * kHalfPanel, p * 64, k0, hk, b);
+          tma_load_4d(&tv, &k_full[st], sV + st * Cfg::kStepBytes + p * kHalfPanel, p * 64, k0, hk, b);
+        }
       }
       if (!ok) {
         report_status(a.status, kStatusWindowProducerTimeout);
         const uint64_t t0 = globaltimer_ns();
         while (!mbar_try_wait(q_full, 0) && globaltimer_ns() - t0 < 100000000ull) {
         }
-        for (int i = max(0, t - ST); i <= t; ++i) {
+        for (int i = max(0, t - ST); i < t; ++i)
           while (!mbar_try_wait(&k_full[i % ST], (i / ST) & 1) && globaltimer_ns() - t0 < 100000000ull) {
           }
-          while (!mbar_try_wait(&v_full[i % ST], (i / ST) & 1) && globaltimer_ns() - t0 < 100000000ull) {
-          }
-        }
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      constexpr uint32_t kS = make_idesc(kTile, kHalfTile, false, false, AttnType<T>::kFmt);
-      constexpr uint32_t kD = make_idesc(kTile, DP, false, true, AttnType<T>::kFmt);
-      const uint32_t q_base = smem_u32(sQ), g_base = smem_u32(sG);
-      bool ok = mbar_wait_bounded(q_full, 0, abort, limit);
-      auto scores = [&](int t) {
-        const int st = t % ST;
-        const uint32_t ph = (t / ST) & 1;
-        if (!mbar_wait_bounded(&v_full[st], ph, abort, limit) || !mbar_wait_bounded(&k_full[st], ph, abort, limit))
-          return false;
-        tc_fence_after();
-        const uint32_t k_base = smem_u32(sK + st * Cfg::kStepBytes), v_base = smem_u32(sV + st * Cfg::kStepBytes);
+    const bool leader = elect_one();
+    constexpr uint32_t kS = make_idesc(kTile, kHalfTile, false, false, AttnType<T>::kFmt);
+    constexpr uint32_t kD = make_idesc(kTile, DP, false, true, AttnType<T>::kFmt);
+    const uint32_t q_base = smem_u32(sQ), g_base = smem_u32(sG);
+    bool ok = warp_wait(q_full, 0, abort, limit);
+    auto scores = [&](int t) {
+      const int st = t % ST, buf = t % Cfg::kBufs;
+      if (!warp_wait(&k_full[st], (t / ST) & 1, abort, limit)) return false;
+      // the buffer's dS of three steps ago has been read
+      if (t >= Cfg::kBufs && !warp_wait(&acc_done[buf], (t / Cfg::kBufs - 1) & 1, abort, limit)) return false;
+      tc_fence_after();
+      const uint32_t k_base = smem_u32(sK + st * Cfg::kStepBytes), v_base = smem_u32(sV + st * Cfg::kStepBytes);
+      const uint32_t d = tmem + buf * 128;
 #pragma unroll
-        for (int k = 0; k < DP / 16; ++k) {
-          const uint32_t qo = (k / 4) * kPanel + (k % 4) * 32, ko = (k / 4) * kHalfPanel + (k % 4) * 32;
-          umma_f16(tmem, make_sdesc_sw128(q_base + qo, 16, 1024), make_sdesc_sw128(k_base + ko, 16, 1024), kS, k != 0);
-        }
-#pragma unroll
-        for (int k = 0; k < DP / 16; ++k) {
-          const uint32_t qo = (k / 4) * kPanel + (k % 4) * 32, ko = (k / 4) * kHalfPanel + (k % 4) * 32;
-          umma_f16(tmem + 64, make_sdesc_sw128(g_base + qo, 16, 1024), make_sdesc_sw128(v_base + ko, 16, 1024), kS,
-                   k != 0);
-        }
-        umma_commit(&v_empty[st]);
-        umma_commit(s_full);
-        return true;
-      };
-      if (ok) ok = scores(0);
-      for (int t = 0; t < tiles.n && ok; ++t) {
-        const int st = t % ST;
-        ok = mbar_wait_bounded(p_full, t & 1, abort, limit);
-        if (!ok) break;
-        tc_fence_after();
-        if (!Cfg::kOverlay && t + 1 < tiles.n && !scores(t + 1)) { ok = false; break; }
-        const uint32_t k_base = smem_u32(sK + st * Cfg::kStepBytes);
-#pragma unroll
-        for (int k = 0; k < kHalfTile / 16; ++k)
-          umma_f16_ts(tmem + Cfg::kDQ, tmem + Cfg::kDS + k * 8, make_sdesc_sw128(k_base + k * 2048, kHalfPanel, 1024), kD,
-                      (t | k) != 0);
-        umma_commit(&k_empty[st]);
-        umma_commit(o_full);
-        if (Cfg::kOverlay && t + 1 < tiles.n) ok = mbar_wait_bounded(o_full, t & 1, abort, limit) && scores(t + 1);
+      for (int k = 0; k < DP / 16; ++k) {
+        const uint32_t qo = (k / 4) * kPanel + (k % 4) * 32, ko = (k / 4) * kHalfPanel + (k % 4) * 32;
+        umma_ss(leader, d, sdesc_low(q_base + qo, 16), sdesc_low(k_base + ko, 16), kS, k != 0);
       }
-      if (!ok) {
-        report_status(a.status, kStatusWindowMmaTimeout);
-        umma_commit(drain);
-        const uint64_t t0 = globaltimer_ns();
-        while (!mbar_try_wait(drain, 0) && globaltimer_ns() - t0 < 100000000ull) {
-        }
+#pragma unroll
+      for (int k = 0; k < DP / 16; ++k) {
+        const uint32_t qo = (k / 4) * kPanel + (k % 4) * 32, ko = (k / 4) * kHalfPanel + (k % 4) * 32;
+        umma_ss(leader, d + 64, sdesc_low(g_base + qo, 16), sdesc_low(v_base + ko, 16), kS, k != 0);
+      }
+      umma_commit_by(leader, &s_full[buf]);
+      return true;
+    };
+    for (int t = 0; t < min(tiles.n, Cfg::kBufs - 1) && ok; ++t) ok = scores(t);
+    for (int t = 0; t < tiles.n && ok; ++t) {
+      const int st = t % ST, buf = t % Cfg::kBufs;
+      if (!warp_wait(&p_full[buf], (t / Cfg::kBufs) & 1, abort, limit)) { ok = false; break; }
+      tc_fence_after();
+      const uint32_t k_base = smem_u32(sK + st * Cfg::kStepBytes);
+#pragma unroll
+      for (int k = 0; k < kHalfTile / 16; ++k)
+        umma_ts(leader, tmem + Cfg::kDQ, tmem + buf * 128 + half_col(k), sdesc_low(k_base + k * 2048, kHalfPanel), kD,
+                (t | k) != 0);
+      umma_commit_by(leader, &k_empty[st]);
+      umma_commit_by(leader, &acc_done[buf]);
+      if (t + Cfg::kBufs - 1 < tiles.n) ok = scores(t + Cfg::kBufs - 1);
+    }
+    if (ok) {
+      umma_commit_by(leader, all_done);
+    } else {
+      if (lane == 0) report_status(a.status, kStatusWindowMmaTimeout);
+      umma_commit_by(leader, drain);
+      const uint64_t t0 = globaltimer_ns();
+      while (!mbar_try_wait(drain, 0) && globaltimer_ns() - t0 < 100000000ull) {
       }
     }
   } else {
-    const int quarter = warp & 3;
-    const int i = q0 + quarter * 32 + lane;
+    const int quarter = warp & 3, which = (warp - 2) / 8, half = (warp - 2) / 4 % 2;
+    const int r = quarter * 32 + lane, i = q0 + r;
     const uint32_t row = tmem + ((uint32_t)(quarter * 32) << 16);
     const float c = a.scale_log2;
-    const int64_t at = ((int64_t)b * a.hq + h) * a.s_pad + i;
-    const float L = lse[at];
-    float dl = 0.f;
-    if (i < a.s) {
-      const T* orow = o + (((int64_t)b * a.s + i) * a.hq + h) * a.d;
-      const T* grow = go + b * go_b + i * go_s + h * go_h;
-      for (int e = 0; e < a.d; e += 8) {
-        const uint4 ou = *reinterpret_cast<const uint4*>(orow + e), gu = *reinterpret_cast<const uint4*>(grow + e);
-        const T *op = reinterpret_cast<const T*>(&ou), *gp = reinterpret_cast<const T*>(&gu);
+    const int64_t at = ((int64_t)b * a.hq + h) * a.s_pad + q0;
+    const float L = lse[at + r];
+    {
+      // delta of 8 rows per warp, DP / 8 lanes to a row
+      constexpr int kLanes = DP / 8, kRows = 32 / kLanes;
+      const int col = lane % kLanes * 8;
+      float v[8 / kRows];
 #pragma unroll
-        for (int n = 0; n < 8; ++n) dl += (float)op[n] * (float)gp[n];
-      }
-    }
-    delta[at] = dl;
-    bool ok = true;
-    for (int t = 0; t < tiles.n; ++t) {
-      const int k0 = tiles.k0(t);
-      if (!mbar_wait_bounded(s_full, t & 1, abort, limit)) { ok = false; break; }
-      tc_fence_after();
-      uint32_t x[64], y[64];
+      for (int n = 0; n < 8 / kRows; ++n) {
+        const int rr = q0 + (warp - 2) * 8 + n * kRows + lane / kLanes;
+        v[n] = 0.f;
+        if (rr < a.s && col < a.d) {
+          const uint4 ou = *reinterpret_cast<const uint4*>(o + (((int64_t)b * a.s + rr) * a.hq + h) * a.d + col);
+          const uint4 gu = *reinterpret_cast<const uint4*>(go + b * go_b + rr * go_s + h * go_h + col);
+          const T *op = reinterpret_cast<const T*>(&ou), *gp = reinterpret_cast<const T*>(&gu);
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        tmem_ld_32x32b_x32(row + j * 32, reinterpret_cast<uint32_t(&)[32]>(x[j * 32]));
-        tmem_ld_32x32b_x32(row + 64 + j * 32, reinterpret_cast<uint32_t(&)[32]>(y[j * 32]));
-      }
-      tmem_wait_ld();
-      if (!tiles.whole(a, q0, k0)) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const uint32_t seen = seen_mask(a, i, k0 + j * 32);
-#pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (!((seen >> e) & 1u)) x[j * 32 + e] = 0xff800000u;
+          for (int e = 0; e < 8; ++e) v[n] += (float)op[e] * (float)gp[e];
         }
       }
 #pragma unroll
-      for (int e = 0; e < 64; e += 2) {
+      for (int n = 0; n < 8 / kRows; ++n) {
+#pragma unroll
+        for (int m = kLanes / 2; m > 0; m >>= 1) v[n] += __shfl_xor_sync(0xffffffffu, v[n], m);
+        const int rr = (warp - 2) * 8 + n * kRows + lane / kLanes;
+        if (col == 0) {
+          s_delta[rr] = v[n];
+          delta[at + rr] = v[n];
+        }
+      }
+      asm volatile("bar.sync 1, 512;" ::: "memory");
+    }
+    const float dl = s_delta[r];
+    bool ok = true;
+    for (int t = which; t < tiles.n; t += 2) {
+      const int k0 = tiles.k0(t), buf = t % Cfg::kBufs;
+      const uint32_t at_buf = row + buf * 128 + half * 32;
+      if (!warp_wait(&s_full[buf], (t / Cfg::kBufs) & 1, abort, limit)) { ok = false; break; }
+      tc_fence_after();
+      uint32_t x[32], y[32];
+      tmem_ld_32x32b_x32(at_buf, x);
+      tmem_ld_32x32b_x32(at_buf + 64, y);
+      tmem_wait_ld();
+      if (!tiles.whole(a, q0, k0)) {
+        const uint32_t seen = seen_mask(a, i, k0 + half * 32);
+#pragma unroll
+        for (int e = 0; e < 32; ++e)
+          if (!((seen >> e) & 1u)) x[e] = 0xff800000u;
+      }
+#pragma unroll
+      for (int e = 0; e < 32; e += 2) {
         const float p0 = ex2(__uint_as_float(x[e]) * c - L), p1 = ex2(__uint_as_float(x[e + 1]) * c - L);
         x[e / 2] = pack2(p0 * (__uint_as_float(y[e]) - dl), p1 * (__uint_as_float(y[e + 1]) - dl), T{});
       }
-      if (!Cfg::kOverlay && t > 0) {  // dS's place is free once the step before is done
-        if (!mbar_wait_bounded(o_full, (t - 1) & 1, abort, limit)) { ok = false; break; }
-        tc_fence_after();
-      }
-      tmem_st_32x32b_x32(row + Cfg::kDS, x);
+      tmem_st_32x32b_x16(at_buf, x);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(p_full);
+      if (lane == 0) mbar_arrive(&p_full[buf]);
     }
-    if (ok) ok = mbar_wait_bounded(o_full, (tiles.n - 1) & 1, abort, limit);
+    if (ok) ok = warp_wait(all_done, 0, abort, limit);
     if (!ok) {
       if (lane == 0) report_status(a.status, kStatusWindowSoftmaxTimeout);
     } else {
       tc_fence_after();
       T* out = dq + (((int64_t)b * a.s + i) * a.hq + h) * a.d;
-#pragma unroll
-      for (int j = 0; j < DP / 32; ++j) {
+      for (int j = which * 2 + half; j < DP / 32; j += 4) {  // a quarter of the row's columns
         uint32_t y[32];
         tmem_ld_32x32b_x32(row + Cfg::kDQ + j * 32, y);
         tmem_wait_ld();
@@ -597,16 +606,18 @@ struct DkvCfg {
   static constexpr int kStatBytes = kHalfTile * 4;
   static constexpr int kSmemBytes = 2 * kRowBytes + kStages * (2 * kStepBytes + 2 * kStatBytes) + 1024 + 512;
   static constexpr int kTmemCols = 512;
-  // columns: two buffers of (S^T, dP^T) with P^T and dS^T on them, then dV and dK
-  static constexpr int kDV = 256, kDK = 256 + DP;
+  // columns: buffers of (S^T, dP^T) with P^T and dS^T on them, then dV and dK
+  static constexpr int kBufs = DP == 64 ? 3 : 2;
+  static constexpr int kDV = kBufs * 128, kDK = kDV + DP;
 };
 
 // One CTA per (128 keys, key head, sequence, part). With the keys as rows, P^T
 // and dS^T come out of TMEM in the place where dV += P^T dO and dK += dS^T Q
 // want their A operand, so neither passes through shared memory. Two groups of
-// four warps take the steps in turn, each with its own buffer.
+// eight warps take the steps in turn, each with its own buffer; within a group
+// two threads share a key row, half of the step's queries each.
 template <typename T, int DP>
-__global__ void __launch_bounds__(320, 1)
+__global__ void __launch_bounds__(576, 1)
     window_dkv_tc(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                   const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap tg,
                   const float* __restrict__ lse, const float* __restrict__ delta, T* __restrict__ dk,
@@ -622,12 +633,12 @@ __global__ void __launch_bounds__(320, 1)
   float* sL = reinterpret_cast<float*>(sG + ST * Cfg::kStepBytes);
   float* sD = sL + ST * kHalfTile;
   uint64_t* bars = reinterpret_cast<uint64_t*>(sD + ST * kHalfTile);
-  uint64_t *k_full = bars, *q_full = bars + 1, *q_empty = bars + 5, *s_full = bars + 9, *p_full = bars + 11,
-           *acc_done = bars + 13, *all_done = bars + 15, *drain = bars + 16;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 17);
-  volatile int* abort = reinterpret_cast<volatile int*>(bars + 18);
+  uint64_t *k_full = bars, *q_full = bars + 1, *q_empty = bars + 5, *s_full = bars + 9, *p_full = bars + 12,
+           *acc_done = bars + 15, *all_done = bars + 18, *drain = bars + 19;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 20);
+  volatile int* abort = reinterpret_cast<volatile int*>(bars + 21);
 
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
   const int hk = blockIdx.x % a.hkv, group = a.hq / a.hkv;
   const int part = (blockIdx.x / a.hkv) % split.parts();
   const int b = blockIdx.x / a.hkv / split.parts();
@@ -649,9 +660,9 @@ __global__ void __launch_bounds__(320, 1)
       mbar_init(&q_full[i], 1);
       mbar_init(&q_empty[i], 1);
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < Cfg::kBufs; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 4);
+      mbar_init(&p_full[i], 8);
       mbar_init(&acc_done[i], 1);
     }
     mbar_init(all_done, 1);
@@ -702,88 +713,92 @@ __global__ void __launch_bounds__(320, 1)
       }
     }
   } else if (warp == 1) {
-    if (lane == 0 && n > 0) {
+    if (n > 0) {
+      const bool leader = elect_one();
       constexpr uint32_t kS = make_idesc(kTile, kHalfTile, false, false, AttnType<T>::kFmt);
       constexpr uint32_t kD = make_idesc(kTile, DP, false, true, AttnType<T>::kFmt);
       const uint32_t k_base = smem_u32(sK), v_base = smem_u32(sV);
-      bool ok = mbar_wait_bounded(k_full, 0, abort, limit);
+      bool ok = warp_wait(k_full, 0, abort, limit);
       auto scores = [&](int t) {
-        const int st = t % ST, buf = t & 1;
-        if (!mbar_wait_bounded(&q_full[st], (t / ST) & 1, abort, limit)) return false;
-        // the buffer's P^T and dS^T of two steps ago have been read
-        if (t >= 2 && !mbar_wait_bounded(&acc_done[buf], ((t >> 1) - 1) & 1, abort, limit)) return false;
+        const int st = t % ST, buf = t % Cfg::kBufs;
+        if (!warp_wait(&q_full[st], (t / ST) & 1, abort, limit)) return false;
+        // the buffer's P^T and dS^T of the step before in it have been read
+        if (t >= Cfg::kBufs && !warp_wait(&acc_done[buf], (t / Cfg::kBufs - 1) & 1, abort, limit)) return false;
         tc_fence_after();
         const uint32_t q_base = smem_u32(sQ + st * Cfg::kStepBytes), g_base = smem_u32(sG + st * Cfg::kStepBytes);
         const uint32_t d = tmem + buf * 128;
 #pragma unroll
         for (int k = 0; k < DP / 16; ++k) {
           const uint32_t ko = (k / 4) * kPanel + (k % 4) * 32, qo = (k / 4) * kHalfPanel + (k % 4) * 32;
-          umma_f16(d, make_sdesc_sw128(k_base + ko, 16, 1024), make_sdesc_sw128(q_base + qo, 16, 1024), kS, k != 0);
+          umma_ss(leader, d, sdesc_low(k_base + ko, 16), sdesc_low(q_base + qo, 16), kS, k != 0);
         }
 #pragma unroll
         for (int k = 0; k < DP / 16; ++k) {
           const uint32_t ko = (k / 4) * kPanel + (k % 4) * 32, qo = (k / 4) * kHalfPanel + (k % 4) * 32;
-          umma_f16(d + 64, make_sdesc_sw128(v_base + ko, 16, 1024), make_sdesc_sw128(g_base + qo, 16, 1024), kS, k != 0);
+          umma_ss(leader, d + 64, sdesc_low(v_base + ko, 16), sdesc_low(g_base + qo, 16), kS, k != 0);
         }
-        umma_commit(&s_full[buf]);
+        umma_commit_by(leader, &s_full[buf]);
         return true;
       };
-      if (ok) ok = scores(0);
+      // Scores run ahead of the steps' sums: by two steps with three buffers. With two
+      // they have to come before the sums of the step that the other group works on.
+      constexpr int kAhead = Cfg::kBufs - 1;
+      for (int t = 0; t < min(n, kAhead) && ok; ++t) ok = scores(t);
       for (int t = 0; t < n && ok; ++t) {
-        const int st = t % ST, buf = t & 1;
-        if (t + 1 < n && !scores(t + 1)) { ok = false; break; }
-        if (!mbar_wait_bounded(&p_full[buf], (t >> 1) & 1, abort, limit)) { ok = false; break; }
+        const int st = t % ST, buf = t % Cfg::kBufs;
+        if (Cfg::kBufs == 2 && t + 1 < n && !scores(t + 1)) { ok = false; break; }
+        if (!warp_wait(&p_full[buf], (t / Cfg::kBufs) & 1, abort, limit)) { ok = false; break; }
         tc_fence_after();
         const uint32_t q_base = smem_u32(sQ + st * Cfg::kStepBytes), g_base = smem_u32(sG + st * Cfg::kStepBytes);
         const uint32_t d = tmem + buf * 128;
 #pragma unroll
         for (int k = 0; k < kHalfTile / 16; ++k)
-          umma_f16_ts(tmem + Cfg::kDV, d + k * 8, make_sdesc_sw128(g_base + k * 2048, kHalfPanel, 1024), kD, (t | k) != 0);
+          umma_ts(leader, tmem + Cfg::kDV, d + half_col(k), sdesc_low(g_base + k * 2048, kHalfPanel), kD, (t | k) != 0);
 #pragma unroll
         for (int k = 0; k < kHalfTile / 16; ++k)
-          umma_f16_ts(tmem + Cfg::kDK, d + 64 + k * 8, make_sdesc_sw128(q_base + k * 2048, kHalfPanel, 1024), kD,
+          umma_ts(leader, tmem + Cfg::kDK, d + 64 + half_col(k), sdesc_low(q_base + k * 2048, kHalfPanel), kD,
                       (t | k) != 0);
-        umma_commit(&q_empty[st]);
-        umma_commit(&acc_done[buf]);
+        umma_commit_by(leader, &q_empty[st]);
+        umma_commit_by(leader, &acc_done[buf]);
+        if (Cfg::kBufs > 2 && t + kAhead < n) ok = scores(t + kAhead);
       }
       if (ok) {
-        umma_commit(all_done);
+        umma_commit_by(leader, all_done);
       } else {
-        report_status(a.status, kStatusWindowMmaTimeout);
-        umma_commit(drain);
+        if (lane == 0) report_status(a.status, kStatusWindowMmaTimeout);
+        umma_commit_by(leader, drain);
         const uint64_t t0 = globaltimer_ns();
         while (!mbar_try_wait(drain, 0) && globaltimer_ns() - t0 < 100000000ull) {
         }
       }
     }
   } else {
-    const int quarter = warp & 3, which = (warp - 2) / 4;
+    const int quarter = warp & 3, which = (warp - 2) / 8, half = (warp - 2) / 4 % 2;
     const int r = quarter * 32 + lane, j = k0 + r;
     const uint32_t row = tmem + ((uint32_t)(quarter * 32) << 16);
-    const uint32_t buf = row + which * 128;
     const float c = a.scale_log2;
     bool ok = true;
     for (int t = which; t < n; t += 2) {
       const int st = t % ST, q0 = (q_first + (lo + t) % nq) * kHalfTile;
-      if (!mbar_wait_bounded(&s_full[which], (t >> 1) & 1, abort, limit)) { ok = false; break; }
+      const int nbuf = t % Cfg::kBufs;
+      const uint32_t buf = row + nbuf * 128;
+      if (!warp_wait(&s_full[nbuf], (t / Cfg::kBufs) & 1, abort, limit)) { ok = false; break; }
       tc_fence_after();
-      uint32_t x[64], y[64];
-#pragma unroll
-      for (int n2 = 0; n2 < 2; ++n2) {
-        tmem_ld_32x32b_x32(buf + n2 * 32, reinterpret_cast<uint32_t(&)[32]>(x[n2 * 32]));
-        tmem_ld_32x32b_x32(buf + 64 + n2 * 32, reinterpret_cast<uint32_t(&)[32]>(y[n2 * 32]));
-      }
+      uint32_t x[32], y[32];
+      tmem_ld_32x32b_x32(buf + half * 32, x);
+      tmem_ld_32x32b_x32(buf + 64 + half * 32, y);
       tmem_wait_ld();
       // queries q0 + e that see key j: e in [j - q0, j + window - q0), without an end for first tokens
       if (!(q0 >= k0 + kTile - 1 && (q0 + kHalfTile - 1 - k0 < a.window || k0 + kTile <= a.sinks))) {
-        const int e0 = j - q0, e1 = j < a.sinks ? kHalfTile : (int)min((int64_t)kHalfTile, (int64_t)j + a.window - q0);
+        const int e0 = j - q0 - half * 32;
+        const int e1 = j < a.sinks ? kHalfTile : (int)min((int64_t)kHalfTile, (int64_t)j + a.window - q0 - half * 32);
 #pragma unroll
-        for (int e = 0; e < 64; ++e)
+        for (int e = 0; e < 32; ++e)
           if (e < e0 || e >= e1) x[e] = 0xff800000u;
       }
-      const float *pl = sL + st * kHalfTile, *pd = sD + st * kHalfTile;
+      const float *pl = sL + st * kHalfTile + half * 32, *pd = sD + st * kHalfTile + half * 32;
 #pragma unroll
-      for (int e = 0; e < 64; e += 4) {
+      for (int e = 0; e < 32; e += 4) {
         const float4 L = *reinterpret_cast<const float4*>(pl + e), D = *reinterpret_cast<const float4*>(pd + e);
         const float p0 = ex2(__uint_as_float(x[e]) * c - L.x), p1 = ex2(__uint_as_float(x[e + 1]) * c - L.y);
         const float p2 = ex2(__uint_as_float(x[e + 2]) * c - L.z), p3 = ex2(__uint_as_float(x[e + 3]) * c - L.w);
@@ -792,19 +807,19 @@ __global__ void __launch_bounds__(320, 1)
         y[e / 2] = pack2(p0 * (__uint_as_float(y[e]) - D.x), p1 * (__uint_as_float(y[e + 1]) - D.y), T{});
         y[e / 2 + 1] = pack2(p2 * (__uint_as_float(y[e + 2]) - D.z), p3 * (__uint_as_float(y[e + 3]) - D.w), T{});
       }
-      tmem_st_32x32b_x32(buf, x);
-      tmem_st_32x32b_x32(buf + 64, y);
+      tmem_st_32x32b_x16(buf + half * 32, x);
+      tmem_st_32x32b_x16(buf + 64 + half * 32, y);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[which]);
+      if (lane == 0) mbar_arrive(&p_full[nbuf]);
     }
-    if (ok && n > 0) ok = mbar_wait_bounded(all_done, 0, abort, limit);
+    if (ok && n > 0) ok = warp_wait(all_done, 0, abort, limit);
     if (!ok) {
       if (lane == 0) report_status(a.status, kStatusWindowSoftmaxTimeout);
     } else {
       tc_fence_after();
-      // the first group stores dV, the second dK
+      // the first group stores dV, the second dK, each thread half of a row
       const uint32_t acc = row + (which == 0 ? Cfg::kDV : Cfg::kDK);
       const float f = which == 0 ? 1.f : a.scale;
       T* out = (which == 0 ? dv : dk) + (((int64_t)b * a.s + j) * a.hkv + hk) * a.d;
@@ -813,7 +828,7 @@ __global__ void __launch_bounds__(320, 1)
         slot = work + ((((int64_t)b * a.hkv + hk) * split.slots() + split.slot(tile) + mine) * 2 + which) * kTile * DP +
                (int64_t)r * DP;
 #pragma unroll
-      for (int j2 = 0; j2 < DP / 32; ++j2) {
+      for (int j2 = half * (DP / 64); j2 < (half + 1) * (DP / 64); ++j2) {
         uint32_t y[32];
         if (n > 0) {
           tmem_ld_32x32b_x32(acc + j2 * 32, y);

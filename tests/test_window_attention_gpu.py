@@ -64,6 +64,17 @@ def test_large_scores(d):
     check(q, k, v, do, 400, 3)
 
 
+@pytest.mark.parametrize("d", [64, 128])
+def test_unseen_keys_with_far_larger_scores(d):
+    """Keys that a row does not see, in the tiles that it reads, score hundreds more than those that it sees."""
+    q, k, v, do = make(1, 400, 2, 1, d)
+    with torch.no_grad():
+        q[..., 0] = 4.0
+        k[..., 0] = 0.0
+        k[:, 60::97, :, 0] = 512.0
+    check(q, k, v, do, 40, 1)
+
+
 def test_equal_and_zero_inputs():
     q, k, v, do = make(1, 300, 2, 2, 64)
     with torch.no_grad():
