@@ -114,6 +114,70 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// Pairs of floats: one instruction works on both.
+using f2 = unsigned long long;
+__device__ __forceinline__ f2 make_f2(float lo, float hi) {
+  f2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float lo_of(f2 x) {
+  float lo, hi;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(x));
+  return lo;
+}
+__device__ __forceinline__ float hi_of(f2 x) {
+  float lo, hi;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(x));
+  return hi;
+}
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
+  f2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f2 add2(f2 a, f2 b) {
+  f2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
+  f2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// 2^x of a pair on the FMA pipes: x = n + f with n the nearest whole number (by
+// adding 1.5 * 2^23, whose low bits then hold n) and f in [-1/2, 1/2]; 2^f by a
+// polynomial of degree 4 (minimax in relative error, found by reweighted least
+// squares with the constant term held at 1: off by 2^-18.4 at most); n goes into
+// the exponent as a whole number. x is at most 127; from -127 down the result is
+// exactly 0 (f = 0 there, and the exponent field becomes 0).
+__device__ __forceinline__ f2 ex2_poly(f2 x) {
+  x = make_f2(fmaxf(lo_of(x), -127.f), fmaxf(hi_of(x), -127.f));
+  const f2 t = add2(x, make_f2(12582912.f, 12582912.f));
+  const f2 n = add2(t, make_f2(-12582912.f, -12582912.f));
+  const f2 f = fma2(n, make_f2(-1.f, -1.f), x);
+  f2 p = fma2(f, make_f2(0.009582853f, 0.009582853f), make_f2(0.055906426f, 0.055906426f));
+  p = fma2(p, f, make_f2(0.24024099f, 0.24024099f));
+  p = fma2(p, f, make_f2(0.69312418f, 0.69312418f));
+  p = fma2(p, f, make_f2(1.f, 1.f));
+  return make_f2(__uint_as_float(__float_as_uint(lo_of(p)) + (__float_as_uint(lo_of(t)) << 23)),
+                 __uint_as_float(__float_as_uint(hi_of(p)) + (__float_as_uint(hi_of(t)) << 23)));
+}
+// 2^x of pair `i` of a row: one pair in kPolyEvery by the polynomial, the others by the
+// special-function unit, whose four results a cycle and quarter of an SM bound these
+// kernels otherwise.
+constexpr int kPolyEvery = 4;
+__device__ __forceinline__ f2 ex2_pair(int i, f2 x) {
+  return i % kPolyEvery == kPolyEvery - 1 ? ex2_poly(x) : make_f2(ex2(lo_of(x)), ex2(hi_of(x)));
+}
+
 // two floats as a packed pair of the element type, `lo` in the low half
 __device__ __forceinline__ uint32_t pack2(float lo, float hi, __nv_bfloat16) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
@@ -122,6 +186,11 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi, __nv_bfloat16) {
 __device__ __forceinline__ uint32_t pack2(float lo, float hi, __half) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(f2 x, T tag) {
+  return pack2(lo_of(x), hi_of(x), tag);
 }
 
 }  // namespace bdion

@@ -134,8 +134,8 @@ KeySplit split_keys(const WinArgs& a) {
 
 }  // namespace
 
-// o [b, s, hq, d], and log2 of each row's sum of exponentials [b, hq, s
-// rounded up to 128] (+inf behind the last position) for the backward pass
+// o [b, s, hq, d], and minus the log2 of each row's sum of exponentials [b, hq,
+// s rounded up to 128] (-inf behind the last position) for the backward pass
 std::tuple<at::Tensor, at::Tensor> window_attention_fwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
                                                         int64_t window, int64_t sinks) {
   const WinArgs a = make_args(q, k, v, window, sinks);
@@ -181,7 +181,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> window_attention_bwd(const at::Te
   by_case(q.scalar_type(), a.d, [&](auto tag, auto dp) {
     using E = decltype(tag);
     constexpr int DP = decltype(dp)::value;
-    launch(window_dq_tc<E, DP>, (int64_t)a.b * a.hq * (a.s_pad / kTile), 576, DqCfg<E, DP>::kSmemBytes, st, q128, k64,
+    launch(window_dq_tc<E, DP>, (int64_t)a.b * a.hq * (a.s_pad / kTile), 320, DqCfg<E, DP>::kSmemBytes, st, q128, k64,
            v64, g128, (const E*)o.data_ptr(), (const E*)go.data_ptr(), go.stride(0), go.stride(1), go.stride(2),
            lse.data_ptr<float>(), delta.data_ptr<float>(), (E*)dq.data_ptr(), a);
     at::Tensor work;

@@ -90,7 +90,7 @@ struct FwdCfg {
 template <typename T, int DP>
 __global__ void __launch_bounds__(192, 2)
     window_fwd_tc(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
-                  const __grid_constant__ CUtensorMap tv, T* __restrict__ o, float* __restrict__ lse, const WinArgs a) {
+                  const __grid_constant__ CUtensorMap tv, T* __restrict__ o, float* __restrict__ neg_lse, const WinArgs a) {
   using Cfg = FwdCfg<T, DP>;
   constexpr int ST = Cfg::kStages;
   extern __shared__ uint8_t smem_raw[];
@@ -244,7 +244,8 @@ __global__ void __launch_bounds__(192, 2)
       load();
       float mt[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int e = 0; e < 64; ++e) mt[e % 4] = fmaxf(mt[e % 4], __uint_as_float(x[e]));
+      for (int e = 0; e < 64; e += 2)
+        mt[e / 2 % 4] = max3(mt[e / 2 % 4], __uint_as_float(x[e]), __uint_as_float(x[e + 1]));
       const float top = fmaxf(fmaxf(mt[0], mt[1]), fmaxf(mt[2], mt[3]));
       // move the reference where this step exceeds it by more than 8 powers of two
       float f = 1.f;
@@ -254,15 +255,17 @@ __global__ void __launch_bounds__(192, 2)
         l *= f;
       }
       const float mc = m == -INFINITY ? 0.f : m * c;
-      float sum[4] = {};
+      const f2 c2 = make_f2(c, c), neg_mc = make_f2(-mc, -mc);
+      f2 sum[2] = {};
 #pragma unroll
-      for (int e = 0; e < 64; e += 2) {
-        const float p0 = ex2(__uint_as_float(x[e]) * c - mc), p1 = ex2(__uint_as_float(x[e + 1]) * c - mc);
-        sum[e % 4] += p0;
-        sum[e % 4 + 1] += p1;
-        pk[e / 2] = pack2(p0, p1, T{});
+      for (int e = 0; e < 32; ++e) {
+        const f2 z = make_f2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1]));
+        const f2 p = ex2_pair(e, fma2(z, c2, neg_mc));
+        sum[e % 2] = add2(sum[e % 2], p);
+        pk[e] = pack2(p, T{});
       }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      sum[0] = add2(sum[0], sum[1]);
+      l += lo_of(sum[0]) + hi_of(sum[0]);
       if (t > 0 && __any_sync(0xffffffffu, f != 1.f)) {
         // O is free once the step before is done
         if (!warp_wait(&o_done[buf ^ 1], ((t - 1) >> 1) & 1, abort, limit)) { ok = false; break; }
@@ -290,7 +293,7 @@ __global__ void __launch_bounds__(192, 2)
     } else {
       tc_fence_after();
       const bool real = i < a.s;
-      lse[((int64_t)b * a.hq + h) * a.s_pad + i] = real ? m * c + log2f(l) : INFINITY;
+      neg_lse[((int64_t)b * a.hq + h) * a.s_pad + i] = real ? -(m * c + log2f(l)) : -INFINITY;
       const float inv = 1.f / l;
       T* orow = o + (((int64_t)b * a.s + i) * a.hq + h) * a.d;
 #pragma unroll
@@ -330,25 +333,26 @@ struct DqCfg {
   static constexpr int kPanels = DP / 64;
   static constexpr int kRowBytes = kPanels * kPanel;       // Q, dO
   static constexpr int kStepBytes = kPanels * kHalfPanel;  // K, V
-  static constexpr int kStages = 4;
-  static constexpr int kSmemBytes = 2 * kRowBytes + 2 * kStages * kStepBytes + 1024 + 256 + kTile * 4;
-  static constexpr int kTmemCols = 512;
-  static constexpr int kBufs = 3;    // columns: three buffers of (S, dP) with dS on S, dQ behind them
-  static constexpr int kDQ = 384;
+  static constexpr int kStages = DP == 64 ? 2 : 1;
+  static constexpr int kSmemBytes = 2 * kRowBytes + 2 * kStages * kStepBytes + 1024 + 128 + kTile * 4;
+  static constexpr int kTmemCols = 256;
+  // columns: S [0, 64), dP [64, 128), dS [128, 192) where there is room (else on S), dQ at the end
+  static constexpr bool kOverlay = DP == 128;
+  static constexpr int kDS = kOverlay ? 0 : 128;
+  static constexpr int kDQ = 256 - DP;
 };
 
-// One CTA per (128 queries, head, sequence), one to an SM: S and dP by the
-// tensor cores, dS = P o (dP - delta), dQ += dS K with dS read from TMEM. Two
-// groups of eight warps take the steps of 64 keys in turn, two threads to a row
-// with half of the keys each; with three buffers the scores of two more steps
-// are under way meanwhile. delta is taken here from O and dO and kept for the
+// One CTA per (128 queries, head, sequence), two to an SM: S and dP by the
+// tensor cores, dS = P o (dP - delta) by two threads per query row (half of the
+// step's keys each: one thread's chain of loads and exponentials was longer
+// than the products), dQ += dS K with dS read from TMEM. delta is taken here from O and dO and kept for the
 // dK / dV kernel (0 behind the last position).
 template <typename T, int DP>
-__global__ void __launch_bounds__(576, 1)
+__global__ void __launch_bounds__(320, 2)
     window_dq_tc(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                  const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap tg,
                  const T* __restrict__ o, const T* __restrict__ go, int64_t go_b, int64_t go_s, int64_t go_h,
-                 const float* __restrict__ lse, float* __restrict__ delta, T* __restrict__ dq, const WinArgs a) {
+                 const float* __restrict__ neg_lse, float* __restrict__ neg_delta, T* __restrict__ dq, const WinArgs a) {
   using Cfg = DqCfg<T, DP>;
   constexpr int ST = Cfg::kStages;
   extern __shared__ uint8_t smem_raw[];
@@ -358,11 +362,11 @@ __global__ void __launch_bounds__(576, 1)
   uint8_t* sK = sG + Cfg::kRowBytes;
   uint8_t* sV = sK + ST * Cfg::kStepBytes;
   uint64_t* bars = reinterpret_cast<uint64_t*>(sV + ST * Cfg::kStepBytes);
-  uint64_t *q_full = bars, *k_full = bars + 1, *k_empty = bars + 5, *s_full = bars + 9, *p_full = bars + 12,
-           *acc_done = bars + 15, *all_done = bars + 18, *drain = bars + 19;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 20);
-  volatile int* abort = reinterpret_cast<volatile int*>(bars + 21);
-  float* s_delta = reinterpret_cast<float*>(bars + 24);
+  uint64_t *q_full = bars, *k_full = bars + 1, *k_empty = bars + 3, *v_full = bars + 5, *v_empty = bars + 7,
+           *s_full = bars + 9, *p_full = bars + 10, *o_full = bars + 11, *drain = bars + 12;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 13);
+  volatile int* abort = reinterpret_cast<volatile int*>(bars + 14);
+  float* s_delta = reinterpret_cast<float*>(bars + 16);
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
   const int h = blockIdx.x % a.hq;
@@ -374,16 +378,15 @@ __global__ void __launch_bounds__(576, 1)
 
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
-    for (int i = 0; i < ST; ++i) {
+    for (int i = 0; i < 2; ++i) {
       mbar_init(&k_full[i], 1);
       mbar_init(&k_empty[i], 1);
+      mbar_init(&v_full[i], 1);
+      mbar_init(&v_empty[i], 1);
     }
-    for (int i = 0; i < Cfg::kBufs; ++i) {
-      mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 8);
-      mbar_init(&acc_done[i], 1);
-    }
-    mbar_init(all_done, 1);
+    mbar_init(s_full, 1);
+    mbar_init(p_full, 8);
+    mbar_init(o_full, 1);
     mbar_init(drain, 1);
     *abort = 0;
     fence_mbar_init();
@@ -410,88 +413,96 @@ __global__ void __launch_bounds__(576, 1)
       for (; t < tiles.n; ++t) {
         const int st = t % ST, k0 = tiles.k0(t);
         const uint32_t ph = (t / ST) & 1;
+        // V is free once dP is done, K only after dQ
+        if (!mbar_wait_bounded(&v_empty[st], ph ^ 1, abort, limit)) { ok = false; break; }
+        mbar_arrive_expect_tx(&v_full[st], Cfg::kStepBytes);
+        for (int p = 0; p < Cfg::kPanels; ++p)
+          tma_load_4d(&tv, &v_full[st], sV + st * Cfg::kStepBytes + p * kHalfPanel, p * 64, k0, hk, b);
         if (!mbar_wait_bounded(&k_empty[st], ph ^ 1, abort, limit)) { ok = false; break; }
-        mbar_arrive_expect_tx(&k_full[st], 2 * Cfg::kStepBytes);
-        for (int p = 0; p < Cfg::kPanels; ++p) {
+        mbar_arrive_expect_tx(&k_full[st], Cfg::kStepBytes);
+        for (int p = 0; p < Cfg::kPanels; ++p)
           tma_load_4d(&tk, &k_full[st], sK + st * Cfg::kStepBytes + p * kHalfPanel, p * 64, k0, hk, b);
-          tma_load_4d(&tv, &k_full[st], sV + st * Cfg::kStepBytes + p * kHalfPanel, p * 64, k0, hk, b);
-        }
       }
       if (!ok) {
         report_status(a.status, kStatusWindowProducerTimeout);
         const uint64_t t0 = globaltimer_ns();
         while (!mbar_try_wait(q_full, 0) && globaltimer_ns() - t0 < 100000000ull) {
         }
-        for (int i = max(0, t - ST); i < t; ++i)
+        for (int i = max(0, t - ST); i <= t; ++i) {
           while (!mbar_try_wait(&k_full[i % ST], (i / ST) & 1) && globaltimer_ns() - t0 < 100000000ull) {
           }
+          while (!mbar_try_wait(&v_full[i % ST], (i / ST) & 1) && globaltimer_ns() - t0 < 100000000ull) {
+          }
+        }
       }
     }
   } else if (warp == 1) {
-    const bool leader = elect_one();
-    constexpr uint32_t kS = make_idesc(kTile, kHalfTile, false, false, AttnType<T>::kFmt);
-    constexpr uint32_t kD = make_idesc(kTile, DP, false, true, AttnType<T>::kFmt);
-    const uint32_t q_base = smem_u32(sQ), g_base = smem_u32(sG);
-    bool ok = warp_wait(q_full, 0, abort, limit);
-    auto scores = [&](int t) {
-      const int st = t % ST, buf = t % Cfg::kBufs;
-      if (!warp_wait(&k_full[st], (t / ST) & 1, abort, limit)) return false;
-      // the buffer's dS of three steps ago has been read
-      if (t >= Cfg::kBufs && !warp_wait(&acc_done[buf], (t / Cfg::kBufs - 1) & 1, abort, limit)) return false;
-      tc_fence_after();
-      const uint32_t k_base = smem_u32(sK + st * Cfg::kStepBytes), v_base = smem_u32(sV + st * Cfg::kStepBytes);
-      const uint32_t d = tmem + buf * 128;
+    {
+      const bool leader = elect_one();
+      constexpr uint32_t kS = make_idesc(kTile, kHalfTile, false, false, AttnType<T>::kFmt);
+      constexpr uint32_t kD = make_idesc(kTile, DP, false, true, AttnType<T>::kFmt);
+      const uint32_t q_base = smem_u32(sQ), g_base = smem_u32(sG);
+      bool ok = warp_wait(q_full, 0, abort, limit);
+      auto scores = [&](int t) {
+        const int st = t % ST;
+        const uint32_t ph = (t / ST) & 1;
+        if (!warp_wait(&v_full[st], ph, abort, limit) || !warp_wait(&k_full[st], ph, abort, limit))
+          return false;
+        tc_fence_after();
+        const uint32_t k_base = smem_u32(sK + st * Cfg::kStepBytes), v_base = smem_u32(sV + st * Cfg::kStepBytes);
 #pragma unroll
-      for (int k = 0; k < DP / 16; ++k) {
-        const uint32_t qo = (k / 4) * kPanel + (k % 4) * 32, ko = (k / 4) * kHalfPanel + (k % 4) * 32;
-        umma_ss(leader, d, sdesc_low(q_base + qo, 16), sdesc_low(k_base + ko, 16), kS, k != 0);
+        for (int k = 0; k < DP / 16; ++k) {
+          const uint32_t qo = (k / 4) * kPanel + (k % 4) * 32, ko = (k / 4) * kHalfPanel + (k % 4) * 32;
+          umma_ss(leader, tmem, sdesc_low(q_base + qo, 16), sdesc_low(k_base + ko, 16), kS, k != 0);
+        }
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k) {
+          const uint32_t qo = (k / 4) * kPanel + (k % 4) * 32, ko = (k / 4) * kHalfPanel + (k % 4) * 32;
+          umma_ss(leader, tmem + 64, sdesc_low(g_base + qo, 16), sdesc_low(v_base + ko, 16), kS, k != 0);
+        }
+        umma_commit_by(leader, &v_empty[st]);
+        umma_commit_by(leader, s_full);
+        return true;
+      };
+      if (ok) ok = scores(0);
+      for (int t = 0; t < tiles.n && ok; ++t) {
+        const int st = t % ST;
+        ok = warp_wait(p_full, t & 1, abort, limit);
+        if (!ok) break;
+        tc_fence_after();
+        if (!Cfg::kOverlay && t + 1 < tiles.n && !scores(t + 1)) { ok = false; break; }
+        const uint32_t k_base = smem_u32(sK + st * Cfg::kStepBytes);
+#pragma unroll
+        for (int k = 0; k < kHalfTile / 16; ++k)
+          umma_ts(leader, tmem + Cfg::kDQ, tmem + Cfg::kDS + half_col(k), sdesc_low(k_base + k * 2048, kHalfPanel), kD,
+                      (t | k) != 0);
+        umma_commit_by(leader, &k_empty[st]);
+        umma_commit_by(leader, o_full);
+        if (Cfg::kOverlay && t + 1 < tiles.n) ok = warp_wait(o_full, t & 1, abort, limit) && scores(t + 1);
       }
-#pragma unroll
-      for (int k = 0; k < DP / 16; ++k) {
-        const uint32_t qo = (k / 4) * kPanel + (k % 4) * 32, ko = (k / 4) * kHalfPanel + (k % 4) * 32;
-        umma_ss(leader, d + 64, sdesc_low(g_base + qo, 16), sdesc_low(v_base + ko, 16), kS, k != 0);
-      }
-      umma_commit_by(leader, &s_full[buf]);
-      return true;
-    };
-    for (int t = 0; t < min(tiles.n, Cfg::kBufs - 1) && ok; ++t) ok = scores(t);
-    for (int t = 0; t < tiles.n && ok; ++t) {
-      const int st = t % ST, buf = t % Cfg::kBufs;
-      if (!warp_wait(&p_full[buf], (t / Cfg::kBufs) & 1, abort, limit)) { ok = false; break; }
-      tc_fence_after();
-      const uint32_t k_base = smem_u32(sK + st * Cfg::kStepBytes);
-#pragma unroll
-      for (int k = 0; k < kHalfTile / 16; ++k)
-        umma_ts(leader, tmem + Cfg::kDQ, tmem + buf * 128 + half_col(k), sdesc_low(k_base + k * 2048, kHalfPanel), kD,
-                (t | k) != 0);
-      umma_commit_by(leader, &k_empty[st]);
-      umma_commit_by(leader, &acc_done[buf]);
-      if (t + Cfg::kBufs - 1 < tiles.n) ok = scores(t + Cfg::kBufs - 1);
-    }
-    if (ok) {
-      umma_commit_by(leader, all_done);
-    } else {
-      if (lane == 0) report_status(a.status, kStatusWindowMmaTimeout);
-      umma_commit_by(leader, drain);
-      const uint64_t t0 = globaltimer_ns();
-      while (!mbar_try_wait(drain, 0) && globaltimer_ns() - t0 < 100000000ull) {
+      if (!ok) {
+        if (lane == 0) report_status(a.status, kStatusWindowMmaTimeout);
+        umma_commit_by(leader, drain);
+        const uint64_t t0 = globaltimer_ns();
+        while (!mbar_try_wait(drain, 0) && globaltimer_ns() - t0 < 100000000ull) {
+        }
       }
     }
   } else {
-    const int quarter = warp & 3, which = (warp - 2) / 8, half = (warp - 2) / 4 % 2;
+    const int quarter = warp & 3, half = (warp - 2) / 4;
     const int r = quarter * 32 + lane, i = q0 + r;
     const uint32_t row = tmem + ((uint32_t)(quarter * 32) << 16);
     const float c = a.scale_log2;
     const int64_t at = ((int64_t)b * a.hq + h) * a.s_pad + q0;
-    const float L = lse[at + r];
+    const f2 c2 = make_f2(c, c), neg_l = make_f2(neg_lse[at + r], neg_lse[at + r]);
     {
-      // delta of 8 rows per warp, DP / 8 lanes to a row
+      // delta of 16 rows per warp, DP / 8 lanes to a row
       constexpr int kLanes = DP / 8, kRows = 32 / kLanes;
       const int col = lane % kLanes * 8;
-      float v[8 / kRows];
+      float v[16 / kRows];
 #pragma unroll
-      for (int n = 0; n < 8 / kRows; ++n) {
-        const int rr = q0 + (warp - 2) * 8 + n * kRows + lane / kLanes;
+      for (int n = 0; n < 16 / kRows; ++n) {
+        const int rr = q0 + (warp - 2) * 16 + n * kRows + lane / kLanes;
         v[n] = 0.f;
         if (rr < a.s && col < a.d) {
           const uint4 ou = *reinterpret_cast<const uint4*>(o + (((int64_t)b * a.s + rr) * a.hq + h) * a.d + col);
@@ -502,27 +513,26 @@ __global__ void __launch_bounds__(576, 1)
         }
       }
 #pragma unroll
-      for (int n = 0; n < 8 / kRows; ++n) {
+      for (int n = 0; n < 16 / kRows; ++n) {
 #pragma unroll
         for (int m = kLanes / 2; m > 0; m >>= 1) v[n] += __shfl_xor_sync(0xffffffffu, v[n], m);
-        const int rr = (warp - 2) * 8 + n * kRows + lane / kLanes;
+        const int rr = (warp - 2) * 16 + n * kRows + lane / kLanes;
         if (col == 0) {
-          s_delta[rr] = v[n];
-          delta[at + rr] = v[n];
+          s_delta[rr] = -v[n];
+          neg_delta[at + rr] = -v[n];
         }
       }
-      asm volatile("bar.sync 1, 512;" ::: "memory");
+      asm volatile("bar.sync 1, 256;" ::: "memory");
     }
-    const float dl = s_delta[r];
+    const f2 neg_d = make_f2(s_delta[r], s_delta[r]);
     bool ok = true;
-    for (int t = which; t < tiles.n; t += 2) {
-      const int k0 = tiles.k0(t), buf = t % Cfg::kBufs;
-      const uint32_t at_buf = row + buf * 128 + half * 32;
-      if (!warp_wait(&s_full[buf], (t / Cfg::kBufs) & 1, abort, limit)) { ok = false; break; }
+    for (int t = 0; t < tiles.n; ++t) {
+      const int k0 = tiles.k0(t);
+      if (!warp_wait(s_full, t & 1, abort, limit)) { ok = false; break; }
       tc_fence_after();
       uint32_t x[32], y[32];
-      tmem_ld_32x32b_x32(at_buf, x);
-      tmem_ld_32x32b_x32(at_buf + 64, y);
+      tmem_ld_32x32b_x32(row + half * 32, x);
+      tmem_ld_32x32b_x32(row + 64 + half * 32, y);
       tmem_wait_ld();
       if (!tiles.whole(a, q0, k0)) {
         const uint32_t seen = seen_mask(a, i, k0 + half * 32);
@@ -531,23 +541,29 @@ __global__ void __launch_bounds__(576, 1)
           if (!((seen >> e) & 1u)) x[e] = 0xff800000u;
       }
 #pragma unroll
-      for (int e = 0; e < 32; e += 2) {
-        const float p0 = ex2(__uint_as_float(x[e]) * c - L), p1 = ex2(__uint_as_float(x[e + 1]) * c - L);
-        x[e / 2] = pack2(p0 * (__uint_as_float(y[e]) - dl), p1 * (__uint_as_float(y[e + 1]) - dl), T{});
+      for (int e = 0; e < 16; ++e) {
+        const f2 z = make_f2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1]));
+        const f2 g = make_f2(__uint_as_float(y[2 * e]), __uint_as_float(y[2 * e + 1]));
+        x[e] = pack2(mul2(ex2_pair(e, fma2(z, c2, neg_l)), add2(g, neg_d)), T{});
       }
-      tmem_st_32x32b_x16(at_buf, x);
+      if (!Cfg::kOverlay && t > 0) {  // dS's place is free once the step before is done
+        if (!warp_wait(o_full, (t - 1) & 1, abort, limit)) { ok = false; break; }
+        tc_fence_after();
+      }
+      tmem_st_32x32b_x16(row + Cfg::kDS + half * 32, x);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[buf]);
+      if (lane == 0) mbar_arrive(p_full);
     }
-    if (ok) ok = warp_wait(all_done, 0, abort, limit);
+    if (ok) ok = warp_wait(o_full, (tiles.n - 1) & 1, abort, limit);
     if (!ok) {
       if (lane == 0) report_status(a.status, kStatusWindowSoftmaxTimeout);
     } else {
       tc_fence_after();
       T* out = dq + (((int64_t)b * a.s + i) * a.hq + h) * a.d;
-      for (int j = which * 2 + half; j < DP / 32; j += 4) {  // a quarter of the row's columns
+#pragma unroll
+      for (int j = half * (DP / 64); j < (half + 1) * (DP / 64); ++j) {
         uint32_t y[32];
         tmem_ld_32x32b_x32(row + Cfg::kDQ + j * 32, y);
         tmem_wait_ld();
@@ -620,7 +636,7 @@ template <typename T, int DP>
 __global__ void __launch_bounds__(576, 1)
     window_dkv_tc(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                   const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap tg,
-                  const float* __restrict__ lse, const float* __restrict__ delta, T* __restrict__ dk,
+                  const float* __restrict__ neg_lse, const float* __restrict__ neg_delta, T* __restrict__ dk,
                   T* __restrict__ dv, float* __restrict__ work, const KeySplit split, const WinArgs a) {
   using Cfg = DkvCfg<T, DP>;
   constexpr int ST = Cfg::kStages;
@@ -699,8 +715,8 @@ __global__ void __launch_bounds__(576, 1)
           tma_load_4d(&tg, &q_full[st], sG + st * Cfg::kStepBytes + p * kHalfPanel, p * 64, q0, h, b);
         }
         const int64_t at = ((int64_t)b * a.hq + h) * a.s_pad + q0;
-        bulk_load(sL + st * kHalfTile, lse + at, Cfg::kStatBytes, &q_full[st]);
-        bulk_load(sD + st * kHalfTile, delta + at, Cfg::kStatBytes, &q_full[st]);
+        bulk_load(sL + st * kHalfTile, neg_lse + at, Cfg::kStatBytes, &q_full[st]);
+        bulk_load(sD + st * kHalfTile, neg_delta + at, Cfg::kStatBytes, &q_full[st]);
       }
       if (!ok) {
         report_status(a.status, kStatusWindowProducerTimeout);
@@ -797,15 +813,14 @@ __global__ void __launch_bounds__(576, 1)
           if (e < e0 || e >= e1) x[e] = 0xff800000u;
       }
       const float *pl = sL + st * kHalfTile + half * 32, *pd = sD + st * kHalfTile + half * 32;
+      const f2 c2 = make_f2(c, c);
 #pragma unroll
-      for (int e = 0; e < 32; e += 4) {
-        const float4 L = *reinterpret_cast<const float4*>(pl + e), D = *reinterpret_cast<const float4*>(pd + e);
-        const float p0 = ex2(__uint_as_float(x[e]) * c - L.x), p1 = ex2(__uint_as_float(x[e + 1]) * c - L.y);
-        const float p2 = ex2(__uint_as_float(x[e + 2]) * c - L.z), p3 = ex2(__uint_as_float(x[e + 3]) * c - L.w);
-        x[e / 2] = pack2(p0, p1, T{});
-        x[e / 2 + 1] = pack2(p2, p3, T{});
-        y[e / 2] = pack2(p0 * (__uint_as_float(y[e]) - D.x), p1 * (__uint_as_float(y[e + 1]) - D.y), T{});
-        y[e / 2 + 1] = pack2(p2 * (__uint_as_float(y[e + 2]) - D.z), p3 * (__uint_as_float(y[e + 3]) - D.w), T{});
+      for (int e = 0; e < 16; ++e) {
+        const f2 z = make_f2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1]));
+        const f2 g = make_f2(__uint_as_float(y[2 * e]), __uint_as_float(y[2 * e + 1]));
+        const f2 p = ex2_pair(e, fma2(z, c2, *reinterpret_cast<const f2*>(pl + 2 * e)));
+        x[e] = pack2(p, T{});
+        y[e] = pack2(mul2(p, add2(g, *reinterpret_cast<const f2*>(pd + 2 * e))), T{});
       }
       tmem_st_32x32b_x16(buf + half * 32, x);
       tmem_st_32x32b_x16(buf + 64 + half * 32, y);
