@@ -13,25 +13,20 @@
 #include <mutex>
 #include <tuple>
 
-#include "common.cuh"
 #include "host_utils.h"
+#include "ptx_attn.cuh"
 
 namespace bdion {
 
 namespace {
 
 constexpr int kThreads = 512;
+constexpr int kRowThreads = 256;  // of the kernel that holds rows in registers
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxTop = 1024;     // entries kept per row
 constexpr int kMaxCand = 2048;    // candidates collected per row before ranking
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 
 __device__ __forceinline__ float as_f(__nv_bfloat16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ float as_f(__half v) { return __half2float(v); }
@@ -183,6 +178,12 @@ struct Raw8 {
     }
   }
   __device__ __forceinline__ void get(float* v) const { load8(reinterpret_cast<const T*>(u), v); }
+  __device__ __forceinline__ void get(f2 (&v)[4]) const {
+    float x[8];
+    get(x);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = make_f2(x[2 * i], x[2 * i + 1]);
+  }
 };
 
 
@@ -292,19 +293,18 @@ __global__ void __launch_bounds__(kThreads) top_logits_kernel(const T* __restric
         r[i].get(v);
         const float vm = r[i].max();
         sum.raise(vm, c);
-        float s0 = 0.f, s1 = 0.f;
+        const f2 neg_m = make_f2(-sum.m, -sum.m), c2 = make_f2(c, c);
+        f2 s2 = make_f2(0.f, 0.f);
 #pragma unroll
         for (int e = 0; e < 8; e += 2) {
-          s0 += ex2((v[e] - sum.m) * c);
-          s1 += ex2((v[e + 1] - sum.m) * c);
+          const f2 z = mul2(add2(make_f2(v[e], v[e + 1]), neg_m), c2);
+          s2 = add2(s2, make_f2(ex2(lo_of(z)), ex2(hi_of(z))));
         }
-        sum.s += s0 + s1;
+        sum.s += lo_of(s2) + hi_of(s2);
         if (vm >= thr_f) {
-#pragma unroll 1
-          for (int e = 0; e < 8; ++e) {
-            const float z = as_f(x[lead + g * 8 + e]);
-            if (z >= thr_f) collect_one(z, lead + g * 8 + e);
-          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (v[e] >= thr_f) collect_one(v[e], lead + g * 8 + e);
         }
       }
     }
@@ -600,8 +600,10 @@ __global__ void __launch_bounds__(kThreads) distill_kernel(const T* __restrict__
 constexpr int kEnds = 16;          // elements before the first and after the last 8-element group
 constexpr int kMaxCluster = 8;
 
-// Sums (or maxima) of N values over the block in two barriers; `buf` holds
-// N * (kWarps + 1) floats, which the next call may use at once.
+// Sums (or maxima) of N <= kRowWarps values over a block of kRowThreads in two
+// barriers; `buf` holds N * (kRowWarps + 1) floats, which the next call may use
+// at once.
+constexpr int kRowWarps = kRowThreads / 32;
 template <int N, bool MAX>
 __device__ __forceinline__ void block_all(float (&v)[N], float* buf) {
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -609,11 +611,11 @@ __device__ __forceinline__ void block_all(float (&v)[N], float* buf) {
   for (int i = 0; i < N; ++i) v[i] = MAX ? warp_max(v[i]) : warp_sum(v[i]);
   if (lane == 0) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) buf[N + i * kWarps + warp] = v[i];
+    for (int i = 0; i < N; ++i) buf[N + i * kRowWarps + warp] = v[i];
   }
   __syncthreads();
   if (warp < N) {
-    float x = lane < kWarps ? buf[N + warp * kWarps + lane] : (MAX ? -FLT_MAX : 0.f);
+    float x = lane < kRowWarps ? buf[N + warp * kRowWarps + lane] : (MAX ? -FLT_MAX : 0.f);
     x = MAX ? warp_max(x) : warp_sum(x);
     if (lane == 0) buf[warp] = x;
   }
@@ -639,13 +641,13 @@ enum HardMode { kHardNone, kHardSquare, kHardOther };
 // longer than memory. Temperatures 3 and 4 take powers likewise (kHardOther
 // with `power`), others an exponential of their own.
 template <typename T, typename TG, int NV, int MODE>
-__global__ void __launch_bounds__(kThreads, 2)
+__global__ void __launch_bounds__(kRowThreads, 2)
     distill_row_kernel(const T* __restrict__ logits, TG* __restrict__ grad, const DistillArgs a, int C, int power) {
   namespace cg = cooperative_groups;
   constexpr bool both = MODE != kHardNone;
-  __shared__ uint32_t s_marks[kThreads * NV / 4];  // one byte per group: which of its columns are in the set
+  __shared__ uint32_t s_marks[kRowThreads * NV / 4];  // one byte per group: which of its columns are in the set
   __shared__ uint32_t s_end_marks;
-  __shared__ float red_max[2 * (kWarps + 1)], red_sum[6 * (kWarps + 1)];
+  __shared__ float red_max[2 * (kRowWarps + 1)], red_sum[6 * (kRowWarps + 1)];
   __shared__ float s_p[kMaxTop], s_z[kMaxTop];
   __shared__ int s_i[kMaxTop];
   __shared__ int s_marked, s_twice;
@@ -692,7 +694,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     return i >= 0 && i < V ? (int)i : -1;
   };
   auto clear_marks = [&] {
-    for (int i = tid; i < kThreads * NV / 4; i += kThreads) s_marks[i] = 0;
+    for (int i = tid; i < kRowThreads * NV / 4; i += kRowThreads) s_marks[i] = 0;
     if (tid == 0) s_marked = s_twice = 0, s_end_marks = 0;
   };
 
@@ -707,7 +709,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     const T* xg = logits + row * a.ld_in + p.lead + (int64_t)p.g0 * 8;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
-      if (i * kThreads + tid < p.n) raw[i].load(xg + (i * kThreads + tid) * 8);
+      if (i * kRowThreads + tid < p.n) raw[i].load(xg + (i * kRowThreads + tid) * 8);
   }
   int ahead_i = -1;       // this thread's first entry of the next row
   float ahead_t = 0.f;
@@ -728,7 +730,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   const T* next_x = logits + (row + stride) * a.ld_in + next.lead + (int64_t)next.g0 * 8;
   // the next row's group i into the place of this row's
   auto load_next = [&](int i) {
-    if (next_label >= 0 && i * kThreads + tid < next.n) raw[i].load(next_x + (i * kThreads + tid) * 8);
+    if (next_label >= 0 && i * kRowThreads + tid < next.n) raw[i].load(next_x + (i * kRowThreads + tid) * 8);
   };
   const int now_i = ahead_i;
   const float now_t = ahead_t;
@@ -740,7 +742,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     const float zero[8] = {};
     if (tid == 0 && rank == 0) a.row_loss[row] = 0.f;
     if (grad != nullptr) {
-      for (int g = tid; g < n_mine; g += kThreads) store8(gx + lead + (g0 + g) * 8, zero);
+      for (int g = tid; g < n_mine; g += kRowThreads) store8(gx + lead + (g0 + g) * 8, zero);
       if (rank == 0 && tid < lead) put(gx + tid, 0.f);
       if (rank == 0 && tail0 + tid < V) put(gx + tail0 + tid, 0.f);
     }
@@ -758,7 +760,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 
   float mx[2] = {-FLT_MAX, -FLT_MAX};  // outside the set, in it
   float tmax = -FLT_MAX;
-  for (int j = tid; j < a.k; j += kThreads) {
+  for (int j = tid; j < a.k; j += kRowThreads) {
     const int i = j == tid ? now_i : index_of(row, j);
     const float t = (j == tid ? now_t : a.top_values[row * a.k + j]) * a.inv_tau;
     int mine = -1;  // this block's column, or -1
@@ -784,31 +786,29 @@ __global__ void __launch_bounds__(kThreads, 2)
   if (a.top_lse != nullptr) {
     tlse = a.top_lse[row];
   } else {
-    tmax = block_max(tmax, red_max);
-    float s = 0.f;
-    for (int j = tid; j < a.k; j += kThreads) s += s_p[j] == -INFINITY ? 0.f : ex2((s_p[j] - tmax) * kLog2e);
-    s = block_sum(s, red_max);
-    tlse = tmax + logf(s);
+    float tm[1] = {tmax}, ts[1] = {};
+    block_all<1, true>(tm, red_max);
+    for (int j = tid; j < a.k; j += kRowThreads) ts[0] += s_p[j] == -INFINITY ? 0.f : ex2((s_p[j] - tm[0]) * kLog2e);
+    block_all<1, false>(ts, red_sum);
+    tlse = tm[0] + logf(ts[0]);
   }
   __syncthreads();
 
   // maximum outside the set, then the sums under it; columns in the set count as -inf
-  auto get = [&](int i, float* v) {
-    raw[i].get(v);
-    const uint32_t marks = reinterpret_cast<const uint8_t*>(s_marks)[i * kThreads + tid];
-    if (marks) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if ((marks >> e) & 1u) v[e] = -INFINITY;
-    }
-  };
+  auto marks_of = [&](int i) -> uint32_t { return reinterpret_cast<const uint8_t*>(s_marks)[i * kRowThreads + tid]; };
+  auto strike = [](float v, uint32_t marks, int e) { return (marks >> e) & 1u ? -INFINITY : v; };
 #pragma unroll
   for (int i = 0; i < NV; ++i)
-    if (i * kThreads + tid < n_mine) {
-      float v[8];
-      get(i, v);
+    if (i * kRowThreads + tid < n_mine) {
+      const uint32_t marks = marks_of(i);
+      if (marks == 0) {
+        mx[0] = fmaxf(mx[0], raw[i].max());
+      } else {
+        float v[8];
+        raw[i].get(v);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) mx[0] = fmaxf(mx[0], v[e]);
+        for (int e = 0; e < 8; ++e) mx[0] = fmaxf(mx[0], strike(v[e], marks, e));
+      }
     }
   const bool end_rest = end_col >= 0 && !((s_end_marks >> tid) & 1u);
   if (end_rest) mx[0] = fmaxf(mx[0], end_z);
@@ -820,18 +820,33 @@ __global__ void __launch_bounds__(kThreads, 2)
     return power == 3 ? y * y * y : power == 4 ? (y * y) * (y * y) : ex2((z - ref) * kLog2e);
   };
   float sum[6] = {};  // rest; rest at temperature 1; set; set at temperature 1; teacher's mass; sum p (log p - z / tau)
+  {
+    const f2 neg_m = make_f2(-m, -m), c2 = make_f2(c, c);
+    f2 rest2 = make_f2(0.f, 0.f), full2 = rest2;
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
-    if (i * kThreads + tid < n_mine) {
-      float v[8];
-      get(i, v);
+    for (int i = 0; i < NV; ++i)
+      if (i * kRowThreads + tid < n_mine) {
+        f2 v[4];
+        raw[i].get(v);
+        const uint32_t marks = marks_of(i);
+        if (marks) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float y = ex2((v[e] - m) * c);
-        sum[0] += y;
-        if (both) sum[1] += full_of(y, v[e], m);
+          for (int e = 0; e < 4; ++e)
+            v[e] = make_f2(strike(lo_of(v[e]), marks, 2 * e), strike(hi_of(v[e]), marks, 2 * e + 1));
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const f2 z = mul2(add2(v[e], neg_m), c2);
+          const f2 y = make_f2(ex2(lo_of(z)), ex2(hi_of(z)));
+          rest2 = add2(rest2, y);
+          if (MODE == kHardSquare) full2 = fma2(y, y, full2);
+          if (MODE == kHardOther)
+            full2 = add2(full2, make_f2(full_of(lo_of(y), lo_of(v[e]), m), full_of(hi_of(y), hi_of(v[e]), m)));
+        }
       }
-    }
+    sum[0] = lo_of(rest2) + hi_of(rest2);
+    sum[1] = lo_of(full2) + hi_of(full2);
+  }
   if (end_rest) {
     const float y = ex2((end_z - m) * c);
     sum[0] += y;
@@ -844,7 +859,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         if (s_i[i] == s_i[j]) return false;
     return true;
   };
-  for (int j = tid; j < a.k; j += kThreads) {
+  for (int j = tid; j < a.k; j += kRowThreads) {
     const float logp = s_p[j] - tlse, p = s_p[j] == -INFINITY ? 0.f : ex2(logp * kLog2e);
     sum[4] += p;
     if (s_i[j] >= 0) {
@@ -920,23 +935,30 @@ __global__ void __launch_bounds__(kThreads, 2)
     f_rest = w_soft * (to_top * inv_B - p_rest / rest_s) + (both ? 0.f : w_hard * to_top * inv_B);
     f_full = both ? w_hard * ex2((rm - top) * kLog2e) * inv_F : 0.f;
   }
+  {
+    const f2 neg_m = make_f2(-rm, -rm), c2 = make_f2(c, c);
+    const f2 fr2 = make_f2(f_rest, f_rest), ff2 = make_f2(f_full, f_full);
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    float v[8];
-    raw[i].get(v);
-    load_next(i);
-    if (i * kThreads + tid < n_mine) {
+    for (int i = 0; i < NV; ++i) {
+      f2 v[4];
+      raw[i].get(v);
+      load_next(i);
+      if (i * kRowThreads + tid < n_mine) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float y = ex2((v[e] - rm) * c);
-        if (MODE == kHardNone)
-          v[e] = f_rest * y;
-        else if (MODE == kHardSquare)
-          v[e] = y * (f_rest + f_full * y);
-        else
-          v[e] = f_rest * y + f_full * full_of(y, v[e], rm);
+        for (int e = 0; e < 4; ++e) {
+          const f2 z = mul2(add2(v[e], neg_m), c2);
+          const f2 y = make_f2(ex2(lo_of(z)), ex2(hi_of(z)));
+          if (MODE == kHardNone)
+            v[e] = mul2(fr2, y);
+          else if (MODE == kHardSquare)
+            v[e] = mul2(y, fma2(y, ff2, fr2));
+          else
+            v[e] = fma2(ff2, make_f2(full_of(lo_of(y), lo_of(v[e]), rm), full_of(hi_of(y), hi_of(v[e]), rm)), mul2(fr2, y));
+        }
+        const float g[8] = {lo_of(v[0]), hi_of(v[0]), lo_of(v[1]), hi_of(v[1]),
+                            lo_of(v[2]), hi_of(v[2]), lo_of(v[3]), hi_of(v[3])};
+        store8(gx + lead + (g0 + i * kRowThreads + tid) * 8, g);
       }
-      store8(gx + lead + (g0 + i * kThreads + tid) * 8, v);
     }
   }
   if (end_col >= 0) {
@@ -946,7 +968,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   __syncthreads();
   auto soft_at = [&](float z) { return ex2((z - top) * c) * inv_B; };
   auto hard_at = [&](float z) { return both ? ex2((z - top) * kLog2e) * inv_F : soft_at(z); };
-  for (int j = tid; j < a.k; j += kThreads) {
+  for (int j = tid; j < a.k; j += kRowThreads) {
     const int i = s_i[j];
     if (i < 0 || !first_of(j)) continue;
     float p = 0.f;
@@ -1107,17 +1129,17 @@ void distill_fwd_bwd(const at::Tensor& logits, const c10::optional<at::Tensor>& 
       if constexpr (std::is_same_v<E, G> || std::is_same_v<E, float>) {
         // Rows of up to kMaxCluster blocks' registers are read once; longer ones, and
         // those whose logits and gradient are not aligned alike, twice.
-        constexpr int kMost = sizeof(E) == 2 ? 8 : 4;  // 32 registers of logits per thread
+        constexpr int kMost = sizeof(E) == 2 ? 16 : 8;  // 64 registers of logits per thread
         const int64_t groups = V / 8;
-        if (a.vec && groups <= (int64_t)kMaxCluster * kThreads * kMost) {
+        if (a.vec && groups <= (int64_t)kMaxCluster * kRowThreads * kMost) {
           int C = 1;
-          while (groups > (int64_t)C * kThreads * kMost) C *= 2;
-          const int64_t per_thread = (groups + C * kThreads - 1) / (C * kThreads);
+          while (groups > (int64_t)C * kRowThreads * kMost) C *= 2;
+          const int64_t per_thread = (groups + C * kRowThreads - 1) / (C * kRowThreads);
           const int power = tau == 3 || tau == 4 ? (int)tau : 0;
           auto run = [&](auto nv, auto mode) {
             cudaLaunchConfig_t cfg = {};
             cfg.gridDim = dim3((unsigned)C);
-            cfg.blockDim = dim3(kThreads);
+            cfg.blockDim = dim3(kRowThreads);
             cfg.stream = s;
             cudaLaunchAttribute attr[1];
             attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -1141,7 +1163,7 @@ void distill_fwd_bwd(const at::Tensor& logits, const c10::optional<at::Tensor>& 
           };
           if (per_thread <= 1)
             by_mode(std::integral_constant<int, 1>{});
-          else if (per_thread <= 4 || kMost == 4)
+          else if (per_thread <= 4)
             by_mode(std::integral_constant<int, 4>{});
           else
             by_mode(std::integral_constant<int, kMost>{});

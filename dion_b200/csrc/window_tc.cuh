@@ -454,12 +454,8 @@ __global__ void __launch_bounds__(320, 2)
         for (int k = 0; k < DP / 16; ++k) {
           const uint32_t qo = (k / 4) * kPanel + (k % 4) * 32, ko = (k / 4) * kHalfPanel + (k % 4) * 32;
           umma_ss(leader, tmem, sdesc_low(q_base + qo, 16), sdesc_low(k_base + ko, 16), kS, k != 0);
-        }
-#pragma unroll
-        for (int k = 0; k < DP / 16; ++k) {
-          const uint32_t qo = (k / 4) * kPanel + (k % 4) * 32, ko = (k / 4) * kHalfPanel + (k % 4) * 32;
           umma_ss(leader, tmem + 64, sdesc_low(g_base + qo, 16), sdesc_low(v_base + ko, 16), kS, k != 0);
-        }
+      }
         umma_commit_by(leader, &v_empty[st]);
         umma_commit_by(leader, s_full);
         return true;
@@ -747,10 +743,6 @@ __global__ void __launch_bounds__(576, 1)
         for (int k = 0; k < DP / 16; ++k) {
           const uint32_t ko = (k / 4) * kPanel + (k % 4) * 32, qo = (k / 4) * kHalfPanel + (k % 4) * 32;
           umma_ss(leader, d, sdesc_low(k_base + ko, 16), sdesc_low(q_base + qo, 16), kS, k != 0);
-        }
-#pragma unroll
-        for (int k = 0; k < DP / 16; ++k) {
-          const uint32_t ko = (k / 4) * kPanel + (k % 4) * 32, qo = (k / 4) * kHalfPanel + (k % 4) * 32;
           umma_ss(leader, d + 64, sdesc_low(v_base + ko, 16), sdesc_low(g_base + qo, 16), kS, k != 0);
         }
         umma_commit_by(leader, &s_full[buf]);
@@ -768,12 +760,11 @@ __global__ void __launch_bounds__(576, 1)
         const uint32_t q_base = smem_u32(sQ + st * Cfg::kStepBytes), g_base = smem_u32(sG + st * Cfg::kStepBytes);
         const uint32_t d = tmem + buf * 128;
 #pragma unroll
-        for (int k = 0; k < kHalfTile / 16; ++k)
+        for (int k = 0; k < kHalfTile / 16; ++k) {
           umma_ts(leader, tmem + Cfg::kDV, d + half_col(k), sdesc_low(g_base + k * 2048, kHalfPanel), kD, (t | k) != 0);
-#pragma unroll
-        for (int k = 0; k < kHalfTile / 16; ++k)
           umma_ts(leader, tmem + Cfg::kDK, d + 64 + half_col(k), sdesc_low(q_base + k * 2048, kHalfPanel), kD,
                       (t | k) != 0);
+        }
         umma_commit_by(leader, &q_empty[st]);
         umma_commit_by(leader, &acc_done[buf]);
         if (Cfg::kBufs > 2 && t + kAhead < n) ok = scores(t + kAhead);
