@@ -114,17 +114,17 @@ void by_case(at::ScalarType t, int d, F f) {
 
 // Parts of the dK / dV kernel. A tile is cut where the whole tiles would not
 // give every SM two parts; a tile with first tokens where its steps would
-// outlast the others'. A part has 8 steps at least: fewer cost more in its
+// outlast the others'. A part has 4 steps at least: fewer cost more in its
 // start and its sums' way through memory than they bring.
 KeySplit split_keys(const WinArgs& a) {
   KeySplit p;
   const int64_t group = a.hq / a.hkv, sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
   p.n_tiles = a.s_pad / kTile;
   p.n_first = std::min(p.n_tiles, (a.sinks + kTile - 1) / kTile);
-  const int64_t heads = (int64_t)a.b * a.hkv, per_head = a.s_pad / kHalfTile;
-  const int64_t band = group * std::min<int64_t>(per_head, ((int64_t)kTile + a.window - 2) / kHalfTile + 1);
+  const int64_t heads = (int64_t)a.b * a.hkv, per_head = a.s_pad / kTile;
+  const int64_t band = group * std::min<int64_t>(per_head, ((int64_t)kTile + a.window - 2) / kTile + 1);
   const int64_t first = group * per_head;
-  auto cut = [](int64_t parts, int64_t steps) { return (int)std::max<int64_t>(1, std::min(parts, steps / 8)); };
+  auto cut = [](int64_t parts, int64_t steps) { return (int)std::max<int64_t>(1, std::min(parts, steps / 4)); };
   p.c_band = cut((2 * sms + heads * p.n_tiles - 1) / (heads * p.n_tiles), band);
   const int64_t total = heads * (p.n_first * first + (p.n_tiles - p.n_first) * band);
   const int64_t longest = std::max((band + p.c_band - 1) / p.c_band, total / (4 * sms));
@@ -174,21 +174,19 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> window_attention_bwd(const at::Te
   if (q.numel() == 0) return {dq, dk.zero_(), dv.zero_()};
   auto delta = at::empty_like(lse);
   const KeySplit split = split_keys(a);
-  const CUtensorMap q128 = head_map(q, kTile, "q"), k128 = head_map(k, kTile, "k"), v128 = head_map(v, kTile, "v"),
-                    g128 = head_map(go, kTile, "the output's gradient"), q64 = head_map(q, kHalfTile, "q"),
-                    k64 = head_map(k, kHalfTile, "k"), v64 = head_map(v, kHalfTile, "v"),
-                    g64 = head_map(go, kHalfTile, "the output's gradient");
+  const CUtensorMap mq = head_map(q, kTile, "q"), mk = head_map(k, kTile, "k"), mv = head_map(v, kTile, "v"),
+                    mg = head_map(go, kTile, "the output's gradient");
   by_case(q.scalar_type(), a.d, [&](auto tag, auto dp) {
     using E = decltype(tag);
     constexpr int DP = decltype(dp)::value;
-    launch(window_dq_tc<E, DP>, (int64_t)a.b * a.hq * (a.s_pad / kTile), 320, DqCfg<E, DP>::kSmemBytes, st, q128, k64,
-           v64, g128, (const E*)o.data_ptr(), (const E*)go.data_ptr(), go.stride(0), go.stride(1), go.stride(2),
+    launch(window_dq_tc<E, DP>, (int64_t)a.b * a.hq * (a.s_pad / kTile), 576, DqCfg<E, DP>::kSmemBytes, st, mq, mk, mv,
+           mg, (const E*)o.data_ptr(), (const E*)go.data_ptr(), go.stride(0), go.stride(1), go.stride(2),
            lse.data_ptr<float>(), delta.data_ptr<float>(), (E*)dq.data_ptr(), a);
     at::Tensor work;
     const int64_t slots = (int64_t)a.b * a.hkv * split.slots();
     if (slots > 0) work = at::empty({slots, 2, kTile, DP}, lse.options());
-    launch(window_dkv_tc<E, DP>, (int64_t)a.b * a.hkv * split.parts(), 576, DkvCfg<E, DP>::kSmemBytes, st, q64, k128,
-           v128, g64, lse.data_ptr<float>(), delta.data_ptr<float>(), (E*)dk.data_ptr(), (E*)dv.data_ptr(),
+    launch(window_dkv_tc<E, DP>, (int64_t)a.b * a.hkv * split.parts(), 576, DkvCfg<E, DP>::kSmemBytes, st, mq, mk, mv,
+           mg, lse.data_ptr<float>(), delta.data_ptr<float>(), (E*)dk.data_ptr(), (E*)dv.data_ptr(),
            slots > 0 ? work.data_ptr<float>() : nullptr, split, a);
     if (slots > 0) {
       const int tile0 = split.c_first > 1 ? 0 : split.n_first;

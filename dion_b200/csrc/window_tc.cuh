@@ -323,50 +323,53 @@ __global__ void __launch_bounds__(192, 2)
 }
 
 // ------------------------------------------------------------ backward: dQ
-// Column of the 16 elements that product k of a step reads. Each of the two
+// Column of the 16 elements that product k of a step reads. Each of the four
 // threads of a row packs its 32 elements into the first 16 of the 32 columns
-// that it has read itself, so neither waits for the other.
-__device__ constexpr int half_col(int k) { return k / 2 * 32 + k % 2 * 8; }
+// that it has read itself, so none waits for another.
+__device__ constexpr int part_col(int k) { return k / 2 * 32 + k % 2 * 8; }
 
 template <typename T, int DP>
 struct DqCfg {
   static constexpr int kPanels = DP / 64;
-  static constexpr int kRowBytes = kPanels * kPanel;       // Q, dO
-  static constexpr int kStepBytes = kPanels * kHalfPanel;  // K, V
-  static constexpr int kStages = DP == 64 ? 2 : 1;
-  static constexpr int kSmemBytes = 2 * kRowBytes + 2 * kStages * kStepBytes + 1024 + 128 + kTile * 4;
-  static constexpr int kTmemCols = 256;
-  // columns: S [0, 64), dP [64, 128), dS [128, 192) where there is room (else on S), dQ at the end
-  static constexpr bool kOverlay = DP == 128;
-  static constexpr int kDS = kOverlay ? 0 : 128;
-  static constexpr int kDQ = 256 - DP;
+  static constexpr int kRowBytes = kPanels * kPanel;  // Q, dO; K, V of a step
+  // K stays until its step's dQ, so the step after next needs a third place for it
+  static constexpr int kStagesK = 3, kStagesV = 2;
+  static constexpr int kSmemBytes = (2 + kStagesK + kStagesV) * kRowBytes + 1024 + 256 + kTile * 4;
+  static constexpr int kTmemCols = 512;
+  // columns: S at 0, two buffers of dP with dS on them, dQ
+  static constexpr int kDP = 128, kDQ = 384;
 };
 
-// One CTA per (128 queries, head, sequence), two to an SM: S and dP by the
-// tensor cores, dS = P o (dP - delta) by two threads per query row (half of the
-// step's keys each: one thread's chain of loads and exponentials was longer
-// than the products), dQ += dS K with dS read from TMEM. delta is taken here from O and dO and kept for the
-// dK / dV kernel (0 behind the last position).
+// One CTA per (128 queries, head, sequence), one to an SM, steps of 128 keys: S
+// and dP by the tensor cores, dS = P o (dP - delta) by four threads per query
+// row (a quarter of the step's keys each), dQ += dS K with dS read from TMEM.
+// The next step's S is computed as soon as the rows have read this one's, its dP
+// goes into the other buffer, so the rows work from step to step without waiting
+// for the sums. (Steps of 64 keys: a product of 128 x 64 x 16 takes as long from
+// shared memory as one of 128 x 128 x 16.) delta is taken here from O and dO and
+// kept, negated, for the dK / dV kernel (0 behind the last position).
 template <typename T, int DP>
-__global__ void __launch_bounds__(320, 2)
+__global__ void __launch_bounds__(576, 1)
     window_dq_tc(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                  const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap tg,
                  const T* __restrict__ o, const T* __restrict__ go, int64_t go_b, int64_t go_s, int64_t go_h,
-                 const float* __restrict__ neg_lse, float* __restrict__ neg_delta, T* __restrict__ dq, const WinArgs a) {
+                 const float* __restrict__ neg_lse, float* __restrict__ neg_delta, T* __restrict__ dq,
+                 const WinArgs a) {
   using Cfg = DqCfg<T, DP>;
-  constexpr int ST = Cfg::kStages;
+  constexpr int SK = Cfg::kStagesK, SV = Cfg::kStagesV;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sQ = smem;
   uint8_t* sG = sQ + Cfg::kRowBytes;
   uint8_t* sK = sG + Cfg::kRowBytes;
-  uint8_t* sV = sK + ST * Cfg::kStepBytes;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sV + ST * Cfg::kStepBytes);
-  uint64_t *q_full = bars, *k_full = bars + 1, *k_empty = bars + 3, *v_full = bars + 5, *v_empty = bars + 7,
-           *s_full = bars + 9, *p_full = bars + 10, *o_full = bars + 11, *drain = bars + 12;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 13);
-  volatile int* abort = reinterpret_cast<volatile int*>(bars + 14);
-  float* s_delta = reinterpret_cast<float*>(bars + 16);
+  uint8_t* sV = sK + SK * Cfg::kRowBytes;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sV + SV * Cfg::kRowBytes);
+  uint64_t *q_full = bars, *k_full = bars + 1, *k_empty = bars + 4, *v_full = bars + 7, *v_empty = bars + 9,
+           *s_full = bars + 11, *s_read = bars + 12, *dp_full = bars + 13, *ds_full = bars + 15, *dq_done = bars + 17,
+           *all_done = bars + 19, *drain = bars + 20;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 21);
+  volatile int* abort = reinterpret_cast<volatile int*>(bars + 22);
+  float* s_delta = reinterpret_cast<float*>(bars + 24);
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
   const int h = blockIdx.x % a.hq;
@@ -374,19 +377,24 @@ __global__ void __launch_bounds__(320, 2)
   const int q0 = (blockIdx.x / a.hq) % n_q * kTile;
   const int b = blockIdx.x / a.hq / n_q;
   const int hk = h / (a.hq / a.hkv);
-  const KeyTiles<kHalfTile> tiles(a, q0);
+  const KeyTiles<kTile> tiles(a, q0);
 
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
-    for (int i = 0; i < 2; ++i) {
+    mbar_init(s_full, 1);
+    mbar_init(s_read, 16);
+    for (int i = 0; i < SK; ++i) {
       mbar_init(&k_full[i], 1);
       mbar_init(&k_empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
       mbar_init(&v_full[i], 1);
       mbar_init(&v_empty[i], 1);
+      mbar_init(&dp_full[i], 1);
+      mbar_init(&ds_full[i], 16);
+      mbar_init(&dq_done[i], 1);
     }
-    mbar_init(s_full, 1);
-    mbar_init(p_full, 8);
-    mbar_init(o_full, 1);
+    mbar_init(all_done, 1);
     mbar_init(drain, 1);
     *abort = 0;
     fence_mbar_init();
@@ -411,94 +419,100 @@ __global__ void __launch_bounds__(320, 2)
       int t = 0;
       bool ok = true;
       for (; t < tiles.n; ++t) {
-        const int st = t % ST, k0 = tiles.k0(t);
-        const uint32_t ph = (t / ST) & 1;
-        // V is free once dP is done, K only after dQ
-        if (!mbar_wait_bounded(&v_empty[st], ph ^ 1, abort, limit)) { ok = false; break; }
-        mbar_arrive_expect_tx(&v_full[st], Cfg::kStepBytes);
+        const int sk = t % SK, sv = t % SV, k0 = tiles.k0(t);
+        // K is free once dQ is done, V already after dP
+        if (!mbar_wait_bounded(&k_empty[sk], ((t / SK) & 1) ^ 1, abort, limit)) { ok = false; break; }
+        mbar_arrive_expect_tx(&k_full[sk], Cfg::kRowBytes);
         for (int p = 0; p < Cfg::kPanels; ++p)
-          tma_load_4d(&tv, &v_full[st], sV + st * Cfg::kStepBytes + p * kHalfPanel, p * 64, k0, hk, b);
-        if (!mbar_wait_bounded(&k_empty[st], ph ^ 1, abort, limit)) { ok = false; break; }
-        mbar_arrive_expect_tx(&k_full[st], Cfg::kStepBytes);
+          tma_load_4d(&tk, &k_full[sk], sK + sk * Cfg::kRowBytes + p * kPanel, p * 64, k0, hk, b);
+        if (!mbar_wait_bounded(&v_empty[sv], ((t / SV) & 1) ^ 1, abort, limit)) { ok = false; break; }
+        mbar_arrive_expect_tx(&v_full[sv], Cfg::kRowBytes);
         for (int p = 0; p < Cfg::kPanels; ++p)
-          tma_load_4d(&tk, &k_full[st], sK + st * Cfg::kStepBytes + p * kHalfPanel, p * 64, k0, hk, b);
+          tma_load_4d(&tv, &v_full[sv], sV + sv * Cfg::kRowBytes + p * kPanel, p * 64, k0, hk, b);
       }
       if (!ok) {
         report_status(a.status, kStatusWindowProducerTimeout);
         const uint64_t t0 = globaltimer_ns();
         while (!mbar_try_wait(q_full, 0) && globaltimer_ns() - t0 < 100000000ull) {
         }
-        for (int i = max(0, t - ST); i <= t; ++i) {
-          while (!mbar_try_wait(&k_full[i % ST], (i / ST) & 1) && globaltimer_ns() - t0 < 100000000ull) {
+        for (int i = max(0, t - SK); i <= t; ++i) {
+          while (!mbar_try_wait(&k_full[i % SK], (i / SK) & 1) && globaltimer_ns() - t0 < 100000000ull) {
           }
-          while (!mbar_try_wait(&v_full[i % ST], (i / ST) & 1) && globaltimer_ns() - t0 < 100000000ull) {
+          while (!mbar_try_wait(&v_full[i % SV], (i / SV) & 1) && globaltimer_ns() - t0 < 100000000ull) {
           }
         }
       }
     }
   } else if (warp == 1) {
-    {
-      const bool leader = elect_one();
-      constexpr uint32_t kS = make_idesc(kTile, kHalfTile, false, false, AttnType<T>::kFmt);
-      constexpr uint32_t kD = make_idesc(kTile, DP, false, true, AttnType<T>::kFmt);
-      const uint32_t q_base = smem_u32(sQ), g_base = smem_u32(sG);
-      bool ok = warp_wait(q_full, 0, abort, limit);
-      auto scores = [&](int t) {
-        const int st = t % ST;
-        const uint32_t ph = (t / ST) & 1;
-        if (!warp_wait(&v_full[st], ph, abort, limit) || !warp_wait(&k_full[st], ph, abort, limit))
-          return false;
-        tc_fence_after();
-        const uint32_t k_base = smem_u32(sK + st * Cfg::kStepBytes), v_base = smem_u32(sV + st * Cfg::kStepBytes);
+    const bool leader = elect_one();
+    constexpr uint32_t kS = make_idesc(kTile, kTile, false, false, AttnType<T>::kFmt);
+    constexpr uint32_t kD = make_idesc(kTile, DP, false, true, AttnType<T>::kFmt);
+    const uint32_t q_base = smem_u32(sQ), g_base = smem_u32(sG);
+    bool ok = warp_wait(q_full, 0, abort, limit);
+    auto scores = [&](int t) {  // S of step t; the rows have read the step before it
+      if (!warp_wait(&k_full[t % SK], (t / SK) & 1, abort, limit)) return false;
+      if (t > 0 && !warp_wait(s_read, (t - 1) & 1, abort, limit)) return false;
+      tc_fence_after();
+      const uint32_t k_base = smem_u32(sK + t % SK * Cfg::kRowBytes);
 #pragma unroll
-        for (int k = 0; k < DP / 16; ++k) {
-          const uint32_t qo = (k / 4) * kPanel + (k % 4) * 32, ko = (k / 4) * kHalfPanel + (k % 4) * 32;
-          umma_ss(leader, tmem, sdesc_low(q_base + qo, 16), sdesc_low(k_base + ko, 16), kS, k != 0);
-          umma_ss(leader, tmem + 64, sdesc_low(g_base + qo, 16), sdesc_low(v_base + ko, 16), kS, k != 0);
+      for (int k = 0; k < DP / 16; ++k) {
+        const uint32_t off = (k / 4) * kPanel + (k % 4) * 32;
+        umma_ss(leader, tmem, sdesc_low(q_base + off, 16), sdesc_low(k_base + off, 16), kS, k != 0);
       }
-        umma_commit_by(leader, &v_empty[st]);
-        umma_commit_by(leader, s_full);
-        return true;
-      };
-      if (ok) ok = scores(0);
-      for (int t = 0; t < tiles.n && ok; ++t) {
-        const int st = t % ST;
-        ok = warp_wait(p_full, t & 1, abort, limit);
-        if (!ok) break;
-        tc_fence_after();
-        if (!Cfg::kOverlay && t + 1 < tiles.n && !scores(t + 1)) { ok = false; break; }
-        const uint32_t k_base = smem_u32(sK + st * Cfg::kStepBytes);
+      umma_commit_by(leader, s_full);
+      return true;
+    };
+    auto grads = [&](int t) {  // dP of step t; its buffer's dS of two steps ago has been read
+      if (!warp_wait(&v_full[t % SV], (t / SV) & 1, abort, limit)) return false;
+      if (t >= 2 && !warp_wait(&dq_done[t & 1], ((t >> 1) - 1) & 1, abort, limit)) return false;
+      tc_fence_after();
+      const uint32_t v_base = smem_u32(sV + t % SV * Cfg::kRowBytes);
 #pragma unroll
-        for (int k = 0; k < kHalfTile / 16; ++k)
-          umma_ts(leader, tmem + Cfg::kDQ, tmem + Cfg::kDS + half_col(k), sdesc_low(k_base + k * 2048, kHalfPanel), kD,
-                      (t | k) != 0);
-        umma_commit_by(leader, &k_empty[st]);
-        umma_commit_by(leader, o_full);
-        if (Cfg::kOverlay && t + 1 < tiles.n) ok = warp_wait(o_full, t & 1, abort, limit) && scores(t + 1);
+      for (int k = 0; k < DP / 16; ++k) {
+        const uint32_t off = (k / 4) * kPanel + (k % 4) * 32;
+        umma_ss(leader, tmem + Cfg::kDP + (t & 1) * 128, sdesc_low(g_base + off, 16), sdesc_low(v_base + off, 16), kS,
+                k != 0);
       }
-      if (!ok) {
-        if (lane == 0) report_status(a.status, kStatusWindowMmaTimeout);
-        umma_commit_by(leader, drain);
-        const uint64_t t0 = globaltimer_ns();
-        while (!mbar_try_wait(drain, 0) && globaltimer_ns() - t0 < 100000000ull) {
-        }
+      umma_commit_by(leader, &v_empty[t % SV]);
+      umma_commit_by(leader, &dp_full[t & 1]);
+      return true;
+    };
+    if (ok) ok = scores(0) && grads(0);
+    for (int t = 0; t < tiles.n && ok; ++t) {
+      if (t + 1 < tiles.n && !(scores(t + 1) && grads(t + 1))) { ok = false; break; }
+      if (!warp_wait(&ds_full[t & 1], (t >> 1) & 1, abort, limit)) { ok = false; break; }
+      tc_fence_after();
+      const uint32_t k_base = smem_u32(sK + t % SK * Cfg::kRowBytes);
+#pragma unroll
+      for (int k = 0; k < kTile / 16; ++k)
+        umma_ts(leader, tmem + Cfg::kDQ, tmem + Cfg::kDP + (t & 1) * 128 + part_col(k), sdesc_low(k_base + k * 2048, kPanel),
+                kD, (t | k) != 0);
+      umma_commit_by(leader, &k_empty[t % SK]);
+      umma_commit_by(leader, &dq_done[t & 1]);
+    }
+    if (ok) {
+      umma_commit_by(leader, all_done);
+    } else {
+      if (lane == 0) report_status(a.status, kStatusWindowMmaTimeout);
+      umma_commit_by(leader, drain);
+      const uint64_t t0 = globaltimer_ns();
+      while (!mbar_try_wait(drain, 0) && globaltimer_ns() - t0 < 100000000ull) {
       }
     }
   } else {
-    const int quarter = warp & 3, half = (warp - 2) / 4;
+    const int quarter = warp & 3, part = (warp - 2) / 4;
     const int r = quarter * 32 + lane, i = q0 + r;
     const uint32_t row = tmem + ((uint32_t)(quarter * 32) << 16);
-    const float c = a.scale_log2;
     const int64_t at = ((int64_t)b * a.hq + h) * a.s_pad + q0;
-    const f2 c2 = make_f2(c, c), neg_l = make_f2(neg_lse[at + r], neg_lse[at + r]);
+    const f2 c2 = make_f2(a.scale_log2, a.scale_log2), neg_l = make_f2(neg_lse[at + r], neg_lse[at + r]);
     {
-      // delta of 16 rows per warp, DP / 8 lanes to a row
+      // delta of 8 rows per warp, DP / 8 lanes to a row
       constexpr int kLanes = DP / 8, kRows = 32 / kLanes;
       const int col = lane % kLanes * 8;
-      float v[16 / kRows];
+      float v[8 / kRows];
 #pragma unroll
-      for (int n = 0; n < 16 / kRows; ++n) {
-        const int rr = q0 + (warp - 2) * 16 + n * kRows + lane / kLanes;
+      for (int n = 0; n < 8 / kRows; ++n) {
+        const int rr = q0 + (warp - 2) * 8 + n * kRows + lane / kLanes;
         v[n] = 0.f;
         if (rr < a.s && col < a.d) {
           const uint4 ou = *reinterpret_cast<const uint4*>(o + (((int64_t)b * a.s + rr) * a.hq + h) * a.d + col);
@@ -509,16 +523,16 @@ __global__ void __launch_bounds__(320, 2)
         }
       }
 #pragma unroll
-      for (int n = 0; n < 16 / kRows; ++n) {
+      for (int n = 0; n < 8 / kRows; ++n) {
 #pragma unroll
         for (int m = kLanes / 2; m > 0; m >>= 1) v[n] += __shfl_xor_sync(0xffffffffu, v[n], m);
-        const int rr = (warp - 2) * 16 + n * kRows + lane / kLanes;
+        const int rr = (warp - 2) * 8 + n * kRows + lane / kLanes;
         if (col == 0) {
           s_delta[rr] = -v[n];
           neg_delta[at + rr] = -v[n];
         }
       }
-      asm volatile("bar.sync 1, 256;" ::: "memory");
+      asm volatile("bar.sync 1, 512;" ::: "memory");
     }
     const f2 neg_d = make_f2(s_delta[r], s_delta[r]);
     bool ok = true;
@@ -526,40 +540,43 @@ __global__ void __launch_bounds__(320, 2)
       const int k0 = tiles.k0(t);
       if (!warp_wait(s_full, t & 1, abort, limit)) { ok = false; break; }
       tc_fence_after();
-      uint32_t x[32], y[32];
-      tmem_ld_32x32b_x32(row + half * 32, x);
-      tmem_ld_32x32b_x32(row + 64 + half * 32, y);
+      uint32_t x[32];
+      f2 p[16];
+      tmem_ld_32x32b_x32(row + part * 32, x);
       tmem_wait_ld();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(s_read);
       if (!tiles.whole(a, q0, k0)) {
-        const uint32_t seen = seen_mask(a, i, k0 + half * 32);
+        const uint32_t seen = seen_mask(a, i, k0 + part * 32);
 #pragma unroll
         for (int e = 0; e < 32; ++e)
-          if (!((seen >> e) & 1u)) x[e] = 0xff800000u;
+          if (!((seen >> e) & 1u)) x[e] = 0xff800000u;  // -inf
       }
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const f2 z = make_f2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1]));
-        const f2 g = make_f2(__uint_as_float(y[2 * e]), __uint_as_float(y[2 * e + 1]));
-        x[e] = pack2(mul2(ex2_pair(e, fma2(z, c2, neg_l)), add2(g, neg_d)), T{});
-      }
-      if (!Cfg::kOverlay && t > 0) {  // dS's place is free once the step before is done
-        if (!warp_wait(o_full, (t - 1) & 1, abort, limit)) { ok = false; break; }
-        tc_fence_after();
-      }
-      tmem_st_32x32b_x16(row + Cfg::kDS + half * 32, x);
+      for (int e = 0; e < 16; ++e)
+        p[e] = ex2_pair(e, fma2(make_f2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])), c2, neg_l));
+      if (!warp_wait(&dp_full[t & 1], (t >> 1) & 1, abort, limit)) { ok = false; break; }
+      tc_fence_after();
+      const uint32_t buf = row + Cfg::kDP + (t & 1) * 128 + part * 32;
+      tmem_ld_32x32b_x32(buf, x);
+      tmem_wait_ld();
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        x[e] = pack2(mul2(p[e], add2(make_f2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])), neg_d)), T{});
+      tmem_st_32x32b_x16(buf, x);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(p_full);
+      if (lane == 0) mbar_arrive(&ds_full[t & 1]);
     }
-    if (ok) ok = warp_wait(o_full, (tiles.n - 1) & 1, abort, limit);
+    if (ok) ok = warp_wait(all_done, 0, abort, limit);
     if (!ok) {
       if (lane == 0) report_status(a.status, kStatusWindowSoftmaxTimeout);
     } else {
       tc_fence_after();
       T* out = dq + (((int64_t)b * a.s + i) * a.hq + h) * a.d;
-#pragma unroll
-      for (int j = half * (DP / 64); j < (half + 1) * (DP / 64); ++j) {
+      for (int j = part; j < DP / 32; j += 4) {
         uint32_t y[32];
         tmem_ld_32x32b_x32(row + Cfg::kDQ + j * 32, y);
         tmem_wait_ld();
@@ -585,7 +602,7 @@ __global__ void __launch_bounds__(320, 2)
 }
 
 // ------------------------------------------------------------ backward: dK, dV
-// How the key tiles' steps (a step: 64 queries of one head) are split over
+// How the key tiles' steps (a step: 128 queries of one head) are split over
 // CTAs. The queries that see first tokens reach to the end of the sequence,
 // those of every other tile only as far as the window: the tiles with first
 // tokens are cut into `c_first` parts, the others into `c_band`. A part of a
@@ -612,22 +629,24 @@ struct KeySplit {
 template <typename T, int DP>
 struct DkvCfg {
   static constexpr int kPanels = DP / 64;
-  static constexpr int kRowBytes = kPanels * kPanel;       // K, V
-  static constexpr int kStepBytes = kPanels * kHalfPanel;  // Q, dO
-  static constexpr int kStages = DP == 64 ? 4 : 3;
-  static constexpr int kStatBytes = kHalfTile * 4;
-  static constexpr int kSmemBytes = 2 * kRowBytes + kStages * (2 * kStepBytes + 2 * kStatBytes) + 1024 + 512;
+  static constexpr int kRowBytes = kPanels * kPanel;  // K, V; Q, dO of a step
+  static constexpr int kStages = DP == 64 ? 3 : 2;
+  static constexpr int kStatBytes = kTile * 4;
+  static constexpr int kSmemBytes = 2 * kRowBytes + kStages * (2 * kRowBytes + 2 * kStatBytes) + 1024 + 256;
   static constexpr int kTmemCols = 512;
-  // columns: buffers of (S^T, dP^T) with P^T and dS^T on them, then dV and dK
-  static constexpr int kBufs = DP == 64 ? 3 : 2;
-  static constexpr int kDV = kBufs * 128, kDK = kDV + DP;
+  // columns: S^T at 0 with P^T on it, dP^T at 128 with dS^T on it, dV, dK; a second
+  // buffer of S^T behind them where there is room
+  static constexpr int kDPT = 128, kDV = 256, kDK = 256 + DP;
+  static constexpr int kBufs = DP == 64 ? 2 : 1;
+  static constexpr int kSecond = 384;
 };
 
-// One CTA per (128 keys, key head, sequence, part). With the keys as rows, P^T
-// and dS^T come out of TMEM in the place where dV += P^T dO and dK += dS^T Q
-// want their A operand, so neither passes through shared memory. Two groups of
-// eight warps take the steps in turn, each with its own buffer; within a group
-// two threads share a key row, half of the step's queries each.
+// One CTA per (128 keys, key head, sequence, part), steps of 128 queries of one
+// head. With the keys as rows, P^T and dS^T come out of TMEM in the place where
+// dV += P^T dO and dK += dS^T Q want their A operand, so neither passes through
+// shared memory. Four threads share a key row, a quarter of the step's queries
+// each; while they make P^T the tensor cores make dP^T, and dV while they make
+// dS^T.
 template <typename T, int DP>
 __global__ void __launch_bounds__(576, 1)
     window_dkv_tc(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
@@ -635,20 +654,21 @@ __global__ void __launch_bounds__(576, 1)
                   const float* __restrict__ neg_lse, const float* __restrict__ neg_delta, T* __restrict__ dk,
                   T* __restrict__ dv, float* __restrict__ work, const KeySplit split, const WinArgs a) {
   using Cfg = DkvCfg<T, DP>;
-  constexpr int ST = Cfg::kStages;
+  constexpr int ST = Cfg::kStages, NB = Cfg::kBufs;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sK = smem;
   uint8_t* sV = sK + Cfg::kRowBytes;
   uint8_t* sQ = sV + Cfg::kRowBytes;
-  uint8_t* sG = sQ + ST * Cfg::kStepBytes;
-  float* sL = reinterpret_cast<float*>(sG + ST * Cfg::kStepBytes);
-  float* sD = sL + ST * kHalfTile;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sD + ST * kHalfTile);
-  uint64_t *k_full = bars, *q_full = bars + 1, *q_empty = bars + 5, *s_full = bars + 9, *p_full = bars + 12,
-           *acc_done = bars + 15, *all_done = bars + 18, *drain = bars + 19;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 20);
-  volatile int* abort = reinterpret_cast<volatile int*>(bars + 21);
+  uint8_t* sG = sQ + ST * Cfg::kRowBytes;
+  float* sL = reinterpret_cast<float*>(sG + ST * Cfg::kRowBytes);
+  float* sD = sL + ST * kTile;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sD + ST * kTile);
+  uint64_t *k_full = bars, *q_full = bars + 1, *q_empty = bars + 4, *s_full = bars + 7, *p_full = bars + 9,
+           *dv_done = bars + 11, *dp_full = bars + 13, *ds_full = bars + 14, *dk_done = bars + 15, *all_done = bars + 16,
+           *drain = bars + 17;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 18);
+  volatile int* abort = reinterpret_cast<volatile int*>(bars + 19);
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
   const int hk = blockIdx.x % a.hkv, group = a.hq / a.hkv;
@@ -659,24 +679,27 @@ __global__ void __launch_bounds__(576, 1)
   const int parts = split.of(tile), mine = part - split.first_part(tile);
   const int k0 = tile * kTile;
   // steps of the whole tile, and this part's
-  const int q_first = k0 / kHalfTile;
+  const int q_first = k0 / kTile;
   const int last_key = min(k0 + kTile, a.s) - 1;
-  const int q_last = (k0 < a.sinks ? a.s - 1 : (int)min((int64_t)a.s - 1, (int64_t)last_key + a.window - 1)) / kHalfTile;
+  const int q_last = (k0 < a.sinks ? a.s - 1 : (int)min((int64_t)a.s - 1, (int64_t)last_key + a.window - 1)) / kTile;
   const int nq = q_last - q_first + 1;
   const int64_t all = (int64_t)nq * group;
   const int lo = (int)(all * mine / parts), n = (int)(all * (mine + 1) / parts) - lo;
 
   if (threadIdx.x == 0) {
     mbar_init(k_full, 1);
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < ST; ++i) {
       mbar_init(&q_full[i], 1);
       mbar_init(&q_empty[i], 1);
     }
-    for (int i = 0; i < Cfg::kBufs; ++i) {
+    for (int i = 0; i < NB; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 8);
-      mbar_init(&acc_done[i], 1);
+      mbar_init(&p_full[i], 16);
+      mbar_init(&dv_done[i], 1);
     }
+    mbar_init(dp_full, 1);
+    mbar_init(ds_full, 16);
+    mbar_init(dk_done, 1);
     mbar_init(all_done, 1);
     mbar_init(drain, 1);
     *abort = 0;
@@ -703,16 +726,16 @@ __global__ void __launch_bounds__(576, 1)
       int t = 0;
       for (; t < n; ++t) {
         const int st = t % ST;
-        const int h = hk * group + (lo + t) / nq, q0 = (q_first + (lo + t) % nq) * kHalfTile;
+        const int h = hk * group + (lo + t) / nq, q0 = (q_first + (lo + t) % nq) * kTile;
         if (!mbar_wait_bounded(&q_empty[st], ((t / ST) & 1) ^ 1, abort, limit)) { ok = false; break; }
-        mbar_arrive_expect_tx(&q_full[st], 2 * Cfg::kStepBytes + 2 * Cfg::kStatBytes);
+        mbar_arrive_expect_tx(&q_full[st], 2 * Cfg::kRowBytes + 2 * Cfg::kStatBytes);
         for (int p = 0; p < Cfg::kPanels; ++p) {
-          tma_load_4d(&tq, &q_full[st], sQ + st * Cfg::kStepBytes + p * kHalfPanel, p * 64, q0, h, b);
-          tma_load_4d(&tg, &q_full[st], sG + st * Cfg::kStepBytes + p * kHalfPanel, p * 64, q0, h, b);
+          tma_load_4d(&tq, &q_full[st], sQ + st * Cfg::kRowBytes + p * kPanel, p * 64, q0, h, b);
+          tma_load_4d(&tg, &q_full[st], sG + st * Cfg::kRowBytes + p * kPanel, p * 64, q0, h, b);
         }
         const int64_t at = ((int64_t)b * a.hq + h) * a.s_pad + q0;
-        bulk_load(sL + st * kHalfTile, neg_lse + at, Cfg::kStatBytes, &q_full[st]);
-        bulk_load(sD + st * kHalfTile, neg_delta + at, Cfg::kStatBytes, &q_full[st]);
+        bulk_load(sL + st * kTile, neg_lse + at, Cfg::kStatBytes, &q_full[st]);
+        bulk_load(sD + st * kTile, neg_delta + at, Cfg::kStatBytes, &q_full[st]);
       }
       if (!ok) {
         report_status(a.status, kStatusWindowProducerTimeout);
@@ -727,47 +750,59 @@ __global__ void __launch_bounds__(576, 1)
   } else if (warp == 1) {
     if (n > 0) {
       const bool leader = elect_one();
-      constexpr uint32_t kS = make_idesc(kTile, kHalfTile, false, false, AttnType<T>::kFmt);
+      constexpr uint32_t kS = make_idesc(kTile, kTile, false, false, AttnType<T>::kFmt);
       constexpr uint32_t kD = make_idesc(kTile, DP, false, true, AttnType<T>::kFmt);
       const uint32_t k_base = smem_u32(sK), v_base = smem_u32(sV);
+      auto s_col = [&](int t) { return tmem + (NB == 2 && (t & 1) ? Cfg::kSecond : 0); };
       bool ok = warp_wait(k_full, 0, abort, limit);
-      auto scores = [&](int t) {
-        const int st = t % ST, buf = t % Cfg::kBufs;
-        if (!warp_wait(&q_full[st], (t / ST) & 1, abort, limit)) return false;
-        // the buffer's P^T and dS^T of the step before in it have been read
-        if (t >= Cfg::kBufs && !warp_wait(&acc_done[buf], (t / Cfg::kBufs - 1) & 1, abort, limit)) return false;
+      auto scores = [&](int t) {  // S^T of step t; the P^T in its buffer has been read
+        if (!warp_wait(&q_full[t % ST], (t / ST) & 1, abort, limit)) return false;
+        if (t >= NB && !warp_wait(&dv_done[t % NB], (t / NB - 1) & 1, abort, limit)) return false;
         tc_fence_after();
-        const uint32_t q_base = smem_u32(sQ + st * Cfg::kStepBytes), g_base = smem_u32(sG + st * Cfg::kStepBytes);
-        const uint32_t d = tmem + buf * 128;
+        const uint32_t q_base = smem_u32(sQ + t % ST * Cfg::kRowBytes);
 #pragma unroll
         for (int k = 0; k < DP / 16; ++k) {
-          const uint32_t ko = (k / 4) * kPanel + (k % 4) * 32, qo = (k / 4) * kHalfPanel + (k % 4) * 32;
-          umma_ss(leader, d, sdesc_low(k_base + ko, 16), sdesc_low(q_base + qo, 16), kS, k != 0);
-          umma_ss(leader, d + 64, sdesc_low(v_base + ko, 16), sdesc_low(g_base + qo, 16), kS, k != 0);
+          const uint32_t off = (k / 4) * kPanel + (k % 4) * 32;
+          umma_ss(leader, s_col(t), sdesc_low(k_base + off, 16), sdesc_low(q_base + off, 16), kS, k != 0);
         }
-        umma_commit_by(leader, &s_full[buf]);
+        umma_commit_by(leader, &s_full[t % NB]);
         return true;
       };
-      // Scores run ahead of the steps' sums: by two steps with three buffers. With two
-      // they have to come before the sums of the step that the other group works on.
-      constexpr int kAhead = Cfg::kBufs - 1;
-      for (int t = 0; t < min(n, kAhead) && ok; ++t) ok = scores(t);
-      for (int t = 0; t < n && ok; ++t) {
-        const int st = t % ST, buf = t % Cfg::kBufs;
-        if (Cfg::kBufs == 2 && t + 1 < n && !scores(t + 1)) { ok = false; break; }
-        if (!warp_wait(&p_full[buf], (t / Cfg::kBufs) & 1, abort, limit)) { ok = false; break; }
+      auto grads = [&](int t) {  // dP^T of step t; the dS^T before it has been read
+        if (!warp_wait(&q_full[t % ST], (t / ST) & 1, abort, limit)) return false;
+        if (t >= 1 && !warp_wait(dk_done, (t - 1) & 1, abort, limit)) return false;
         tc_fence_after();
-        const uint32_t q_base = smem_u32(sQ + st * Cfg::kStepBytes), g_base = smem_u32(sG + st * Cfg::kStepBytes);
-        const uint32_t d = tmem + buf * 128;
+        const uint32_t g_base = smem_u32(sG + t % ST * Cfg::kRowBytes);
 #pragma unroll
-        for (int k = 0; k < kHalfTile / 16; ++k) {
-          umma_ts(leader, tmem + Cfg::kDV, d + half_col(k), sdesc_low(g_base + k * 2048, kHalfPanel), kD, (t | k) != 0);
-          umma_ts(leader, tmem + Cfg::kDK, d + 64 + half_col(k), sdesc_low(q_base + k * 2048, kHalfPanel), kD,
-                      (t | k) != 0);
+        for (int k = 0; k < DP / 16; ++k) {
+          const uint32_t off = (k / 4) * kPanel + (k % 4) * 32;
+          umma_ss(leader, tmem + Cfg::kDPT, sdesc_low(v_base + off, 16), sdesc_low(g_base + off, 16), kS, k != 0);
         }
+        umma_commit_by(leader, dp_full);
+        return true;
+      };
+      if (ok) ok = scores(0) && grads(0) && (NB == 1 || n == 1 || scores(1));
+      for (int t = 0; t < n && ok; ++t) {
+        const int st = t % ST;
+        const uint32_t q_base = smem_u32(sQ + st * Cfg::kRowBytes), g_base = smem_u32(sG + st * Cfg::kRowBytes);
+        if (!warp_wait(&p_full[t % NB], (t / NB) & 1, abort, limit)) { ok = false; break; }
+        tc_fence_after();
+#pragma unroll
+        for (int k = 0; k < kTile / 16; ++k)
+          umma_ts(leader, tmem + Cfg::kDV, s_col(t) + part_col(k), sdesc_low(g_base + k * 2048, kPanel), kD, (t | k) != 0);
+        umma_commit_by(leader, &dv_done[t % NB]);
+        // with one buffer the next scores come before dK: the rows wait for them
+        if (NB == 1 && t + 1 < n && !scores(t + 1)) { ok = false; break; }
+        if (!warp_wait(ds_full, t & 1, abort, limit)) { ok = false; break; }
+        tc_fence_after();
+#pragma unroll
+        for (int k = 0; k < kTile / 16; ++k)
+          umma_ts(leader, tmem + Cfg::kDK, tmem + Cfg::kDPT + part_col(k), sdesc_low(q_base + k * 2048, kPanel), kD,
+                  (t | k) != 0);
         umma_commit_by(leader, &q_empty[st]);
-        umma_commit_by(leader, &acc_done[buf]);
-        if (Cfg::kBufs > 2 && t + kAhead < n) ok = scores(t + kAhead);
+        umma_commit_by(leader, dk_done);
+        if (NB == 2 && t + 2 < n && !scores(t + 2)) { ok = false; break; }
+        if (t + 1 < n && !grads(t + 1)) { ok = false; break; }
       }
       if (ok) {
         umma_commit_by(leader, all_done);
@@ -780,61 +815,80 @@ __global__ void __launch_bounds__(576, 1)
       }
     }
   } else {
-    const int quarter = warp & 3, which = (warp - 2) / 8, half = (warp - 2) / 4 % 2;
+    const int quarter = warp & 3, part = (warp - 2) / 4;
     const int r = quarter * 32 + lane, j = k0 + r;
     const uint32_t row = tmem + ((uint32_t)(quarter * 32) << 16);
-    const float c = a.scale_log2;
+    const f2 c2 = make_f2(a.scale_log2, a.scale_log2);
     bool ok = true;
-    for (int t = which; t < n; t += 2) {
-      const int st = t % ST, q0 = (q_first + (lo + t) % nq) * kHalfTile;
-      const int nbuf = t % Cfg::kBufs;
-      const uint32_t buf = row + nbuf * 128;
-      if (!warp_wait(&s_full[nbuf], (t / Cfg::kBufs) & 1, abort, limit)) { ok = false; break; }
+    int qt = lo % nq, st = 0;  // this step's query tile (from q_first) and stage
+    for (int t = 0; t < n; ++t) {
+      const int q0 = (q_first + qt) * kTile;
+      const uint32_t s_at = row + (NB == 2 && (t & 1) ? Cfg::kSecond : 0) + part * 32;
+      // (the stage's copies as well: the rows read lse and delta from it)
+      if (!warp_wait(&q_full[st], (t / ST) & 1, abort, limit)) { ok = false; break; }
+      if (!warp_wait(&s_full[t % NB], (t / NB) & 1, abort, limit)) { ok = false; break; }
       tc_fence_after();
-      uint32_t x[32], y[32];
-      tmem_ld_32x32b_x32(buf + half * 32, x);
-      tmem_ld_32x32b_x32(buf + 64 + half * 32, y);
+      uint32_t x[32];
+      f2 p[16];
+      tmem_ld_32x32b_x32(s_at, x);
       tmem_wait_ld();
       // queries q0 + e that see key j: e in [j - q0, j + window - q0), without an end for first tokens
-      if (!(q0 >= k0 + kTile - 1 && (q0 + kHalfTile - 1 - k0 < a.window || k0 + kTile <= a.sinks))) {
-        const int e0 = j - q0 - half * 32;
-        const int e1 = j < a.sinks ? kHalfTile : (int)min((int64_t)kHalfTile, (int64_t)j + a.window - q0 - half * 32);
+      if (!(q0 >= k0 + kTile - 1 && (q0 + kTile - 1 - k0 < a.window || k0 + kTile <= a.sinks))) {
+        const int e0 = j - q0 - part * 32;
+        const int e1 = j < a.sinks ? kTile : (int)min((int64_t)kTile, (int64_t)j + a.window - q0 - part * 32);
 #pragma unroll
         for (int e = 0; e < 32; ++e)
-          if (e < e0 || e >= e1) x[e] = 0xff800000u;
+          if (e < e0 || e >= e1) x[e] = 0xff800000u;  // -inf
       }
-      const float *pl = sL + st * kHalfTile + half * 32, *pd = sD + st * kHalfTile + half * 32;
-      const f2 c2 = make_f2(c, c);
+      const float *pl = sL + st * kTile + part * 32, *pd = sD + st * kTile + part * 32;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const f2 z = make_f2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1]));
-        const f2 g = make_f2(__uint_as_float(y[2 * e]), __uint_as_float(y[2 * e + 1]));
-        const f2 p = ex2_pair(e, fma2(z, c2, *reinterpret_cast<const f2*>(pl + 2 * e)));
-        x[e] = pack2(p, T{});
-        y[e] = pack2(mul2(p, add2(g, *reinterpret_cast<const f2*>(pd + 2 * e))), T{});
+      for (int e = 0; e < 16; e += 2) {
+        const ulonglong2 L = *reinterpret_cast<const ulonglong2*>(pl + 2 * e);
+        p[e] = ex2_pair(e, fma2(make_f2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])), c2, L.x));
+        p[e + 1] = ex2_pair(e + 1, fma2(make_f2(__uint_as_float(x[2 * e + 2]), __uint_as_float(x[2 * e + 3])), c2, L.y));
+        x[e] = pack2(p[e], T{});
+        x[e + 1] = pack2(p[e + 1], T{});
       }
-      tmem_st_32x32b_x16(buf + half * 32, x);
-      tmem_st_32x32b_x16(buf + 64 + half * 32, y);
+      tmem_st_32x32b_x16(s_at, x);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[nbuf]);
+      if (lane == 0) mbar_arrive(&p_full[t % NB]);
+      if (!warp_wait(dp_full, t & 1, abort, limit)) { ok = false; break; }
+      tc_fence_after();
+      tmem_ld_32x32b_x32(row + Cfg::kDPT + part * 32, x);
+      tmem_wait_ld();
+#pragma unroll
+      for (int e = 0; e < 16; e += 2) {
+        const ulonglong2 D = *reinterpret_cast<const ulonglong2*>(pd + 2 * e);
+        const f2 g0 = make_f2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1]));
+        const f2 g1 = make_f2(__uint_as_float(x[2 * e + 2]), __uint_as_float(x[2 * e + 3]));
+        x[e] = pack2(mul2(p[e], add2(g0, D.x)), T{});
+        x[e + 1] = pack2(mul2(p[e + 1], add2(g1, D.y)), T{});
+      }
+      tmem_st_32x32b_x16(row + Cfg::kDPT + part * 32, x);
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(ds_full);
+      qt = qt + 1 == nq ? 0 : qt + 1;
+      st = st + 1 == ST ? 0 : st + 1;
     }
     if (ok && n > 0) ok = warp_wait(all_done, 0, abort, limit);
     if (!ok) {
       if (lane == 0) report_status(a.status, kStatusWindowSoftmaxTimeout);
     } else {
       tc_fence_after();
-      // the first group stores dV, the second dK, each thread half of a row
-      const uint32_t acc = row + (which == 0 ? Cfg::kDV : Cfg::kDK);
-      const float f = which == 0 ? 1.f : a.scale;
-      T* out = (which == 0 ? dv : dk) + (((int64_t)b * a.s + j) * a.hkv + hk) * a.d;
+      // two of a row's threads store dV, two dK, half of the row each
+      const uint32_t acc = row + (part < 2 ? Cfg::kDV : Cfg::kDK);
+      const float f = part < 2 ? 1.f : a.scale;
+      T* out = (part < 2 ? dv : dk) + (((int64_t)b * a.s + j) * a.hkv + hk) * a.d;
       float* slot = nullptr;
       if (parts > 1)
-        slot = work + ((((int64_t)b * a.hkv + hk) * split.slots() + split.slot(tile) + mine) * 2 + which) * kTile * DP +
+        slot = work + ((((int64_t)b * a.hkv + hk) * split.slots() + split.slot(tile) + mine) * 2 + part / 2) * kTile * DP +
                (int64_t)r * DP;
 #pragma unroll
-      for (int j2 = half * (DP / 64); j2 < (half + 1) * (DP / 64); ++j2) {
+      for (int j2 = part % 2 * (DP / 64); j2 < (part % 2 + 1) * (DP / 64); ++j2) {
         uint32_t y[32];
         if (n > 0) {
           tmem_ld_32x32b_x32(acc + j2 * 32, y);
