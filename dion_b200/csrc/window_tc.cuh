@@ -634,19 +634,18 @@ struct DkvCfg {
   static constexpr int kStatBytes = kTile * 4;
   static constexpr int kSmemBytes = 2 * kRowBytes + kStages * (2 * kRowBytes + 2 * kStatBytes) + 1024 + 256;
   static constexpr int kTmemCols = 512;
-  // columns: S^T at 0 with P^T on it, dP^T at 128 with dS^T on it, dV, dK; a second
-  // buffer of S^T behind them where there is room
-  static constexpr int kDPT = 128, kDV = 256, kDK = 256 + DP;
+  // columns: S^T at 0, buffers of dP^T (two where there is room) with P^T and dS^T on
+  // them, dV, dK
   static constexpr int kBufs = DP == 64 ? 2 : 1;
-  static constexpr int kSecond = 384;
+  static constexpr int kDPT = 128, kDV = kDPT + kBufs * 128, kDK = kDV + DP;
 };
 
 // One CTA per (128 keys, key head, sequence, part), steps of 128 queries of one
 // head. With the keys as rows, P^T and dS^T come out of TMEM in the place where
 // dV += P^T dO and dK += dS^T Q want their A operand, so neither passes through
 // shared memory. Four threads share a key row, a quarter of the step's queries
-// each; while they make P^T the tensor cores make dP^T, and dV while they make
-// dS^T.
+// each: a thread reads its 32 columns of dP^T and packs P^T and dS^T into them,
+// so S^T is free for the next step as soon as it has been read.
 template <typename T, int DP>
 __global__ void __launch_bounds__(576, 1)
     window_dkv_tc(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
@@ -664,9 +663,8 @@ __global__ void __launch_bounds__(576, 1)
   float* sL = reinterpret_cast<float*>(sG + ST * Cfg::kRowBytes);
   float* sD = sL + ST * kTile;
   uint64_t* bars = reinterpret_cast<uint64_t*>(sD + ST * kTile);
-  uint64_t *k_full = bars, *q_full = bars + 1, *q_empty = bars + 4, *s_full = bars + 7, *p_full = bars + 9,
-           *dv_done = bars + 11, *dp_full = bars + 13, *ds_full = bars + 14, *dk_done = bars + 15, *all_done = bars + 16,
-           *drain = bars + 17;
+  uint64_t *k_full = bars, *q_full = bars + 1, *q_empty = bars + 4, *s_full = bars + 7, *s_read = bars + 8,
+           *dp_full = bars + 9, *ds_full = bars + 11, *acc_done = bars + 13, *all_done = bars + 15, *drain = bars + 16;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 18);
   volatile int* abort = reinterpret_cast<volatile int*>(bars + 19);
 
@@ -692,14 +690,13 @@ __global__ void __launch_bounds__(576, 1)
       mbar_init(&q_full[i], 1);
       mbar_init(&q_empty[i], 1);
     }
+    mbar_init(s_full, 1);
+    mbar_init(s_read, 16);
     for (int i = 0; i < NB; ++i) {
-      mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 16);
-      mbar_init(&dv_done[i], 1);
+      mbar_init(&dp_full[i], 1);
+      mbar_init(&ds_full[i], 16);
+      mbar_init(&acc_done[i], 1);
     }
-    mbar_init(dp_full, 1);
-    mbar_init(ds_full, 16);
-    mbar_init(dk_done, 1);
     mbar_init(all_done, 1);
     mbar_init(drain, 1);
     *abort = 0;
@@ -753,56 +750,51 @@ __global__ void __launch_bounds__(576, 1)
       constexpr uint32_t kS = make_idesc(kTile, kTile, false, false, AttnType<T>::kFmt);
       constexpr uint32_t kD = make_idesc(kTile, DP, false, true, AttnType<T>::kFmt);
       const uint32_t k_base = smem_u32(sK), v_base = smem_u32(sV);
-      auto s_col = [&](int t) { return tmem + (NB == 2 && (t & 1) ? Cfg::kSecond : 0); };
       bool ok = warp_wait(k_full, 0, abort, limit);
-      auto scores = [&](int t) {  // S^T of step t; the P^T in its buffer has been read
+      auto scores = [&](int t) {  // S^T of step t; the rows have read the one before
         if (!warp_wait(&q_full[t % ST], (t / ST) & 1, abort, limit)) return false;
-        if (t >= NB && !warp_wait(&dv_done[t % NB], (t / NB - 1) & 1, abort, limit)) return false;
+        if (t > 0 && !warp_wait(s_read, (t - 1) & 1, abort, limit)) return false;
         tc_fence_after();
         const uint32_t q_base = smem_u32(sQ + t % ST * Cfg::kRowBytes);
 #pragma unroll
         for (int k = 0; k < DP / 16; ++k) {
           const uint32_t off = (k / 4) * kPanel + (k % 4) * 32;
-          umma_ss(leader, s_col(t), sdesc_low(k_base + off, 16), sdesc_low(q_base + off, 16), kS, k != 0);
+          umma_ss(leader, tmem, sdesc_low(k_base + off, 16), sdesc_low(q_base + off, 16), kS, k != 0);
         }
-        umma_commit_by(leader, &s_full[t % NB]);
+        umma_commit_by(leader, s_full);
         return true;
       };
-      auto grads = [&](int t) {  // dP^T of step t; the dS^T before it has been read
+      auto grads = [&](int t) {  // dP^T of step t; P^T and dS^T in its buffer have been read
         if (!warp_wait(&q_full[t % ST], (t / ST) & 1, abort, limit)) return false;
-        if (t >= 1 && !warp_wait(dk_done, (t - 1) & 1, abort, limit)) return false;
+        if (t >= NB && !warp_wait(&acc_done[t % NB], (t / NB - 1) & 1, abort, limit)) return false;
         tc_fence_after();
         const uint32_t g_base = smem_u32(sG + t % ST * Cfg::kRowBytes);
 #pragma unroll
         for (int k = 0; k < DP / 16; ++k) {
           const uint32_t off = (k / 4) * kPanel + (k % 4) * 32;
-          umma_ss(leader, tmem + Cfg::kDPT, sdesc_low(v_base + off, 16), sdesc_low(g_base + off, 16), kS, k != 0);
+          umma_ss(leader, tmem + Cfg::kDPT + t % NB * 128, sdesc_low(v_base + off, 16), sdesc_low(g_base + off, 16), kS,
+                  k != 0);
         }
-        umma_commit_by(leader, dp_full);
+        umma_commit_by(leader, &dp_full[t % NB]);
         return true;
       };
-      if (ok) ok = scores(0) && grads(0) && (NB == 1 || n == 1 || scores(1));
+      if (ok) ok = scores(0) && grads(0);
       for (int t = 0; t < n && ok; ++t) {
         const int st = t % ST;
         const uint32_t q_base = smem_u32(sQ + st * Cfg::kRowBytes), g_base = smem_u32(sG + st * Cfg::kRowBytes);
-        if (!warp_wait(&p_full[t % NB], (t / NB) & 1, abort, limit)) { ok = false; break; }
+        const uint32_t pds = tmem + Cfg::kDPT + t % NB * 128;
+        if (t + 1 < n && !scores(t + 1)) { ok = false; break; }
+        if (NB == 2 && t + 1 < n && !grads(t + 1)) { ok = false; break; }
+        if (!warp_wait(&ds_full[t % NB], (t / NB) & 1, abort, limit)) { ok = false; break; }
         tc_fence_after();
 #pragma unroll
-        for (int k = 0; k < kTile / 16; ++k)
-          umma_ts(leader, tmem + Cfg::kDV, s_col(t) + part_col(k), sdesc_low(g_base + k * 2048, kPanel), kD, (t | k) != 0);
-        umma_commit_by(leader, &dv_done[t % NB]);
-        // with one buffer the next scores come before dK: the rows wait for them
-        if (NB == 1 && t + 1 < n && !scores(t + 1)) { ok = false; break; }
-        if (!warp_wait(ds_full, t & 1, abort, limit)) { ok = false; break; }
-        tc_fence_after();
-#pragma unroll
-        for (int k = 0; k < kTile / 16; ++k)
-          umma_ts(leader, tmem + Cfg::kDK, tmem + Cfg::kDPT + part_col(k), sdesc_low(q_base + k * 2048, kPanel), kD,
-                  (t | k) != 0);
+        for (int k = 0; k < kTile / 16; ++k) {
+          umma_ts(leader, tmem + Cfg::kDV, pds + part_col(k), sdesc_low(g_base + k * 2048, kPanel), kD, (t | k) != 0);
+          umma_ts(leader, tmem + Cfg::kDK, pds + part_col(k) + 16, sdesc_low(q_base + k * 2048, kPanel), kD, (t | k) != 0);
+        }
         umma_commit_by(leader, &q_empty[st]);
-        umma_commit_by(leader, dk_done);
-        if (NB == 2 && t + 2 < n && !scores(t + 2)) { ok = false; break; }
-        if (t + 1 < n && !grads(t + 1)) { ok = false; break; }
+        umma_commit_by(leader, &acc_done[t % NB]);
+        if (NB == 1 && t + 1 < n && !grads(t + 1)) { ok = false; break; }
       }
       if (ok) {
         umma_commit_by(leader, all_done);
@@ -823,15 +815,18 @@ __global__ void __launch_bounds__(576, 1)
     int qt = lo % nq, st = 0;  // this step's query tile (from q_first) and stage
     for (int t = 0; t < n; ++t) {
       const int q0 = (q_first + qt) * kTile;
-      const uint32_t s_at = row + (NB == 2 && (t & 1) ? Cfg::kSecond : 0) + part * 32;
+      const uint32_t pds = row + Cfg::kDPT + t % NB * 128 + part * 32;
       // (the stage's copies as well: the rows read lse and delta from it)
       if (!warp_wait(&q_full[st], (t / ST) & 1, abort, limit)) { ok = false; break; }
-      if (!warp_wait(&s_full[t % NB], (t / NB) & 1, abort, limit)) { ok = false; break; }
+      if (!warp_wait(s_full, t & 1, abort, limit)) { ok = false; break; }
       tc_fence_after();
-      uint32_t x[32];
+      uint32_t x[32], y[32];
       f2 p[16];
-      tmem_ld_32x32b_x32(s_at, x);
+      tmem_ld_32x32b_x32(row + part * 32, x);
       tmem_wait_ld();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(s_read);
       // queries q0 + e that see key j: e in [j - q0, j + window - q0), without an end for first tokens
       if (!(q0 >= k0 + kTile - 1 && (q0 + kTile - 1 - k0 < a.window || k0 + kTile <= a.sinks))) {
         const int e0 = j - q0 - part * 32;
@@ -846,31 +841,26 @@ __global__ void __launch_bounds__(576, 1)
         const ulonglong2 L = *reinterpret_cast<const ulonglong2*>(pl + 2 * e);
         p[e] = ex2_pair(e, fma2(make_f2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])), c2, L.x));
         p[e + 1] = ex2_pair(e + 1, fma2(make_f2(__uint_as_float(x[2 * e + 2]), __uint_as_float(x[2 * e + 3])), c2, L.y));
-        x[e] = pack2(p[e], T{});
-        x[e + 1] = pack2(p[e + 1], T{});
       }
-      tmem_st_32x32b_x16(s_at, x);
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[t % NB]);
-      if (!warp_wait(dp_full, t & 1, abort, limit)) { ok = false; break; }
+      if (!warp_wait(&dp_full[t % NB], (t / NB) & 1, abort, limit)) { ok = false; break; }
       tc_fence_after();
-      tmem_ld_32x32b_x32(row + Cfg::kDPT + part * 32, x);
+      tmem_ld_32x32b_x32(pds, x);
       tmem_wait_ld();
 #pragma unroll
       for (int e = 0; e < 16; e += 2) {
         const ulonglong2 D = *reinterpret_cast<const ulonglong2*>(pd + 2 * e);
         const f2 g0 = make_f2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1]));
         const f2 g1 = make_f2(__uint_as_float(x[2 * e + 2]), __uint_as_float(x[2 * e + 3]));
-        x[e] = pack2(mul2(p[e], add2(g0, D.x)), T{});
-        x[e + 1] = pack2(mul2(p[e + 1], add2(g1, D.y)), T{});
+        y[e] = pack2(p[e], T{});
+        y[e + 1] = pack2(p[e + 1], T{});
+        y[16 + e] = pack2(mul2(p[e], add2(g0, D.x)), T{});
+        y[16 + e + 1] = pack2(mul2(p[e + 1], add2(g1, D.y)), T{});
       }
-      tmem_st_32x32b_x16(row + Cfg::kDPT + part * 32, x);
+      tmem_st_32x32b_x32(pds, y);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(ds_full);
+      if (lane == 0) mbar_arrive(&ds_full[t % NB]);
       qt = qt + 1 == nq ? 0 : qt + 1;
       st = st + 1 == ST ? 0 : st + 1;
     }

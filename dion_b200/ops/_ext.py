@@ -17,6 +17,9 @@ _CODES = {
     0x102: "GEMM MMA issuer wait timed out",
     0x103: "GEMM epilogue wait timed out",
     0x201: "peer wait timed out in a communication kernel",
+    0x401: "window attention TMA producer wait timed out",
+    0x402: "window attention MMA issuer wait timed out",
+    0x403: "window attention row wait timed out",
     0x301: "Cholesky factor not positive definite",
 }
 
