@@ -165,16 +165,18 @@ __device__ __forceinline__ float key_float(uint32_t key) {  // the float that or
   return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
 
-// Largest threshold that at least k of the n keys reach, bit by bit (one warp);
-// stops early where exactly k do. key(i) may be called for i < n only.
-template <typename F>
-__device__ __forceinline__ uint32_t kth_key(int n, int k, F key) {
+// Largest threshold that at least k of the keys reach (R per lane of one warp, or
+// per thread of the block), bit by bit; stops early where exactly k do.
+template <int R, bool BLOCK>
+__device__ __forceinline__ uint32_t kth_key(const uint32_t (&key)[R], int k) {
   uint32_t thr = 0;
+#pragma unroll 1
   for (int bit = 31; bit >= 0; --bit) {
     const uint32_t t = thr | (1u << bit);
     int cnt = 0;
-    for (int i = threadIdx.x % 32; i < n; i += 32) cnt += key(i) >= t;
-    cnt = __reduce_add_sync(0xffffffffu, cnt);
+#pragma unroll
+    for (int i = 0; i < R; ++i) cnt += BLOCK ? __syncthreads_count(key[i] >= t) : key[i] >= t;
+    if (!BLOCK) cnt = __reduce_add_sync(0xffffffffu, cnt);
     if (cnt >= k) thr = t;
     if (cnt == k) break;
   }
@@ -192,7 +194,7 @@ __device__ __forceinline__ uint32_t kth_key(int n, int k, F key) {
 // values), and rows with a NaN or +inf, take the exact threshold over the whole
 // row bit by bit and keep the lowest indices of the equal ones.
 template <typename T, int G>
-__global__ void __launch_bounds__(kThreads) top_logits_kernel(const T* __restrict__ logits, int64_t ld, int V, int k,
+__global__ void __launch_bounds__(kThreads, 3) top_logits_kernel(const T* __restrict__ logits, int64_t ld, int V, int k,
                                                               bool vec, int ns, float c, float* __restrict__ values,
                                                               int64_t* __restrict__ indices,
                                                               float* __restrict__ lse) {
@@ -237,8 +239,19 @@ __global__ void __launch_bounds__(kThreads) top_logits_kernel(const T* __restric
   for (int i = 0; i < G; ++i) s_max[tid * G + i] = best[i] == -INFINITY ? 0u : order_key(best[i]);
   if (tid == 0) s_n = 0;
   __syncthreads();
-  if (tid < 32) {
-    const uint32_t t = kth_key(kThreads * G, k, [&](int i) { return s_max[i]; });
+  if (G == 1) {
+    if (tid < 32) {
+      uint32_t keys[kThreads / 32];
+#pragma unroll
+      for (int i = 0; i < kThreads / 32; ++i) keys[i] = s_max[i * 32 + tid];
+      const uint32_t t = kth_key<kThreads / 32, false>(keys, k);
+      if (tid == 0) s_thr = t;
+    }
+  } else {
+    uint32_t keys[G];
+#pragma unroll
+    for (int i = 0; i < G; ++i) keys[i] = s_max[i * kThreads + tid];
+    const uint32_t t = kth_key<G, true>(keys, k);
     if (tid == 0) s_thr = t;
   }
   __syncthreads();
@@ -339,8 +352,21 @@ __global__ void __launch_bounds__(kThreads) top_logits_kernel(const T* __restric
     n = min(have, k);
   } else if (n > 2 * k && n > 128) {
     // a second bound, now over the candidates
-    if (tid < 32) {
-      const uint32_t t = kth_key(n, k, [&](int i) { return (uint32_t)(s_cand[0][i] >> 32); });
+    if (n <= kThreads) {
+      if (tid < 32) {
+        uint32_t keys[kThreads / 32];
+#pragma unroll
+        for (int i = 0; i < kThreads / 32; ++i)
+          keys[i] = i * 32 + tid < n ? (uint32_t)(s_cand[0][i * 32 + tid] >> 32) : 0u;
+        const uint32_t t = kth_key<kThreads / 32, false>(keys, k);
+        if (tid == 0) s_thr = t, s_n = 0;
+      }
+    } else {
+      uint32_t keys[kMaxCand / kThreads];
+#pragma unroll
+      for (int i = 0; i < kMaxCand / kThreads; ++i)
+        keys[i] = i * kThreads + tid < n ? (uint32_t)(s_cand[0][i * kThreads + tid] >> 32) : 0u;
+      const uint32_t t = kth_key<kMaxCand / kThreads, true>(keys, k);
       if (tid == 0) s_thr = t, s_n = 0;
     }
     __syncthreads();

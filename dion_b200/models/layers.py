@@ -203,7 +203,8 @@ class _LinearDistillation(torch.autograd.Function):
         T, V = h.shape[0], W.shape[0]
         total = torch.zeros((), device=h.device, dtype=torch.float32)
         grad_h = torch.empty(h.shape, device=h.device, dtype=torch.float32) if need_grad else None
-        grad_W = torch.zeros(W.shape, device=W.device, dtype=torch.float32) if need_grad else None
+        make = torch.empty if T else torch.zeros
+        grad_W = make(W.shape, device=W.device, dtype=torch.float32) if need_grad else None
         for s in range(0, T, chunk):
             e = min(T, s + chunk)
             hc = h[s:e]
@@ -213,10 +214,13 @@ class _LinearDistillation(torch.autograd.Function):
             total += loss_c
             if need_grad:
                 grad_h[s:e] = _mm_fp32(g, W)
+                # grad_W (fp32) = or += g^T @ hc
                 if h.is_cuda and h.dtype == torch.bfloat16:
-                    ops.matmul(g.t(), hc, out=grad_W, C=grad_W, beta=1.0)
-                else:
+                    ops.matmul(g.t(), hc, out=grad_W, C=grad_W if s else None, beta=1.0 if s else 0.0)
+                elif s:
                     grad_W += g.t().float() @ hc.float()
+                else:
+                    grad_W = g.t().float() @ hc.float()
         n = max(T, 1) if labels is None else ((labels >= 0) & (labels < V)).sum().clamp_min(1).float()
         ctx.n = n
         ctx.save_for_backward(grad_h, grad_W)
@@ -227,7 +231,8 @@ class _LinearDistillation(torch.autograd.Function):
     def backward(ctx, go):
         grad_h, grad_W = ctx.saved_tensors
         f = go / ctx.n
-        return ((grad_h * f).to(ctx.dtypes[0]), (grad_W * f).to(ctx.dtypes[1])) + (None,) * 8
+        out = [torch.empty(g.shape, device=g.device, dtype=t) for g, t in zip((grad_h, grad_W), ctx.dtypes)]
+        return (torch.mul(grad_h, f, out=out[0]), torch.mul(grad_W, f, out=out[1])) + (None,) * 8
 
 
 def linear_distillation(h: torch.Tensor, W: torch.Tensor, labels: Optional[torch.Tensor], top_values: torch.Tensor,
