@@ -59,12 +59,15 @@ void top_logits(const at::Tensor& logits, at::Tensor& values, at::Tensor& indice
 void distill_fwd_bwd(const at::Tensor& logits, const c10::optional<at::Tensor>& labels, const at::Tensor& top_values,
                      const at::Tensor& top_indices, const c10::optional<at::Tensor>& top_lse,
                      const c10::optional<at::Tensor>& grad, at::Tensor& loss, double tau, double alpha, double grad_scale);
-std::tuple<at::Tensor, at::Tensor> window_attention_fwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
-                                                        int64_t window, int64_t sinks);
+void scale_cast(const at::Tensor& x, const at::Tensor& f, at::Tensor& out);
+std::tuple<at::Tensor, at::Tensor, at::Tensor> window_attention_fwd(const at::Tensor& q, const at::Tensor& k,
+                                                                    const at::Tensor& v, int64_t window,
+                                                                    int64_t sinks, bool backward);
 std::tuple<at::Tensor, at::Tensor, at::Tensor> window_attention_bwd(const at::Tensor& go, const at::Tensor& q,
                                                                     const at::Tensor& k, const at::Tensor& v,
-                                                                    const at::Tensor& o, const at::Tensor& lse,
-                                                                    int64_t window, int64_t sinks);
+                                                                    const at::Tensor& o, const at::Tensor& o_low,
+                                                                    const at::Tensor& lse, int64_t window,
+                                                                    int64_t sinks);
 void dion_momentum_add(const std::vector<at::Tensor>& M, const std::vector<at::Tensor>& G, at::Tensor& nz);
 void dion_fixup(at::Tensor& P, at::Tensor& R, const at::Tensor& Q0, const at::Tensor& nz);
 void col_sumsq(const at::Tensor& R, at::Tensor& out);
@@ -128,6 +131,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("cross_entropy_fwd_bwd", &bdion::cross_entropy_fwd_bwd);
   m.def("top_logits", &bdion::top_logits, "k largest logits of each row, their indices and the row's log-sum-exp");
   m.def("distill_fwd_bwd", &bdion::distill_fwd_bwd, "distillation loss from a teacher's top logits and its gradient");
+  m.def("scale_cast", &bdion::scale_cast, "fp32 tensor times a device scalar, rounded once to the output's type");
   m.def("window_attention_fwd", &bdion::window_attention_fwd, "sliding-window attention with visible first tokens");
   m.def("window_attention_bwd", &bdion::window_attention_bwd);
   m.def("dion_momentum_add", &bdion::dion_momentum_add);

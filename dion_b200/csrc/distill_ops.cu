@@ -194,7 +194,7 @@ __device__ __forceinline__ uint32_t kth_key(const uint32_t (&key)[R], int k) {
 // values), and rows with a NaN or +inf, take the exact threshold over the whole
 // row bit by bit and keep the lowest indices of the equal ones.
 template <typename T, int G>
-__global__ void __launch_bounds__(kThreads, 3) top_logits_kernel(const T* __restrict__ logits, int64_t ld, int V, int k,
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 3 : 2) top_logits_kernel(const T* __restrict__ logits, int64_t ld, int V, int k,
                                                               bool vec, int ns, float c, float* __restrict__ values,
                                                               int64_t* __restrict__ indices,
                                                               float* __restrict__ lse) {
@@ -702,6 +702,23 @@ __global__ void __launch_bounds__(kThreads, 2)
   }
 }
 
+// out = x * f[0], rounded once
+template <typename TO>
+__global__ void __launch_bounds__(256) scale_cast_kernel(const float* __restrict__ x, const float* __restrict__ f,
+                                                         TO* __restrict__ out, int64_t n) {
+  const float s = *f;
+  const int64_t step = (int64_t)gridDim.x * 256;
+  int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  for (; i < n / 8; i += step) {
+    float v[8];
+    load8(x + i * 8, v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] *= s;
+    store8(out + i * 8, v);
+  }
+  if (blockIdx.x == 0 && (int)threadIdx.x < n % 8) put(out + n / 8 * 8 + threadIdx.x, x[n / 8 * 8 + threadIdx.x] * s);
+}
+
 bool aligned8(const at::Tensor& t) {
   return reinterpret_cast<uintptr_t>(t.data_ptr()) % (8 * t.element_size()) == 0;
 }
@@ -838,6 +855,28 @@ void distill_fwd_bwd(const at::Tensor& logits, const c10::optional<at::Tensor>& 
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   note_launch();
   at::sum_out(loss, rows, 0);
+}
+
+// out (bf16, fp16 or fp32) = x (fp32) * f (one fp32 value on the device)
+void scale_cast(const at::Tensor& x, const at::Tensor& f, at::Tensor& out) {
+  TORCH_CHECK(x.is_cuda() && x.scalar_type() == at::kFloat && x.is_contiguous() && aligned8(x) && f.numel() == 1 &&
+                  f.scalar_type() == at::kFloat && f.device() == x.device(),
+              "dion_b200 scale_cast: contiguous fp32 x and one fp32 factor on one CUDA device");
+  TORCH_CHECK(out.scalar_type() == at::kBFloat16 || out.scalar_type() == at::kHalf || out.scalar_type() == at::kFloat,
+              "dion_b200 scale_cast: bf16, fp16 or fp32 out");
+  check_out(out, x, out.scalar_type(), x.sizes(), "scale_cast out");
+  TORCH_CHECK(aligned8(out), "dion_b200 scale_cast: out aligned to 8 elements");
+  if (x.numel() == 0) return;
+  c10::cuda::CUDAGuard guard(x.device());
+  const int64_t blocks = (x.numel() / 8 + 255) / 256;
+  by_type(out.scalar_type(), [&](auto tag) {
+    using E = decltype(tag);
+    scale_cast_kernel<E><<<(unsigned)std::max<int64_t>(1, std::min<int64_t>(blocks, 148 * 16)), 256, 0,
+                           at::cuda::getCurrentCUDAStream()>>>(x.data_ptr<float>(), f.data_ptr<float>(),
+                                                               static_cast<E*>(out.data_ptr()), x.numel());
+  });
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  note_launch();
 }
 
 }  // namespace bdion

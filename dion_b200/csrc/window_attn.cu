@@ -134,36 +134,42 @@ KeySplit split_keys(const WinArgs& a) {
 
 }  // namespace
 
-// o [b, s, hq, d], and minus the log2 of each row's sum of exponentials [b, hq,
+// o [b, s, hq, d]; with `backward` what its rounding left out, as another tensor of
+// o's type (else an empty one); and minus the log2 of each row's sum of exponentials [b, hq,
 // s rounded up to 128] (-inf behind the last position) for the backward pass
-std::tuple<at::Tensor, at::Tensor> window_attention_fwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
-                                                        int64_t window, int64_t sinks) {
+std::tuple<at::Tensor, at::Tensor, at::Tensor> window_attention_fwd(const at::Tensor& q, const at::Tensor& k,
+                                                                    const at::Tensor& v, int64_t window,
+                                                                    int64_t sinks, bool backward) {
   const WinArgs a = make_args(q, k, v, window, sinks);
   c10::cuda::CUDAGuard guard(q.device());
   bind_context(q);
   auto o = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
+  auto o_low = backward ? at::empty_like(o) : at::empty({0}, o.options());
   auto lse = at::empty({a.b, a.hq, a.s_pad}, q.options().dtype(at::kFloat));
-  if (o.numel() == 0) return {o, lse};
+  if (o.numel() == 0) return {o, o_low, lse};
   const CUtensorMap mq = head_map(q, kTile, "q"), mk = head_map(k, kHalfTile, "k"), mv = head_map(v, kHalfTile, "v");
   by_case(q.scalar_type(), a.d, [&](auto tag, auto dp) {
     using E = decltype(tag);
     constexpr int DP = decltype(dp)::value;
     launch(window_fwd_tc<E, DP>, (int64_t)a.b * a.hq * (a.s_pad / kTile), 192, FwdCfg<E, DP>::kSmemBytes,
-           at::cuda::getCurrentCUDAStream(), mq, mk, mv, (E*)o.data_ptr(), lse.data_ptr<float>(), a);
+           at::cuda::getCurrentCUDAStream(), mq, mk, mv, (E*)o.data_ptr(),
+           backward ? (E*)o_low.data_ptr() : nullptr, lse.data_ptr<float>(), a);
   });
-  return {o, lse};
+  return {o, o_low, lse};
 }
 
 std::tuple<at::Tensor, at::Tensor, at::Tensor> window_attention_bwd(const at::Tensor& go, const at::Tensor& q,
                                                                     const at::Tensor& k, const at::Tensor& v,
-                                                                    const at::Tensor& o, const at::Tensor& lse,
-                                                                    int64_t window, int64_t sinks) {
+                                                                    const at::Tensor& o, const at::Tensor& o_low,
+                                                                    const at::Tensor& lse, int64_t window,
+                                                                    int64_t sinks) {
   const WinArgs a = make_args(q, k, v, window, sinks);
   check_heads(go, q, "the output's gradient");
   TORCH_CHECK(go.sizes() == q.sizes() && o.sizes() == q.sizes() && o.is_contiguous() && o.device() == q.device() &&
-                  o.scalar_type() == q.scalar_type() && lse.is_contiguous() && lse.device() == q.device() &&
+                  o.scalar_type() == q.scalar_type() && o_low.sizes() == q.sizes() && o_low.is_contiguous() &&
+                  o_low.device() == q.device() && o_low.scalar_type() == q.scalar_type() && lse.is_contiguous() && lse.device() == q.device() &&
                   lse.scalar_type() == at::kFloat && lse.numel() == (int64_t)a.b * a.hq * a.s_pad,
-              "dion_b200 window_attention: o and lse as the forward pass gave them");
+              "dion_b200 window_attention: o, its remainder and lse as the forward pass gave them");
   c10::cuda::CUDAGuard guard(q.device());
   bind_context(q);
   auto st = at::cuda::getCurrentCUDAStream();
@@ -180,7 +186,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> window_attention_bwd(const at::Te
     using E = decltype(tag);
     constexpr int DP = decltype(dp)::value;
     launch(window_dq_tc<E, DP>, (int64_t)a.b * a.hq * (a.s_pad / kTile), 576, DqCfg<E, DP>::kSmemBytes, st, mq, mk, mv,
-           mg, (const E*)o.data_ptr(), (const E*)go.data_ptr(), go.stride(0), go.stride(1), go.stride(2),
+           mg, (const E*)o.data_ptr(), (const E*)o_low.data_ptr(), (const E*)go.data_ptr(), go.stride(0), go.stride(1), go.stride(2),
            lse.data_ptr<float>(), delta.data_ptr<float>(), (E*)dq.data_ptr(), a);
     at::Tensor work;
     const int64_t slots = (int64_t)a.b * a.hkv * split.slots();
@@ -203,6 +209,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> window_attention_bwd(const at::Te
 // A dispatcher op, so that selective activation checkpointing can name its
 // output among those that it keeps.
 TORCH_LIBRARY(dion_b200, m) {
-  m.def("window_attention_fwd(Tensor q, Tensor k, Tensor v, int window, int sinks) -> (Tensor, Tensor)");
+  m.def("window_attention_fwd(Tensor q, Tensor k, Tensor v, int window, int sinks, bool backward) -> (Tensor, "
+        "Tensor, Tensor)");
 }
 TORCH_LIBRARY_IMPL(dion_b200, CUDA, m) { m.impl("window_attention_fwd", &bdion::window_attention_fwd); }

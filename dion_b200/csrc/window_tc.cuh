@@ -90,7 +90,8 @@ struct FwdCfg {
 template <typename T, int DP>
 __global__ void __launch_bounds__(192, 2)
     window_fwd_tc(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
-                  const __grid_constant__ CUtensorMap tv, T* __restrict__ o, float* __restrict__ neg_lse, const WinArgs a) {
+                  const __grid_constant__ CUtensorMap tv, T* __restrict__ o, T* __restrict__ o_low,
+                  float* __restrict__ neg_lse, const WinArgs a) {
   using Cfg = FwdCfg<T, DP>;
   constexpr int ST = Cfg::kStages;
   extern __shared__ uint8_t smem_raw[];
@@ -295,7 +296,7 @@ __global__ void __launch_bounds__(192, 2)
       const bool real = i < a.s;
       neg_lse[((int64_t)b * a.hq + h) * a.s_pad + i] = real ? -(m * c + log2f(l)) : -INFINITY;
       const float inv = 1.f / l;
-      T* orow = o + (((int64_t)b * a.s + i) * a.hq + h) * a.d;
+      const int64_t orow = (((int64_t)b * a.s + i) * a.hq + h) * a.d;
 #pragma unroll
       for (int j = 0; j < DP / 32; ++j) {
         uint32_t y[32];
@@ -304,12 +305,20 @@ __global__ void __launch_bounds__(192, 2)
 #pragma unroll
         for (int e = 0; e < 32; e += 8) {
           if (real && j * 32 + e < a.d) {
-            uint4 u;
-            uint32_t* w = reinterpret_cast<uint32_t*>(&u);
+            // o, and what its rounding left out: the backward pass takes delta = do . o from
+            // both. Where one key has nearly all of a row, dP - delta is far smaller than
+            // its terms, and the rounding of o alone made it off by as much as itself.
+            uint4 u, v;
+            uint32_t *hi = reinterpret_cast<uint32_t*>(&u), *lo = reinterpret_cast<uint32_t*>(&v);
 #pragma unroll
-            for (int n = 0; n < 4; ++n)
-              w[n] = pack2(__uint_as_float(y[e + 2 * n]) * inv, __uint_as_float(y[e + 2 * n + 1]) * inv, T{});
-            *reinterpret_cast<uint4*>(orow + j * 32 + e) = u;
+            for (int n = 0; n < 4; ++n) {
+              const float x0 = __uint_as_float(y[e + 2 * n]) * inv, x1 = __uint_as_float(y[e + 2 * n + 1]) * inv;
+              hi[n] = pack2(x0, x1, T{});
+              const T* r = reinterpret_cast<const T*>(&hi[n]);
+              lo[n] = pack2(x0 - (float)r[0], x1 - (float)r[1], T{});
+            }
+            *reinterpret_cast<uint4*>(o + orow + j * 32 + e) = u;
+            if (o_low != nullptr) *reinterpret_cast<uint4*>(o_low + orow + j * 32 + e) = v;
           }
         }
       }
@@ -352,7 +361,7 @@ template <typename T, int DP>
 __global__ void __launch_bounds__(576, 1)
     window_dq_tc(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                  const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap tg,
-                 const T* __restrict__ o, const T* __restrict__ go, int64_t go_b, int64_t go_s, int64_t go_h,
+                 const T* __restrict__ o, const T* __restrict__ o_low, const T* __restrict__ go, int64_t go_b, int64_t go_s, int64_t go_h,
                  const float* __restrict__ neg_lse, float* __restrict__ neg_delta, T* __restrict__ dq,
                  const WinArgs a) {
   using Cfg = DqCfg<T, DP>;
@@ -515,11 +524,13 @@ __global__ void __launch_bounds__(576, 1)
         const int rr = q0 + (warp - 2) * 8 + n * kRows + lane / kLanes;
         v[n] = 0.f;
         if (rr < a.s && col < a.d) {
-          const uint4 ou = *reinterpret_cast<const uint4*>(o + (((int64_t)b * a.s + rr) * a.hq + h) * a.d + col);
+          const int64_t at_o = (((int64_t)b * a.s + rr) * a.hq + h) * a.d + col;
+          const uint4 ou = *reinterpret_cast<const uint4*>(o + at_o), lu = *reinterpret_cast<const uint4*>(o_low + at_o);
           const uint4 gu = *reinterpret_cast<const uint4*>(go + b * go_b + rr * go_s + h * go_h + col);
-          const T *op = reinterpret_cast<const T*>(&ou), *gp = reinterpret_cast<const T*>(&gu);
+          const T *op = reinterpret_cast<const T*>(&ou), *lp = reinterpret_cast<const T*>(&lu),
+                  *gp = reinterpret_cast<const T*>(&gu);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[n] += (float)op[e] * (float)gp[e];
+          for (int e = 0; e < 8; ++e) v[n] += ((float)op[e] + (float)lp[e]) * (float)gp[e];
         }
       }
 #pragma unroll

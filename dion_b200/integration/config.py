@@ -43,6 +43,10 @@ class ModelConfig:
     flavor: str = "160M"
     overrides: Dict[str, Any] = field(default_factory=dict)
     init: str = "normal"
+    # sliding-window attention: every position sees the last attn_window ones and the
+    # first attn_sinks ones (None: all earlier positions)
+    attn_window: Optional[int] = None
+    attn_sinks: int = 0
 
 
 @dataclass

@@ -14,6 +14,7 @@ from typing import Optional, Tuple
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
 from .. import ops
 from ..ops import fused as _fused
@@ -228,11 +229,11 @@ class _LinearDistillation(torch.autograd.Function):
         return total / n
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, go):
         grad_h, grad_W = ctx.saved_tensors
         f = go / ctx.n
-        out = [torch.empty(g.shape, device=g.device, dtype=t) for g, t in zip((grad_h, grad_W), ctx.dtypes)]
-        return (torch.mul(grad_h, f, out=out[0]), torch.mul(grad_W, f, out=out[1])) + (None,) * 8
+        return (_fused.scale_cast(grad_h, f, ctx.dtypes[0]), _fused.scale_cast(grad_W, f, ctx.dtypes[1])) + (None,) * 8
 
 
 def linear_distillation(h: torch.Tensor, W: torch.Tensor, labels: Optional[torch.Tensor], top_values: torch.Tensor,

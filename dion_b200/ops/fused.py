@@ -12,6 +12,7 @@ from typing import NamedTuple, Optional, Tuple
 
 import torch
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
 from ._ext import ext, has_ext
 
@@ -148,15 +149,16 @@ class _WindowAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, window, sinks):
         q, k, v = _tile_rows(q), _tile_rows(k), _tile_rows(v)
-        o, lse = torch.ops.dion_b200.window_attention_fwd(q, k, v, window, sinks)
-        ctx.save_for_backward(q, k, v, o, lse)
+        o, o_low, lse = torch.ops.dion_b200.window_attention_fwd(q, k, v, window, sinks, True)
+        ctx.save_for_backward(q, k, v, o, o_low, lse)
         ctx.window, ctx.sinks = window, sinks
         return o
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, go):
-        q, k, v, o, lse = ctx.saved_tensors
-        dq, dk, dv = ext().window_attention_bwd(_tile_rows(go), q, k, v, o, lse, ctx.window, ctx.sinks)
+        q, k, v, o, o_low, lse = ctx.saved_tensors
+        dq, dk, dv = ext().window_attention_bwd(_tile_rows(go), q, k, v, o, o_low, lse, ctx.window, ctx.sinks)
         return dq, dk, dv, None, None
 
 
@@ -165,8 +167,12 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     ``i - j < window`` or ``j < sinks``. q: [b, s, hq, d], k/v: [b, s, hkv, d]
     (query head h reads key head h // (hq / hkv)) -> [b, s, hq, d]; scores are
     scaled by 1 / sqrt(d). Inputs are finite: a non-finite key or value also
-    reaches rows up to a tile of 128 beyond those that see it."""
+    reaches rows up to a tile of 128 beyond those that see it. The backward pass
+    holds P (dP - delta) in the inputs' type, so in fp16 that is bounded by 65504."""
     _check_window(q, k, v, window, sinks)
+    if not (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)):
+        return torch.ops.dion_b200.window_attention_fwd(_tile_rows(q), _tile_rows(k), _tile_rows(v), int(window),
+                                                        int(sinks), False)[0]
     return _WindowAttention.apply(q, k, v, int(window), int(sinks))
 
 
@@ -260,8 +266,8 @@ def distillation_fwd_bwd(logits: torch.Tensor, labels: Optional[torch.Tensor], t
     (fp32 scalar), and grad_scale times its gradient with respect to the logits
     (in their dtype, or ``grad_dtype`` for fp32 logits; None without ``need_grad``).
 
-    logits: [T, V]; top_values / top_indices: [T, k], k <= 1024, the teacher's
-    logits and their columns (int32 or int64; a column outside [0, V) marks an
+    logits: [T, V] (V up to 2^20 on CUDA); top_values / top_indices: [T, k], k <= 1024,
+    the teacher's logits (constants: no gradient flows to them) and their columns (int32 or int64; a column outside [0, V) marks an
     unused entry, a column may come twice). ``top_lse`` [T] is the teacher's
     log-sum-exp at the temperature: the teacher's probability outside its
     entries then counts as one outcome more, held against the student's
@@ -300,6 +306,15 @@ def distillation_fwd_bwd(logits: torch.Tensor, labels: Optional[torch.Tensor], t
     loss, grad = _distillation_ref(logits.float(), labels, top_values.float(), top_indices.long(),
                                    None if top_lse is None else top_lse.float(), temperature, alpha, need_grad)
     return loss, (grad * grad_scale).to(gdt) if need_grad else None
+
+
+def scale_cast(x: torch.Tensor, f: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """fp32 x times the scalar tensor f, rounded once to ``dtype``."""
+    if _rows_enabled(x) and x.dtype == torch.float32 and x.is_contiguous() and x.data_ptr() % 32 == 0:
+        out = torch.empty(x.shape, device=x.device, dtype=dtype)
+        ext().scale_cast(x, f.to(x.device, torch.float32), out)
+        return out
+    return (x * f).to(dtype)
 
 
 def _distillation_ref(z, labels, top_values, top_indices, top_lse, tau, alpha, need_grad=True):

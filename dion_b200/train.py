@@ -36,9 +36,14 @@ PEAK_FLOPS = {"bfloat16": 2.25e15}
 
 def trainer_config_from_job(job: JobConfig) -> TrainerConfig:
     par = job.parallelism
+    overrides = dict(job.model.overrides)
+    if job.model.attn_window is not None:
+        overrides.update(attn_window=job.model.attn_window, attn_sinks=job.model.attn_sinks)
+    elif job.model.attn_sinks:
+        raise ValueError("--model.attn_sinks needs --model.attn_window")
     return TrainerConfig(
         model=job.model.flavor,
-        model_overrides=dict(job.model.overrides),
+        model_overrides=overrides,
         seq_len=job.training.seq_len,
         local_batch_size=job.training.local_batch_size,
         steps=job.training.steps,

@@ -239,6 +239,15 @@ def test_linear_distillation(dtype):
         assert_within(got, exact, err + 2 * half * exact.abs() + small * 3, "linear")
 
 
+@pytest.mark.parametrize("n", [1, 7, 8, 9, 4099, 1 << 20])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_scale_cast(n, dtype):
+    x = torch.randn(n, device=DEV)
+    f = torch.tensor(0.37, device=DEV)
+    assert torch.equal(fused.scale_cast(x, f, dtype), (x * f).to(dtype))
+    assert torch.equal(fused.scale_cast(x[1:], f, dtype), (x[1:] * f).to(dtype))
+
+
 def test_linear_top_logits():
     g = torch.Generator(device=DEV).manual_seed(0)
     h = torch.randn(2, 150, 256, device=DEV, generator=g).bfloat16()

@@ -92,3 +92,19 @@ def test_activation_checkpointing_gives_the_same_gradients():
     for g in grads[1:]:
         for a, b in zip(grads[0], g):
             torch.testing.assert_close(a, b)
+
+
+def test_command_line_window():
+    """--model.attn_window and --model.attn_sinks reach the model's configuration."""
+    from dion_b200.integration.config import apply_overrides
+    from dion_b200.integration.config_registry import get_config
+    from dion_b200.train import trainer_config_from_job
+
+    job = get_config("llama3_160m_dion")
+    assert trainer_config_from_job(job).model_overrides == job.model.overrides
+    apply_overrides(job, ["--model.attn_window", "9", "--model.attn_sinks", "2"])
+    cfg = trainer_config_from_job(job)
+    assert cfg.model_overrides["attn_window"] == 9 and cfg.model_overrides["attn_sinks"] == 2
+    job.model.attn_window = None
+    with pytest.raises(ValueError, match="attn_window"):
+        trainer_config_from_job(job)

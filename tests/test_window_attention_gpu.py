@@ -75,6 +75,23 @@ def test_unseen_keys_with_far_larger_scores(d):
     check(q, k, v, do, 40, 1)
 
 
+@pytest.mark.parametrize("window,sinks", [(1, 1), (2, 0), (2, 1), (5, 2)])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_few_keys_with_one_that_has_nearly_all(window, sinks, d, dtype):
+    """dP - delta cancels there. Two roundings lie between the inputs and each gradient (of P or dS, and of the
+    result), each at most half / sqrt(3) of the value in the mean square; a quarter more for all that is fp32."""
+    q, k, v, do = make(2, 500, 4, 2, d, dtype, scale=1.3)
+    with torch.no_grad():
+        k[:, :sinks] *= 2
+    o = L.window_attention(q, k, v, window, sinks)
+    want = window_oracle(q, k, v, window, sinks, do)
+    for got, name in zip(torch.autograd.grad(o, (q, k, v), do), ("dq", "dk", "dv")):
+        exact = want[name][0]
+        off = ((got.double() - exact).norm() / exact.norm()).item()
+        assert off <= 1.25 * (2 / 3) ** 0.5 * torch.finfo(dtype).eps / 2, (name, off)
+
+
 def test_equal_and_zero_inputs():
     q, k, v, do = make(1, 300, 2, 2, 64)
     with torch.no_grad():
@@ -202,9 +219,9 @@ def test_refusals():
     with pytest.raises(RuntimeError, match="multiple of 8"):
         fused.window_attention(q[..., :20], k[..., :20], v[..., :20], 4)
     with pytest.raises(RuntimeError, match="bf16 or fp16"):
-        ext.window_attention_fwd(q.float(), k.float(), v.float(), 4, 0)
+        ext.window_attention_fwd(q.float(), k.float(), v.float(), 4, 0, False)
     with pytest.raises(RuntimeError, match="window >= 1"):
-        ext.window_attention_fwd(q.detach(), k.detach(), v.detach(), 0, 0)
+        ext.window_attention_fwd(q.detach(), k.detach(), v.detach(), 0, 0, False)
     with pytest.raises(ValueError, match="one device"):
         fused.window_attention(q, k.cpu(), v.cpu(), 4)
 
