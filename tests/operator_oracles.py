@@ -3,7 +3,7 @@ elementwise error that their kernels' roundings allow.
 
 ``half`` below is the largest relative error of one rounding to the output
 type (finfo.eps / 2); ``small`` half the spacing of its subnormals; ``SLOP``
-covers the fp32 arithmetic (scores of up to 128 products, 2^x to 2^-21, sums)."""
+covers the fp32 arithmetic (scores of up to 128 products, 2^x to 2^-18, sums)."""
 import math
 
 import torch
