@@ -195,13 +195,16 @@ def linear_top_logits(h: torch.Tensor, W: torch.Tensor, k: int, temperature: flo
 class _LinearDistillation(torch.autograd.Function):
     """Mean distillation loss behind the LM head, its gradient computed chunk by
     chunk during forward as in :class:`_LinearCE`. The chunk's gradient of the
-    logits is unscaled (a sum, not a mean) in h's dtype; the division by the
-    number of rows in the loss, known on the device only, is applied with the
-    incoming gradient in backward, before the one rounding of each result."""
+    logits is that of the sum over the rows, in h's dtype, divided by
+    1 - alpha: the entry of a label is then close to -1, which rounds to itself,
+    where -(1 - alpha) would be off by the same part in every row. The number of
+    rows in the loss, known on the device only, and that factor are applied with
+    the incoming gradient in backward, before the one rounding of each result."""
 
     @staticmethod
     def forward(ctx, h, W, labels, top_values, top_indices, top_lse, temperature, alpha, chunk, need_grad):
         T, V = h.shape[0], W.shape[0]
+        scale = 1.0 / (1.0 - alpha) if labels is not None and alpha <= 0.9 else 1.0
         total = torch.zeros((), device=h.device, dtype=torch.float32)
         grad_h = torch.empty(h.shape, device=h.device, dtype=torch.float32) if need_grad else None
         make = torch.empty if T else torch.zeros
@@ -211,7 +214,7 @@ class _LinearDistillation(torch.autograd.Function):
             hc = h[s:e]
             loss_c, g = _fused.distillation_fwd_bwd(
                 _mm_fp32(hc, W.t()), None if labels is None else labels[s:e], top_values[s:e], top_indices[s:e],
-                None if top_lse is None else top_lse[s:e], temperature, alpha, 1.0, h.dtype, need_grad)
+                None if top_lse is None else top_lse[s:e], temperature, alpha, scale, h.dtype, need_grad)
             total += loss_c
             if need_grad:
                 grad_h[s:e] = _mm_fp32(g, W)
@@ -223,7 +226,7 @@ class _LinearDistillation(torch.autograd.Function):
                 else:
                     grad_W = g.t().float() @ hc.float()
         n = max(T, 1) if labels is None else ((labels >= 0) & (labels < V)).sum().clamp_min(1).float()
-        ctx.n = n
+        ctx.n = n * scale
         ctx.save_for_backward(grad_h, grad_W)
         ctx.dtypes = h.dtype, W.dtype
         return total / n
