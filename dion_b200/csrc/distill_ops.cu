@@ -197,12 +197,11 @@ __device__ __forceinline__ uint32_t kth_key(const uint32_t (&key)[R], int k) {
 // 50009 fp32, k = 200: 139 us. Bound by instructions and by the steps in which one
 // warp searches for a bound while the row's others wait; three rows to an SM (two in
 // fp32, whose groups take twice the registers) overlap these. Two full passes took 576 us, a
-// sample of half the size (twice the candidates) 532 us where this took 448.
+// sample of half the size (twice the candidates) 601 us where this took 534.
 template <typename T, int G>
-__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 3 : 2) top_logits_kernel(const T* __restrict__ logits, int64_t ld, int V, int k,
-                                                              bool vec, int ns, float c, float* __restrict__ values,
-                                                              int64_t* __restrict__ indices,
-                                                              float* __restrict__ lse) {
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 3 : 2)
+    top_logits_kernel(const T* __restrict__ logits, int64_t ld, int V, int k, bool vec, int ns, float c,
+                      float* __restrict__ values, int64_t* __restrict__ indices, float* __restrict__ lse) {
   __shared__ float red[kWarps];
   __shared__ uint32_t s_max[kThreads * G];
   __shared__ uint64_t s_cand[2][kMaxCand];
