@@ -6,7 +6,8 @@
 //   dQ = dS K / sqrt(d), dK = dS^T Q / sqrt(d), dV = P^T dO
 //
 // dK and dV of a key head sum over the query heads that share it. The forward
-// pass keeps each row's log-sum-exp; the backward pass recomputes P from it.
+// pass keeps each row's log-sum-exp; the backward pass recomputes P from it. A
+// row that sees one key has P = 1 and dS = 0, which both kernels write as such.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <cuda_fp16.h>

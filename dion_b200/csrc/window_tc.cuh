@@ -52,6 +52,12 @@ struct KeyTiles {
   }
 };
 
+// Query i sees one key: the first position always, every one with a window of one
+// and no first tokens. P = 1 whatever the score there, so dS = 0 exactly, where
+// dP - delta would be the difference of two fp32 sums of the same terms.
+__device__ __forceinline__ bool all_see_one(const WinArgs& a) { return a.window == 1 && a.sinks == 0; }
+__device__ __forceinline__ bool sees_one(const WinArgs& a, int i) { return i == 0 || all_see_one(a); }
+
 // Which of 32 keys k0 .. k0 + 31 query i sees, as a bit mask.
 __device__ __forceinline__ uint32_t seen_mask(const WinArgs& a, int i, int k0) {
   const int hi = i - k0;                       // last visible column
@@ -523,7 +529,9 @@ __global__ void __launch_bounds__(576, 1)
     const int r = quarter * 32 + lane, i = q0 + r;
     const uint32_t row = tmem + ((uint32_t)(quarter * 32) << 16);
     const int64_t at = ((int64_t)b * a.hq + h) * a.s_pad + q0;
-    const f2 c2 = make_f2(a.scale_log2, a.scale_log2), neg_l = make_f2(neg_lse[at + r], neg_lse[at + r]);
+    // a row that sees one key: P = 0 here, for its dS
+    const float nl = sees_one(a, i) ? neg_lse[at + r] - INFINITY : neg_lse[at + r];
+    const f2 c2 = make_f2(a.scale_log2, a.scale_log2), neg_l = make_f2(nl, nl);
     {
       // delta of 8 rows per warp, DP / 8 lanes to a row
       constexpr int kLanes = DP / 8, kRows = 32 / kLanes;
@@ -877,7 +885,9 @@ __global__ void __launch_bounds__(576, 1)
         const f2 g1 = make_f2(__uint_as_float(x[2 * e + 2]), __uint_as_float(x[2 * e + 3]));
         y[e] = pack2(p[e], T{});
         y[e + 1] = pack2(p[e + 1], T{});
-        y[16 + e] = pack2(mul2(p[e], add2(g0, D.x)), T{});
+        // query 0's dS is 0 (see sees_one)
+        const f2 p0 = e == 0 && q0 + part == 0 ? make_f2(0.f, hi_of(p[0])) : p[e];
+        y[16 + e] = pack2(mul2(p0, add2(g0, D.x)), T{});
         y[16 + e + 1] = pack2(mul2(p[e + 1], add2(g1, D.y)), T{});
       }
       tmem_st_32x32b_x32(pds, y);
@@ -895,7 +905,7 @@ __global__ void __launch_bounds__(576, 1)
       tc_fence_after();
       // two of a row's threads store dV, two dK, half of the row each
       const uint32_t acc = row + (part < 2 ? Cfg::kDV : Cfg::kDK);
-      const float f = part < 2 ? 1.f : a.scale;
+      const float f = part < 2 ? 1.f : all_see_one(a) ? 0.f : a.scale;
       T* out = (part < 2 ? dv : dk) + (((int64_t)b * a.s + j) * a.hkv + hk) * a.d;
       float* slot = nullptr;
       if (parts > 1)

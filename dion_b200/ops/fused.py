@@ -166,7 +166,8 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     """Causal attention in which position i sees position j <= i where
     ``i - j < window`` or ``j < sinks``. q: [b, s, hq, d], k/v: [b, s, hkv, d]
     (query head h reads key head h // (hq / hkv)) -> [b, s, hq, d]; scores are
-    scaled by 1 / sqrt(d). Inputs are finite: a non-finite key or value also
+    scaled by 1 / sqrt(d). A row that sees one key (the first one; every one with
+    window 1 and no first tokens) adds exactly 0 to the gradients of q and k. Inputs are finite: a non-finite key or value also
     reaches rows up to a tile of 128 beyond those that see it. The backward pass
     holds P (dP - delta) in the inputs' type, so in fp16 that is bounded by 65504."""
     _check_window(q, k, v, window, sinks)
