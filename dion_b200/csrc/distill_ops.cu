@@ -205,7 +205,9 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 3 : 2)
   __shared__ float red[kWarps];
   __shared__ uint32_t s_max[kThreads * G];
   __shared__ uint64_t s_cand[2][kMaxCand];
-  __shared__ int s_n;
+  // candidates, and those behind the second bound: a place of its own, so that no thread
+  // clears the first count while another has yet to read it
+  __shared__ int s_n, s_left;
   __shared__ uint32_t s_thr;
   const int64_t row = blockIdx.x;
   const T* x = logits + row * ld;
@@ -241,7 +243,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 3 : 2)
   }
 #pragma unroll
   for (int i = 0; i < G; ++i) s_max[tid * G + i] = best[i] == -INFINITY ? 0u : order_key(best[i]);
-  if (tid == 0) s_n = 0;
+  if (tid == 0) s_n = s_left = 0;
   __syncthreads();
   if (G == 1) {
     if (tid < 32) {
@@ -363,7 +365,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 3 : 2)
         for (int i = 0; i < kThreads / 32; ++i)
           keys[i] = i * 32 + tid < n ? (uint32_t)(s_cand[0][i * 32 + tid] >> 32) : 0u;
         const uint32_t t = kth_key<kThreads / 32, false>(keys, k);
-        if (tid == 0) s_thr = t, s_n = 0;
+        if (tid == 0) s_thr = t;
       }
     } else {
       uint32_t keys[kMaxCand / kThreads];
@@ -371,16 +373,16 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 3 : 2)
       for (int i = 0; i < kMaxCand / kThreads; ++i)
         keys[i] = i * kThreads + tid < n ? (uint32_t)(s_cand[0][i * kThreads + tid] >> 32) : 0u;
       const uint32_t t = kth_key<kMaxCand / kThreads, true>(keys, k);
-      if (tid == 0) s_thr = t, s_n = 0;
+      if (tid == 0) s_thr = t;
     }
     __syncthreads();
     thr = s_thr;
     for (int i = tid; i < n; i += kThreads) {
       const uint64_t cand = s_cand[0][i];
-      if ((uint32_t)(cand >> 32) >= thr) s_cand[1][atomicAdd(&s_n, 1)] = cand;
+      if ((uint32_t)(cand >> 32) >= thr) s_cand[1][atomicAdd(&s_left, 1)] = cand;
     }
     __syncthreads();
-    n = s_n;
+    n = s_left;
     from = 1;
   }
   for (int i = tid; i < n; i += kThreads) {
