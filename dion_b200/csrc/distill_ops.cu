@@ -191,8 +191,8 @@ __device__ __forceinline__ uint32_t kth_key(const uint32_t (&key)[R], int k) {
 // once. The host takes ns so that about 256 come together. A candidate's rank
 // is the number of larger ones (value, then the lower index), counted after a
 // second bound has thinned them out. Rows with too many candidates (equal
-// values), and rows with a NaN or +inf, take the exact threshold over the whole
-// row bit by bit and keep the lowest indices of the equal ones.
+// values; also checked: too few), and rows with a NaN or +inf, take the exact
+// threshold over the whole row bit by bit and keep the lowest indices of the equal ones.
 // 4096 x 128256 bf16, k = 64: 378 us, 2.8 TB/s (161 us at the copy rate); 1500 x
 // 50009 fp32, k = 200: 139 us. Bound by instructions and by the steps in which one
 // warp searches for a bound while the row's others wait; three rows to an SM (two in
@@ -214,6 +214,9 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 3 : 2)
   const int tid = threadIdx.x;
   const int lead = vec ? row_lead(row, ld, V, true) : 0;
   const int n8 = (V - lead) / 8, tail0 = lead + n8 * 8, rounds = (n8 + kThreads - 1) / kThreads;
+  // a row whose lead takes its last group may have a round less than the host counted; a
+  // round that was sampled twice would put its columns into two of the sets
+  ns = min(ns, max(rounds, 1));
   auto load = [&](int g, Raw8<T>& r) {
     if (vec)
       r.load(x + lead + g * 8);
@@ -310,7 +313,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 3 : 2)
   int from = 0;
   const bool special = !(sum.s <= FLT_MAX) || !(sum.m <= FLT_MAX);  // a NaN or +inf somewhere
   if (!special && tid == 0) lse[row] = sum.m * c * kLn2 + logf(sum.s);
-  if (n > kMaxCand || special) {
+  if (n > kMaxCand || n < k || special) {
     auto for_all = [&](auto f) {
       for (int col = tid; col < V; col += kThreads) f(col, order_key(as_f(x[col])));
     };

@@ -25,3 +25,23 @@ def test_second_bound_over_the_candidates(k, V):
         again = fused.top_logits(x, k)
         assert torch.equal(val, again.values) and torch.equal(idx, again.indices) and torch.equal(lse, again.lse)
     torch.cuda.current_stream().wait_stream(other)
+
+
+# rows of every lead (the odd widths and strides), widths whose last group of 8 columns a lead takes, so that the row
+# has a round of groups less than the width says, and more entries than one set of columns per thread gives a bound for
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rounds,k", [(1, 257), (1, 512), (1, 1024), (2, 300), (2, 700), (3, 300), (3, 500), (5, 300), (8, 257)])
+def test_widths_with_a_round_less_in_some_rows(rounds, k, dtype):
+    for extra in (8, 9, 11, 14, 15):
+        V = 4096 * rounds + extra
+        x = torch.randn(9, V, device=DEV, generator=torch.Generator(device=DEV).manual_seed(V + k)).to(dtype)
+        check_top(x, k)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V,stride", [(4104, 4105), (4104, 4111), (8200, 8203), (4109, 4200), (32776, 32777)])
+@pytest.mark.parametrize("k", [257, 512, 1000])
+def test_padded_rows(V, stride, k, dtype):
+    x = torch.randn(9, stride, device=DEV, generator=torch.Generator(device=DEV).manual_seed(V)).to(dtype)
+    check_top(x[:, :V], k)
+    check_top(x[:, stride - V:], k)
