@@ -152,14 +152,22 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 
+// the larger of two, NaN where one of them is (fmaxf drops it)
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 // 2^x of a pair on the FMA pipes: x = n + f with n the nearest whole number (by
 // adding 1.5 * 2^23, whose low bits then hold n) and f in [-1/2, 1/2]; 2^f by a
 // polynomial of degree 4 (minimax in relative error, found by reweighted least
-// squares with the constant term held at 1: off by 2^-18.4 at most); n goes into
-// the exponent as a whole number. x is at most 127; from -127 down the result is
-// exactly 0 (f = 0 there, and the exponent field becomes 0).
+// squares with the constant term held at 1: off by 2^-18.4 at most), times 2^n,
+// whose bits are n + 127 in the exponent's place. x is at most 127; from -127 down
+// the result is exactly 0 (the exponent's place is 0). A NaN stays one: it goes
+// through the polynomial, and the product keeps it whatever 2^n becomes.
 __device__ __forceinline__ f2 ex2_poly(f2 x) {
-  x = make_f2(fmaxf(lo_of(x), -127.f), fmaxf(hi_of(x), -127.f));
+  x = make_f2(max_nan(lo_of(x), -127.f), max_nan(hi_of(x), -127.f));
   const f2 t = add2(x, make_f2(12582912.f, 12582912.f));
   const f2 n = add2(t, make_f2(-12582912.f, -12582912.f));
   const f2 f = fma2(n, make_f2(-1.f, -1.f), x);
@@ -167,8 +175,8 @@ __device__ __forceinline__ f2 ex2_poly(f2 x) {
   p = fma2(p, f, make_f2(0.24024099f, 0.24024099f));
   p = fma2(p, f, make_f2(0.69312418f, 0.69312418f));
   p = fma2(p, f, make_f2(1.f, 1.f));
-  return make_f2(__uint_as_float(__float_as_uint(lo_of(p)) + (__float_as_uint(lo_of(t)) << 23)),
-                 __uint_as_float(__float_as_uint(hi_of(p)) + (__float_as_uint(hi_of(t)) << 23)));
+  return mul2(p, make_f2(__uint_as_float((__float_as_uint(lo_of(t)) << 23) + 0x3f800000u),
+                         __uint_as_float((__float_as_uint(hi_of(t)) << 23) + 0x3f800000u)));
 }
 // 2^x of pair `i` of a row: one pair in kPolyEvery by the polynomial, the others by the
 // special-function unit, whose four results a cycle and quarter of an SM bound these

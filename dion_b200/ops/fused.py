@@ -167,9 +167,12 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
     ``i - j < window`` or ``j < sinks``. q: [b, s, hq, d], k/v: [b, s, hkv, d]
     (query head h reads key head h // (hq / hkv)) -> [b, s, hq, d]; scores are
     scaled by 1 / sqrt(d). A row that sees one key (the first one; every one with
-    window 1 and no first tokens) adds exactly 0 to the gradients of q and k. Inputs are finite: a non-finite key or value also
-    reaches rows up to a tile of 128 beyond those that see it. The backward pass
-    holds P (dP - delta) in the inputs' type, so in fp16 that is bounded by 65504."""
+    window 1 and no first tokens) adds exactly 0 to the gradients of q and k.
+    Inputs are finite. A NaN is not lost (one in a key reaches o in every row that
+    sees the key), but a non-finite value, and in the backward pass a non-finite
+    query, key or output's gradient as well, also reaches rows up to a tile of 128
+    beyond those that see it. The backward pass holds P (dP - delta) in the inputs'
+    type, so in fp16 that is bounded by 65504."""
     _check_window(q, k, v, window, sinks)
     if not (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)):
         return torch.ops.dion_b200.window_attention_fwd(_tile_rows(q), _tile_rows(k), _tile_rows(v), int(window),

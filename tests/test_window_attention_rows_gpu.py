@@ -44,3 +44,46 @@ def test_first_row_sees_one_key(b, s, window, sinks, d):
     _, dq, dk, dv = run(q, k, v, do, window, sinks)
     assert not dq.any() and not dk.any() and not dv[:, 1:].any()
     assert_within(dv, *window_oracle(q, k, v, window, sinks, do)["dv"], "dv")
+
+
+# ------------------------------------------------------------------ non-finite inputs
+def sees(s, window, sinks, j):
+    i = torch.arange(s, device=DEV)
+    return (j <= i) & ((i - j < window) | (j < sinks))
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_non_finite_keys_reach_every_row_that_sees_them(d, bad):
+    """At every place of a step's 64 keys: NaN in o and dq of each row that sees the key, in dv of each key that such a
+    row sees; o of the other rows is finite."""
+    s, window, sinks = 200, 30, 1
+    for j in list(range(64, 128)) + [0, 199]:
+        q, k, v, do = make(1, s, 2, 1, d, seed=j)
+        with torch.no_grad():
+            q.abs_()
+            k[:, j, :, 3] = bad
+        o, dq, _, dv = run(q, k, v, do, window, sinks)
+        rows = sees(s, window, sinks, j)
+        assert o[:, rows].isnan().all() and o[:, ~rows].isfinite().all(), j
+        # a row whose only key has a NaN score has no other value either
+        assert dq[:, rows].isnan().all(), j
+        keys = torch.stack([sees(s, window, sinks, t)[rows].any() for t in range(s)])
+        assert dv[:, keys].isnan().all(), j
+
+
+def test_non_finite_queries_and_gradients():
+    """NaN in a query: in its row of o and dq. NaN in the output's gradient: in its row of dq and in dv of the keys that it sees."""
+    s, window, sinks = 200, 30, 1
+    for i in (0, 5, 6, 7, 130, 199):
+        q, k, v, do = make(1, s, 2, 1, 64, seed=i)
+        with torch.no_grad():
+            q[:, i, :, 3] = math.nan
+        o, dq, _, _ = run(q, k, v, do, window, sinks)
+        others = torch.arange(s, device=DEV) != i
+        assert o[:, i].isnan().all() and dq[:, i].isnan().all() and o[:, others].isfinite().all()
+        q, k, v, do = make(1, s, 2, 1, 64, seed=i)
+        do[:, i] = math.nan
+        _, dq, _, dv = run(q, k, v, do, window, sinks)
+        keys = torch.tensor([bool(sees(s, window, sinks, t)[i]) for t in range(s)], device=DEV)
+        assert dq[:, i].isnan().all() and dv[:, keys].isnan().all()
