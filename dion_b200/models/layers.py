@@ -249,7 +249,9 @@ def linear_distillation(h: torch.Tensor, W: torch.Tensor, labels: Optional[torch
     of the sum and of the mean; the loss is 0 if that leaves none."""
     h2 = h.reshape(-1, h.shape[-1])
     flat = lambda t: None if t is None else t.reshape(-1)  # noqa: E731
-    k = top_values.shape[-1]
+    rows = lambda t: t.reshape(math.prod(t.shape[:-1]), t.shape[-1])  # noqa: E731
+    teacher = flat(labels), rows(top_values), rows(top_indices), flat(top_lse), temperature, alpha
+    # of all rows at once: the chunks are slices, which would pass over a row too many
+    _fused._check_distillation((h2.shape[0], W.shape[0]), *teacher)
     need = torch.is_grad_enabled() and (h.requires_grad or W.requires_grad)
-    return _LinearDistillation.apply(h2, W, flat(labels), top_values.reshape(-1, k), top_indices.reshape(-1, k),
-                                     flat(top_lse), temperature, alpha, max(1, chunk), need)
+    return _LinearDistillation.apply(h2, W, *teacher, max(1, chunk), need)

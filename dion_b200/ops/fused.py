@@ -233,6 +233,27 @@ class TopLogits(NamedTuple):
 MAX_TOP = 1024
 
 
+def _check_distillation(shape, labels, top_values, top_indices, top_lse, temperature, alpha) -> None:
+    """Refuses what does not go with logits of ``shape``, or a shape that is not [T, V]."""
+    if len(shape) != 2 or top_values.dim() != 2 or top_values.shape != top_indices.shape:
+        raise ValueError(f"distillation: logits [T, V], top_values and top_indices [T, k], got {tuple(shape)}, "
+                         f"{tuple(top_values.shape)}, {tuple(top_indices.shape)}")
+    T, k = shape[0], top_values.shape[1]
+    if top_values.shape[0] != T or not 1 <= k <= MAX_TOP:
+        raise ValueError(f"distillation: {T} rows of 1 to {MAX_TOP} teacher entries, got {tuple(top_values.shape)}")
+    if top_indices.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"distillation: int32 or int64 top_indices, got {top_indices.dtype}")
+    for name, t in (("labels", labels), ("top_lse", top_lse)):
+        if t is not None and t.shape != (T,):
+            raise ValueError(f"distillation: {name} [{T}], got {tuple(t.shape)}")
+    if not temperature > 0 or not 0 <= alpha <= 1:
+        raise ValueError(f"distillation: temperature > 0 and 0 <= alpha <= 1, got {temperature} and {alpha}")
+    if labels is None and alpha != 1:
+        raise ValueError("distillation: alpha < 1 needs labels")
+    if labels is not None and labels.dtype != torch.int64:
+        raise ValueError(f"distillation: int64 labels, got {labels.dtype}")
+
+
 def _rows_enabled(x: torch.Tensor) -> bool:
     return ((not _DISABLED) and x.is_cuda and x.dtype in (torch.bfloat16, torch.float16, torch.float32) and has_ext()
             and hasattr(ext(), "top_logits"))
@@ -278,24 +299,8 @@ def distillation_fwd_bwd(logits: torch.Tensor, labels: Optional[torch.Tensor], t
     probability outside them. Without it the entries are normalised among
     themselves. labels: int64 [T] (a row whose label is outside [0, V) is left
     out: loss and gradient 0), or None with alpha = 1."""
-    if logits.dim() != 2 or top_values.dim() != 2 or top_values.shape != top_indices.shape:
-        raise ValueError(f"distillation: logits [T, V], top_values and top_indices [T, k], got {tuple(logits.shape)}, "
-                         f"{tuple(top_values.shape)}, {tuple(top_indices.shape)}")
+    _check_distillation(logits.shape, labels, top_values, top_indices, top_lse, temperature, alpha)
     T, V = logits.shape
-    k = top_values.shape[1]
-    if top_values.shape[0] != T or not 1 <= k <= MAX_TOP:
-        raise ValueError(f"distillation: {T} rows of 1 to {MAX_TOP} teacher entries, got {tuple(top_values.shape)}")
-    if top_indices.dtype not in (torch.int32, torch.int64):
-        raise ValueError(f"distillation: int32 or int64 top_indices, got {top_indices.dtype}")
-    for name, t in (("labels", labels), ("top_lse", top_lse)):
-        if t is not None and t.shape != (T,):
-            raise ValueError(f"distillation: {name} [{T}], got {tuple(t.shape)}")
-    if not temperature > 0 or not 0 <= alpha <= 1:
-        raise ValueError(f"distillation: temperature > 0 and 0 <= alpha <= 1, got {temperature} and {alpha}")
-    if labels is None and alpha != 1:
-        raise ValueError("distillation: alpha < 1 needs labels")
-    if labels is not None and labels.dtype != torch.int64:
-        raise ValueError(f"distillation: int64 labels, got {labels.dtype}")
     gdt = grad_dtype or logits.dtype
     if gdt != logits.dtype and (logits.dtype != torch.float32 or gdt not in (torch.bfloat16, torch.float16)):
         raise ValueError(f"distillation: a {gdt} gradient of {logits.dtype} logits")

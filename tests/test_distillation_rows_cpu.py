@@ -1,0 +1,51 @@
+"""Distillation: refusals behind the LM head, and its ranges (CPU)."""
+import pytest
+import torch
+
+from dion_b200.models import layers as L
+
+from test_distillation_cpu import distill_case
+
+
+# ------------------------------------------------------------------ refusals
+def linear_case(T=6):
+    z, labels, val, idx, lse = distill_case(T, 24, 3, True)
+    h, W = torch.randn(T, 8), torch.randn(24, 8)
+    return dict(h=h, W=W, labels=labels, top_values=val, top_indices=idx, top_lse=lse, alpha=0.5)
+
+
+@pytest.mark.parametrize("name", ["labels", "top_values", "top_indices", "top_lse", "top_values,top_indices", "h"])
+@pytest.mark.parametrize("chunk", [2, 4096])
+def test_linear_refuses_other_numbers_of_rows(name, chunk):
+    """More rows than tokens are not cut, fewer are not an empty chunk."""
+    for rows in (slice(0, 4), [0, 1, 2, 3, 4, 5, 0, 1]):
+        kw = linear_case()
+        for n in name.split(","):
+            kw[n] = kw[n][rows]
+        with pytest.raises(ValueError, match="distillation"):
+            L.linear_distillation(**kw, chunk=chunk)
+
+
+@pytest.mark.parametrize("change,message", [
+    (dict(top_indices=torch.zeros(3, 6).long()), "top_indices"),   # as many entries in other rows
+    (dict(alpha=1.5), "alpha"), (dict(alpha=float("nan")), "alpha"), (dict(labels=None), "needs labels"),
+    (dict(temperature=0.0), "temperature"), (dict(temperature=float("nan")), "temperature"),
+    (dict(top_values=torch.zeros(6, 0), top_indices=torch.zeros(6, 0).long()), "1 to 1024"),
+    (dict(labels=torch.zeros(6)), "int64 labels"),
+])
+def test_linear_refusals(change, message):
+    kw = linear_case()
+    kw.update(change)
+    with pytest.raises(ValueError, match=message):
+        L.linear_distillation(**kw)
+    empty = {n: t[:0] if torch.is_tensor(t) and n != "W" else t for n, t in kw.items()}
+    with pytest.raises(ValueError, match=message):
+        L.linear_distillation(**empty)
+
+
+def test_linear_without_rows():
+    kw = {n: t[:0] if torch.is_tensor(t) and n != "W" else t for n, t in linear_case().items()}
+    kw["h"], kw["W"] = kw["h"].requires_grad_(), kw["W"].requires_grad_()
+    loss = L.linear_distillation(**kw)
+    loss.backward()
+    assert loss.item() == 0 and kw["h"].grad.shape == (0, 8) and not kw["W"].grad.any()
