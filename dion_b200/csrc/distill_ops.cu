@@ -768,7 +768,7 @@ void top_logits(const at::Tensor& logits, at::Tensor& values, at::Tensor& indice
   const int64_t T = logits.size(0);
   const int V = (int)logits.size(1), k = (int)values.size(1);
   TORCH_CHECK(k >= 1 && k <= std::min(V, kMaxTop), "dion_b200 top_logits: 1 <= k <= min(V, 1024)");
-  TORCH_CHECK(tau > 0, "dion_b200 top_logits: temperature > 0");
+  TORCH_CHECK(tau >= 1e-18 && tau <= 1e18, "dion_b200 top_logits: temperature > 0 (1e-18 to 1e18)");
   check_out(values, logits, at::kFloat, {T, k}, "top_logits values");
   check_out(indices, logits, at::kLong, {T, k}, "top_logits indices");
   check_out(lse, logits, at::kFloat, {T}, "top_logits lse");
@@ -803,7 +803,7 @@ void distill_fwd_bwd(const at::Tensor& logits, const c10::optional<at::Tensor>& 
   const int64_t T = logits.size(0);
   const int V = (int)logits.size(1), k = (int)top_values.size(1);
   TORCH_CHECK(k >= 1 && k <= kMaxTop, "dion_b200 distill: 1 to 1024 teacher entries per row");
-  TORCH_CHECK(tau > 0, "dion_b200 distill: temperature > 0");
+  TORCH_CHECK(tau >= 1e-18 && tau <= 1e18, "dion_b200 distill: temperature > 0 (1e-18 to 1e18)");
   check_out(top_values, logits, at::kFloat, {T, k}, "distill top_values");
   TORCH_CHECK(top_indices.scalar_type() == at::kLong || top_indices.scalar_type() == at::kInt,
               "dion_b200 distill: int32 or int64 top_indices");

@@ -233,6 +233,12 @@ class TopLogits(NamedTuple):
 MAX_TOP = 1024
 
 
+def _check_temperature(op: str, temperature: float) -> None:
+    # its square and its inverse are fp32 factors
+    if not 1e-18 <= temperature <= 1e18:
+        raise ValueError(f"{op}: temperature > 0 (1e-18 to 1e18), got {temperature}")
+
+
 def _check_distillation(shape, labels, top_values, top_indices, top_lse, temperature, alpha) -> None:
     """Refuses what does not go with logits of ``shape``, or a shape that is not [T, V]."""
     if len(shape) != 2 or top_values.dim() != 2 or top_values.shape != top_indices.shape:
@@ -246,8 +252,9 @@ def _check_distillation(shape, labels, top_values, top_indices, top_lse, tempera
     for name, t in (("labels", labels), ("top_lse", top_lse)):
         if t is not None and t.shape != (T,):
             raise ValueError(f"distillation: {name} [{T}], got {tuple(t.shape)}")
-    if not temperature > 0 or not 0 <= alpha <= 1:
-        raise ValueError(f"distillation: temperature > 0 and 0 <= alpha <= 1, got {temperature} and {alpha}")
+    _check_temperature("distillation", temperature)
+    if not 0 <= alpha <= 1:
+        raise ValueError(f"distillation: 0 <= alpha <= 1, got {alpha}")
     if labels is None and alpha != 1:
         raise ValueError("distillation: alpha < 1 needs labels")
     if labels is not None and labels.dtype != torch.int64:
@@ -262,14 +269,13 @@ def _rows_enabled(x: torch.Tensor) -> bool:
 def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0) -> TopLogits:
     """The k largest logits of every row of [T, V] in falling order (equal ones
     by the lower index, a NaN above all), with the row's log-sum-exp at
-    ``temperature``. 1 <= k <= min(V, 1024)."""
+    ``temperature`` (1e-18 to 1e18). 1 <= k <= min(V, 1024)."""
     if logits.dim() != 2:
         raise ValueError(f"top_logits: logits [T, V], got {tuple(logits.shape)}")
     T, V = logits.shape
     if not 1 <= k <= min(V, MAX_TOP):
         raise ValueError(f"top_logits: 1 <= k <= min(V, {MAX_TOP}), got k = {k} with V = {V}")
-    if not temperature > 0:
-        raise ValueError(f"top_logits: temperature > 0, got {temperature}")
+    _check_temperature("top_logits", temperature)
     if _rows_enabled(logits):
         x = logits if logits.stride(1) == 1 or V == 1 else logits.contiguous()
         values = torch.empty(T, k, device=x.device, dtype=torch.float32)
@@ -298,7 +304,7 @@ def distillation_fwd_bwd(logits: torch.Tensor, labels: Optional[torch.Tensor], t
     entries then counts as one outcome more, held against the student's
     probability outside them. Without it the entries are normalised among
     themselves. labels: int64 [T] (a row whose label is outside [0, V) is left
-    out: loss and gradient 0), or None with alpha = 1."""
+    out: loss and gradient 0), or None with alpha = 1. Temperatures from 1e-18 to 1e18."""
     _check_distillation(logits.shape, labels, top_values, top_indices, top_lse, temperature, alpha)
     T, V = logits.shape
     gdt = grad_dtype or logits.dtype

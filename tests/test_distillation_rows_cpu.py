@@ -3,6 +3,7 @@ import pytest
 import torch
 
 from dion_b200.models import layers as L
+from dion_b200.ops import fused
 
 from test_distillation_cpu import distill_case
 
@@ -41,6 +42,15 @@ def test_linear_refusals(change, message):
     empty = {n: t[:0] if torch.is_tensor(t) and n != "W" else t for n, t in kw.items()}
     with pytest.raises(ValueError, match=message):
         L.linear_distillation(**empty)
+
+
+@pytest.mark.parametrize("temperature", [float("inf"), float("nan"), 1e-30, 1e30])
+def test_temperatures_out_of_range(temperature):
+    z, labels, val, idx, lse = distill_case(3, 16, 2, True)
+    with pytest.raises(ValueError, match="temperature"):
+        fused.distillation_fwd_bwd(z, labels, val, idx, lse, temperature, 0.5)
+    with pytest.raises(ValueError, match="temperature"):
+        L.top_logits(z, 2, temperature)
 
 
 def test_linear_without_rows():
