@@ -21,7 +21,6 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kMaxTop = 1024;     // entries kept per row
 constexpr int kMaxCand = 2048;    // candidates collected per row before ranking
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
 
 __device__ __forceinline__ float as_f(__nv_bfloat16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ float as_f(__half v) { return __half2float(v); }
@@ -200,8 +199,8 @@ __device__ __forceinline__ uint32_t kth_key(const uint32_t (&key)[R], int k) {
 // sample of half the size (twice the candidates) 601 us where this took 534.
 template <typename T, int G>
 __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 3 : 2)
-    top_logits_kernel(const T* __restrict__ logits, int64_t ld, int V, int k, bool vec, int ns, float c,
-                      float* __restrict__ values, int64_t* __restrict__ indices, float* __restrict__ lse) {
+    top_logits_kernel(const T* __restrict__ logits, int64_t ld, int V, int k, bool vec, int ns, float inv_tau,
+                      float c, float* __restrict__ values, int64_t* __restrict__ indices, float* __restrict__ lse) {
   __shared__ float red[kWarps];
   __shared__ uint32_t s_max[kThreads * G];
   __shared__ uint64_t s_cand[2][kMaxCand];
@@ -312,7 +311,8 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 3 : 2)
   int n = s_n;
   int from = 0;
   const bool special = !(sum.s <= FLT_MAX) || !(sum.m <= FLT_MAX);  // a NaN or +inf somewhere
-  if (!special && tid == 0) lse[row] = sum.m * c * kLn2 + logf(sum.s);
+  // (m * c would overflow for a row that is masked throughout by the type's lowest value)
+  if (!special && tid == 0) lse[row] = sum.m * inv_tau + logf(sum.s);
   if (n > kMaxCand || n < k || special) {
     auto for_all = [&](auto f) {
       for (int col = tid; col < V; col += kThreads) f(col, order_key(as_f(x[col])));
@@ -782,8 +782,8 @@ void top_logits(const at::Tensor& logits, at::Tensor& values, at::Tensor& indice
     const int ns = std::max(1, std::min(rounds, (rounds * k + 255) / 256));
     auto launch = [&](auto g) {
       top_logits_kernel<E, decltype(g)::value><<<(unsigned)T, kThreads, 0, s>>>(
-          static_cast<const E*>(logits.data_ptr()), logits.stride(0), V, k, aligned8(logits), ns, (float)(kLog2e / tau),
-          values.data_ptr<float>(), indices.data_ptr<int64_t>(), lse.data_ptr<float>());
+          static_cast<const E*>(logits.data_ptr()), logits.stride(0), V, k, aligned8(logits), ns, (float)(1 / tau),
+          (float)(kLog2e / tau), values.data_ptr<float>(), indices.data_ptr<int64_t>(), lse.data_ptr<float>());
     };
     // at least twice as many groups as entries keeps the candidates near 1.4 k
     if (k <= kThreads / 2)

@@ -45,3 +45,17 @@ def test_padded_rows(V, stride, k, dtype):
     x = torch.randn(9, stride, device=DEV, generator=torch.Generator(device=DEV).manual_seed(V)).to(dtype)
     check_top(x[:, :V], k)
     check_top(x[:, stride - V:], k)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V", [100, 700, 5003])
+def test_rows_of_the_lowest_value(dtype, V):
+    """A row that is masked throughout by the type's lowest value (its log-sum-exp is that value, to rounding), one that is
+    masked but for a few columns, and one of the largest values."""
+    x = torch.randn(4, V, device=DEV, generator=torch.Generator(device=DEV).manual_seed(V)).to(dtype)
+    x[0] = torch.finfo(dtype).min
+    x[1, 5:] = torch.finfo(dtype).min
+    x[2, ::2] = torch.finfo(dtype).max
+    for tau in (1.0, 2.0, 1.5):
+        lse = check_top(x, 7, tau)[2]
+        assert lse.isfinite().all()
