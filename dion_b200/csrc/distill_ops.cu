@@ -495,7 +495,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     const int64_t i = a.idx64 ? static_cast<const int64_t*>(a.top_indices)[row * a.k + j]
                               : static_cast<const int*>(a.top_indices)[row * a.k + j];
     const bool in = i >= 0 && i < V;
-    const float t = a.top_values[row * a.k + j] * a.inv_tau;
+    const float t = a.top_values[row * a.k + j];
     s_i[j] = in ? (int)i : -1;
     s_p[j] = in ? t : -INFINITY;
     if (in) {
@@ -509,17 +509,22 @@ __global__ void __launch_bounds__(kThreads, 2)
       tmax = fmaxf(tmax, t);
     }
   }
-  float tlse;
+  // log p = (t - tref) / tau - tlog of an entry t. Without a log-sum-exp tref is the
+  // entries' maximum: the softmax does not know an offset that all of them have, and a
+  // sum tref / tau + tlog would round the second term away where the first is large (at
+  // the type's lowest value altogether).
+  float tref = 0.f, tlog;
   if (a.top_lse != nullptr) {
-    tlse = a.top_lse[row];
+    tlog = a.top_lse[row];
   } else {
-    tmax = block_max(tmax, red);
+    tref = block_max(tmax, red);
     float s = 0.f;
     for (int j = tid; j < a.k; j += kThreads)
-      if (s_i[j] >= 0) s += ex2((s_p[j] - tmax) * kLog2e);
+      if (s_i[j] >= 0) s += ex2((s_p[j] - tref) * c);
     s = block_sum(s, red);
-    tlse = tmax + logf(s);  // -inf without entries; s_p stays -inf there and gives p = 0 below
+    tlog = logf(s);  // -inf without entries; s_p stays -inf there and gives p = 0 below
   }
+  auto log_p = [&](float t) { return (t - tref) * a.inv_tau - tlog; };
   __syncthreads();
 
   // y = 2^(c (z - ref)) of the teacher's softmax -> the label's
@@ -611,12 +616,12 @@ __global__ void __launch_bounds__(kThreads, 2)
   for (int j = tid; j < a.k; j += kThreads)
     if (s_i[j] >= 0) zmax = fmaxf(zmax, s_z[j]);
   const float top = fmaxf(block_max(zmax, red), rm);
-  float set = 0.f, setf = 0.f, psum = 0.f, cross = 0.f;  // the last: sum p (log p - z / tau)
+  float set = 0.f, setf = 0.f, psum = 0.f, cross = 0.f;  // the last: sum p (log p - (z - top) / tau)
   for (int j = tid; j < a.k; j += kThreads)
     if (s_i[j] >= 0) {
-      const float p = s_p[j] == -INFINITY ? 0.f : ex2((s_p[j] - tlse) * kLog2e);
+      const float lp = log_p(s_p[j]), p = s_p[j] == -INFINITY ? 0.f : ex2(lp * kLog2e);
       psum += p;
-      if (p != 0.f) cross += p * (s_p[j] - tlse - s_z[j] * a.inv_tau);
+      if (p != 0.f) cross += p * (lp - (s_z[j] - top) * a.inv_tau);
       if (first_of(j)) {
         const float y = ex2((s_z[j] - top) * c);
         set += y;
@@ -636,12 +641,12 @@ __global__ void __launch_bounds__(kThreads, 2)
   const bool has_rest = a.top_lse != nullptr && s_marked < V;
   const float p_rest = has_rest ? fmaxf(1.f - psum, 0.f) : 0.f;
   if (tid == 0) {
-    const float logz = top * a.inv_tau + logf(B);  // log of the sum of exp(z / tau)
-    float kl = psum != 0.f ? cross + psum * logz : 0.f;
-    if (p_rest > 0.f) kl += p_rest * (logf(p_rest) - (rm * a.inv_tau + logf(rest) - logz));
-    const float log_full = both ? top + logf(F) : logz;
+    // all logits relative to the largest one: the loss does not know a common offset
+    const float logB = logf(B);  // log of the sum of exp((z - top) / tau)
+    float kl = psum != 0.f ? cross + psum * logB : 0.f;
+    if (p_rest > 0.f) kl += p_rest * (logf(p_rest) - ((rm - top) * a.inv_tau + logf(rest) - logB));
     a.row_loss[row] = (a.alpha > 0.f ? a.alpha * a.tau * a.tau * kl : 0.f) +
-                      (hard ? (1.f - a.alpha) * (log_full - zy) : 0.f);
+                      (hard ? (1.f - a.alpha) * ((both ? logf(F) : logB) + (top - zy)) : 0.f);
   }
   if (grad == nullptr) return;
 
@@ -701,7 +706,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     if (i < 0 || !first_of(j)) continue;
     float p = 0.f;
     for (int e = j; e < (twice ? a.k : j + 1); ++e)
-      if (s_i[e] == i && s_p[e] != -INFINITY) p += ex2((s_p[e] - tlse) * kLog2e);
+      if (s_i[e] == i && s_p[e] != -INFINITY) p += ex2(log_p(s_p[e]) * kLog2e);
     float g = w_soft * (soft_at(s_z[j]) - p);
     if (hard) g += w_hard * (hard_at(s_z[j]) - (i == label ? 1.f : 0.f));
     put(gx + i, g);

@@ -337,24 +337,29 @@ def _distillation_ref(z, labels, top_values, top_indices, top_lse, tau, alpha, n
     ninf = float("-inf")
     valid = (top_indices >= 0) & (top_indices < V)
     at = top_indices.clamp(0, V - 1)
-    t = torch.where(valid, top_values / tau, ninf)
-    tl = torch.logsumexp(t, 1, keepdim=True) if top_lse is None else top_lse[:, None]
-    logp = t - tl
+    t = torch.where(valid, top_values, ninf)
+    # to the row's maximum, before anything is rounded: an offset that all of a row have means nothing
+    relative = lambda x: x - x.amax(1, keepdim=True).clamp_min(torch.finfo(x.dtype).min)  # noqa: E731
+    if top_lse is None:
+        t = relative(t) / tau
+        logp = t - torch.logsumexp(t, 1, keepdim=True)
+    else:
+        t = t / tau
+        logp = t - top_lse[:, None]
     p = torch.where(t == ninf, 0.0, logp.exp())
-    zt = z / tau
-    logz = torch.logsumexp(zt, 1, keepdim=True)
-    kl = torch.where(p == 0, 0.0, p * (logp - (zt.gather(1, at) - logz))).sum(1)
-    q = (zt - logz).exp() if need_grad else None
+    logq = torch.log_softmax(relative(z) / tau, 1)
+    kl = torch.where(p == 0, 0.0, p * (logp - logq.gather(1, at))).sum(1)
+    q = logq.exp() if need_grad else None
     mass = p.sum(1, keepdim=True)
     soft = q
     if top_lse is not None:
         inside = torch.zeros_like(z).scatter_add(1, at, valid.to(z.dtype)) > 0
         p_rest = torch.where(inside.all(1, keepdim=True), 0.0, (1 - mass).clamp_min(0))
-        rest = torch.logsumexp(zt.masked_fill(inside, ninf), 1, keepdim=True)
-        kl = kl + torch.where(p_rest > 0, p_rest * (p_rest.log() - (rest - logz)), 0.0)[:, 0]
+        rest = torch.logsumexp(logq.masked_fill(inside, ninf), 1, keepdim=True)
+        kl = kl + torch.where(p_rest > 0, p_rest * (p_rest.log() - rest), 0.0)[:, 0]
         mass = mass + p_rest
         if need_grad:
-            soft = soft - torch.where(inside | (rest == ninf), 0.0, p_rest * (zt - rest).exp())
+            soft = soft - torch.where(inside | (rest == ninf), 0.0, p_rest * (logq - rest).exp())
     loss = alpha * tau * tau * kl if alpha > 0 else torch.zeros_like(kl)
     grad = None
     if need_grad:

@@ -1,0 +1,62 @@
+"""Rows of logits that the distillation loss does not tell from ordinary ones: a common offset, the type's lowest value
+throughout. Shared by the CPU and the GPU tests."""
+import torch
+
+from dion_b200.ops import fused
+
+from operator_oracles import assert_within, distill_oracle, halves
+from test_distillation_cpu import distill_case
+
+OFFSET = 2.0 ** 14
+
+
+def check_offset(tau, rest, alpha, device, dtype=torch.float32):
+    """The softmax does not know a common offset of its logits. Values are multiples of 2^-8 (the log-sum-exp of 2^-9),
+    so that adding the offset is exact in fp32: what changes is the kernel's rounding alone. The oracle, and its
+    tolerance, are those of the rows without it."""
+    z, labels, val, idx, lse = distill_case(9, 700, 12, rest, tau=tau, device=device)
+    z, val = ((t * 256).round() / 256 for t in (z, val))
+    if rest:
+        lse = (lse * 512).round() / 512
+    labels = labels if alpha < 1 else None
+    want, wg, tl, tg = distill_oracle(z, labels, val, idx, lse, tau, alpha)
+    for off_z, off_t in ((0.0, 0.0), (OFFSET, 0.0), (-OFFSET, 0.0), (0.0, OFFSET), (0.0, -OFFSET)):
+        if off_t and rest:
+            continue  # their log-sum-exp is an input, rounded by whoever gave it
+        loss, grad = fused.distillation_fwd_bwd(z + off_z, labels, val + off_t, idx, lse, tau, alpha)
+        assert abs(loss.item() - want.item()) <= tl.item(), (off_z, off_t, loss.item(), want.item(), tl.item())
+        assert_within(grad, wg, halves(grad.dtype)[0] * wg.abs() + tg + 1e-30, f"grad {off_z} {off_t}")
+
+
+def check_lowest(rest, alpha, device, dtype):
+    """Every logit of a row at its type's lowest value: as a row of zeros. So are the teacher's entries where they are
+    normalised among themselves."""
+    z, labels, val, idx, lse = distill_case(6, 500, 8, rest, device=device)
+    labels[:] = idx[:, 0]
+    labels[1] = 499
+    z, zeros = z.to(dtype), torch.zeros(6, 500, device=device)
+    zeros[3:] = z[3:].float()
+    z[:3] = torch.finfo(dtype).min
+    tv = val.clone()
+    if not rest:
+        val[2], tv[2] = 0.0, torch.finfo(torch.float32).min
+    want, wg, tl, tg = distill_oracle(zeros, labels, val, idx, lse, 1.0, alpha)
+    loss, grad = fused.distillation_fwd_bwd(z, labels, tv, idx, lse, 1.0, alpha)
+    assert abs(loss.item() - want.item()) <= tl.item(), (loss.item(), want.item(), tl.item())
+    half, small = halves(grad.dtype)
+    assert_within(grad, wg, half * wg.abs() + tg + small + 1e-30, "grad")
+
+
+def check_masked_vocabulary(rest, device, dtype):
+    """A student whose vocabulary is masked by the type's lowest value outside a few columns, the teacher's among them."""
+    z, labels, val, idx, lse = distill_case(4, 500, 8, rest, device=device)
+    keep = torch.zeros(4, 500, dtype=torch.bool, device=device).scatter_(1, idx, True)
+    keep[:, :3] = True
+    labels[:] = 1
+    z = z.to(dtype).masked_fill(~keep, torch.finfo(dtype).min)
+    out = z.float().masked_fill(~keep, float("-inf"))
+    want, wg, tl, tg = distill_oracle(out, labels, val, idx, lse, 2.0, 0.5)
+    loss, grad = fused.distillation_fwd_bwd(z, labels, val, idx, lse, 2.0, 0.5)
+    assert abs(loss.item() - want.item()) <= tl.item(), (loss.item(), want.item(), tl.item())
+    half, small = halves(grad.dtype)
+    assert_within(grad, wg, half * wg.abs() + tg + small + 1e-30, "grad")

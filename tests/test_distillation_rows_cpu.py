@@ -5,6 +5,7 @@ import torch
 from dion_b200.models import layers as L
 from dion_b200.ops import fused
 
+from distillation_extremes import check_lowest, check_masked_vocabulary, check_offset
 from test_distillation_cpu import distill_case
 
 
@@ -59,3 +60,21 @@ def test_linear_without_rows():
     loss = L.linear_distillation(**kw)
     loss.backward()
     assert loss.item() == 0 and kw["h"].grad.shape == (0, 8) and not kw["W"].grad.any()
+
+
+# ------------------------------------------------------------------ extreme logits
+@pytest.mark.parametrize("rest", [False, True])
+@pytest.mark.parametrize("tau,alpha", [(1.0, 1.0), (1.0, 0.5), (2.0, 0.5), (1.5, 1.0)])
+def test_common_offset(tau, alpha, rest):
+    check_offset(tau, rest, alpha, "cpu")
+
+
+@pytest.mark.parametrize("rest", [False, True])
+@pytest.mark.parametrize("alpha", [1.0, 0.5])
+def test_rows_of_the_lowest_value(alpha, rest):
+    check_lowest(rest, alpha, "cpu", torch.float32)
+
+
+@pytest.mark.parametrize("rest", [False, True])
+def test_vocabulary_masked_by_the_lowest_value(rest):
+    check_masked_vocabulary(rest, "cpu", torch.float32)
