@@ -195,16 +195,29 @@ def linear_top_logits(h: torch.Tensor, W: torch.Tensor, k: int, temperature: flo
 class _LinearDistillation(torch.autograd.Function):
     """Mean distillation loss behind the LM head, its gradient computed chunk by
     chunk during forward as in :class:`_LinearCE`. The chunk's gradient of the
-    logits is that of the sum over the rows, in h's dtype, divided by
-    1 - alpha: the entry of a label is then close to -1, which rounds to itself,
-    where -(1 - alpha) would be off by the same part in every row. The number of
-    rows in the loss, known on the device only, and that factor are applied with
-    the incoming gradient in backward, before the one rounding of each result."""
+    logits is that of the sum over the rows, in h's dtype, times a factor of
+    :meth:`_scale`. The number of rows in the loss, known on the device only, and
+    that factor are applied with the incoming gradient in backward, before the
+    one rounding of each result."""
+
+    @staticmethod
+    def _scale(dtype, labels, temperature, alpha):
+        """Factor of the logits' gradient between the loss and the head's products.
+        1 / (1 - alpha) with labels: the entry of a label is then close to -1, which
+        rounds to itself, where -(1 - alpha) would be off by the same part in every
+        row. In fp16 a power of two on top: an entry of a 128k vocabulary is 8e-6 on
+        average, among the subnormals (spacing 6e-8), while no entry exceeds
+        (1 - alpha) + alpha * temperature; that bound is brought to 2^14 ... 2^15."""
+        hard = 1.0 - alpha if labels is not None and alpha < 1 else 0.0
+        scale = 1.0 / hard if hard else 1.0
+        if dtype == torch.float16:
+            scale *= 2.0 ** (15 - math.ceil(math.log2((hard + alpha * temperature) * scale)))
+        return scale
 
     @staticmethod
     def forward(ctx, h, W, labels, top_values, top_indices, top_lse, temperature, alpha, chunk, need_grad):
         T, V = h.shape[0], W.shape[0]
-        scale = 1.0 / (1.0 - alpha) if labels is not None and alpha <= 0.9 else 1.0
+        scale = _LinearDistillation._scale(h.dtype, labels, temperature, alpha)
         total = torch.zeros((), device=h.device, dtype=torch.float32)
         grad_h = torch.empty(h.shape, device=h.device, dtype=torch.float32) if need_grad else None
         make = torch.empty if T else torch.zeros
