@@ -640,23 +640,35 @@ __global__ void __launch_bounds__(kThreads, 2)
   }
   const bool has_rest = a.top_lse != nullptr && s_marked < V;
   const float p_rest = has_rest ? fmaxf(1.f - psum, 0.f) : 0.f;
+  const float q_set = set / B;
   if (tid == 0) {
     // all logits relative to the largest one: the loss does not know a common offset
     const float logB = logf(B);  // log of the sum of exp((z - top) / tau)
     float kl = psum != 0.f ? cross + psum * logB : 0.f;
-    if (p_rest > 0.f) kl += p_rest * (logf(p_rest) - ((rm - top) * a.inv_tau + logf(rest) - logB));
+    if (p_rest > 0.f) {
+      // log(p_rest / q_rest); where the set holds little, from the set's two sums, whose
+      // roundings are far smaller than those of two numbers near 1
+      const float log_ratio = q_set < 0.5f && psum < 0.5f
+                                  ? log1pf(-psum) - log1pf(-q_set)
+                                  : logf(p_rest) - ((rm - top) * a.inv_tau + logf(rest) - logB);
+      kl += p_rest * log_ratio;
+    }
     a.row_loss[row] = (a.alpha > 0.f ? a.alpha * a.tau * a.tau * kl : 0.f) +
                       (hard ? (1.f - a.alpha) * ((both ? logf(F) : logB) + (top - zy)) : 0.f);
   }
   if (grad == nullptr) return;
 
-  // gradient. Outside the set: w_hard softmax(z) + w_soft (q - p_rest q / q_rest)
+  // gradient. Outside the set: w_hard softmax(z) + w_soft q (1 - p_rest / q_rest), where
+  // 1 - p_rest / q_rest = (psum - q_set) / q_rest: at a high temperature the set holds
+  // little on either side, and the difference of two numbers near 1 would keep few bits
   const float w_soft = a.grad_scale * a.alpha * a.tau * (psum + p_rest == 0.f ? 0.f : 1.f);
   const float w_hard = hard ? a.grad_scale * (1.f - a.alpha) : 0.f;
   const float inv_B = 1.f / B, inv_F = both ? 1.f / F : inv_B;
-  float f_rest = 0.f, f_full = 0.f;  // factors of 2^(c (z - rm)) and of 2^(log2e (z - rm))
+  // factors of 2^(c (z - rm)), the first of them the teacher's part alone, and of 2^(log2e (z - rm))
+  float f_soft = 0.f, f_rest = 0.f, f_full = 0.f;
   if (rest > 0.f || rest != rest) {
-    f_rest = w_soft * (to_top * inv_B - p_rest / rest) + (both ? 0.f : w_hard * to_top * inv_B);
+    f_soft = w_soft * (p_rest > 0.f ? (psum - q_set) / rest : to_top * inv_B);
+    f_rest = f_soft + (both ? 0.f : w_hard * to_top * inv_B);
     f_full = both ? w_hard * to_top_full * inv_F : 0.f;
   }
   const f2 neg_m = make_f2(-rm, -rm), c2 = make_f2(c, c), fr2 = make_f2(f_rest, f_rest), ff2 = make_f2(f_full, f_full);
@@ -712,8 +724,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     put(gx + i, g);
   }
   if (hard && tid == 0 && !is_marked((int)label)) {
-    const float r = rest > 0.f ? p_rest * ex2((zy - rm) * c) / rest : 0.f;
-    put(gx + label, w_soft * (soft_at(zy) - r) + w_hard * (hard_at(zy) - 1.f));
+    put(gx + label, f_soft * ex2((zy - rm) * c) + w_hard * (hard_at(zy) - 1.f));
   }
 }
 

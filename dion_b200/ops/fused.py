@@ -355,11 +355,15 @@ def _distillation_ref(z, labels, top_values, top_indices, top_lse, tau, alpha, n
     if top_lse is not None:
         inside = torch.zeros_like(z).scatter_add(1, at, valid.to(z.dtype)) > 0
         p_rest = torch.where(inside.all(1, keepdim=True), 0.0, (1 - mass).clamp_min(0))
+        q_set = torch.where(inside, logq.exp(), 0.0).sum(1, keepdim=True)
         rest = torch.logsumexp(logq.masked_fill(inside, ninf), 1, keepdim=True)
-        kl = kl + torch.where(p_rest > 0, p_rest * (p_rest.log() - rest), 0.0)[:, 0]
-        mass = mass + p_rest
+        # where the set holds little, from its sums: their roundings are far smaller than those of two numbers near 1
+        ratio = torch.where((mass < 0.5) & (q_set < 0.5), (-mass).log1p() - (-q_set).log1p(), p_rest.log() - rest)
+        kl = kl + torch.where(p_rest > 0, p_rest * ratio, 0.0)[:, 0]
         if need_grad:
-            soft = soft - torch.where(inside | (rest == ninf), 0.0, p_rest * (logq - rest).exp())
+            outside = torch.where(p_rest > 0, (mass - q_set) * (logq - rest).exp(), q)
+            soft = torch.where(inside | (rest == ninf), q, outside)
+        mass = mass + p_rest
     loss = alpha * tau * tau * kl if alpha > 0 else torch.zeros_like(kl)
     grad = None
     if need_grad:

@@ -60,3 +60,25 @@ def check_masked_vocabulary(rest, device, dtype):
     assert abs(loss.item() - want.item()) <= tl.item(), (loss.item(), want.item(), tl.item())
     half, small = halves(grad.dtype)
     assert_within(grad, wg, half * wg.abs() + tg + small + 1e-30, "grad")
+
+
+def check_high_temperature(tau, V, k, device, gdt=None):
+    """The teacher's entries hold little, and little more than the student gives them. Tolerances, with e = 2^-24: a
+    log-probability is off by 2^-20 of itself (its fp32 sum, 2^x to 2 e, its argument's rounding), so a probability by
+    2^-19 of itself for logarithms to 12, and p and q, their sums over the set and their difference by 2^-18 (p + q).
+    Outside the set the gradient is alpha tau q (sum p - sum q) / q_rest; the loss sum p (log p - log q) + p_rest (log(1 - sum p) -
+    log(1 - sum q)). Twice each."""
+    z, _, val, idx, lse = distill_case(7, V, k, True, tau=tau, seed=3, device=device)
+    want, wg, _, _ = distill_oracle(z, None, val, idx, lse, tau, 1.0)
+    loss, grad = fused.distillation_fwd_bwd(z, None, val, idx, lse, tau, 1.0, 1.0, gdt)
+    logq = torch.log_softmax(z.double() / tau, 1)
+    lp, lq = val.double() / tau - lse.double()[:, None], logq.gather(1, idx)
+    both = lp.exp().sum(1) + lq.exp().sum(1)
+    tl = tau * tau * ((lp.exp() * (lp.abs() + lq.abs())).sum(1) * 2.0 ** -19 + both * 2.0 ** -17).sum()
+    assert abs(loss.item() - want.item()) <= tl.item() + 2.0 ** -20 * want.abs().item(), (loss.item(), want.item(), tl.item())
+    out = torch.ones_like(z, dtype=torch.bool).scatter_(1, idx, False)
+    tol = tau * logq.exp() * (both * 2.0 ** -17)[:, None]
+    half, small = halves(grad.dtype)
+    tol = tol + (half + 2.0 ** -18) * wg.abs() + small
+    tol = torch.where(out, tol, tol + tau * (logq.exp() * 2.0 ** -17).scatter_add(1, idx, lp.exp() * 2.0 ** -17))
+    assert_within(grad, wg, tol, "grad")

@@ -5,7 +5,7 @@ import torch
 from dion_b200.models import layers as L
 from dion_b200.ops import fused
 
-from distillation_extremes import check_lowest, check_masked_vocabulary, check_offset
+from distillation_extremes import check_high_temperature, check_lowest, check_masked_vocabulary, check_offset
 from test_distillation_cpu import distill_case
 
 
@@ -78,3 +78,8 @@ def test_rows_of_the_lowest_value(alpha, rest):
 @pytest.mark.parametrize("rest", [False, True])
 def test_vocabulary_masked_by_the_lowest_value(rest):
     check_masked_vocabulary(rest, "cpu", torch.float32)
+
+
+@pytest.mark.parametrize("tau,V,k", [(10.0, 5003, 4), (30.0, 20000, 16), (100.0, 20000, 64)])
+def test_high_temperature(tau, V, k):
+    check_high_temperature(tau, V, k, "cpu")

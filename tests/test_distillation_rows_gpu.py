@@ -4,7 +4,7 @@ import torch
 
 from dion_b200.models import layers as L
 
-from distillation_extremes import check_lowest, check_masked_vocabulary, check_offset
+from distillation_extremes import check_high_temperature, check_lowest, check_masked_vocabulary, check_offset
 from operator_oracles import distill_oracle, halves
 from test_distillation_cpu import distill_case
 from test_distillation_gpu import TYPES
@@ -33,19 +33,23 @@ def test_vocabulary_masked_by_the_lowest_value(rest, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
-@pytest.mark.parametrize("labelled,alpha,tau", [(True, 0.5, 1.0), (True, 0.0, 1.0), (True, 0.95, 2.0), (True, 0.999999, 1.0), (False, 1.0, 1.0)])
+@pytest.mark.parametrize("labelled,alpha,tau", [(True, 0.5, 1.0), (True, 0.0, 1.0), (True, 0.95, 2.0), (True, 0.999999, 1.0), (False, 1.0, 1.0),
+                                                (False, 1.0, 30.0)])
 def test_head_gradient_over_a_large_vocabulary(labelled, alpha, tau, dtype):
     """The head's rows that are neither labels nor teacher entries sum gradients of 1e-5 and less, the labels' rows one
     of nearly 1 - alpha. In the mean square over such rows, two roundings (the logits' gradient, the result), each
     half / sqrt(3) of its value, and a quarter more for all that is fp32. (The loss is scaled as fp16 wants, so that
-    the result itself is not among the subnormals.)"""
+    the result itself is not among the subnormals.) In fp16 an entry of the logits' gradient that is a subnormal under
+    its factor, 2^14 / temperature at least, is off by up to 2^-25 whatever its size, 2^-25 / sqrt(3) in the mean
+    square, so each of the head's entries by that / factor * sqrt(sum h^2): what is 2^-39 of the largest possible
+    entry (at temperature 30 without labels, the rows in question are) keeps fewer bits."""
     T, V, D = 96, 128256, 64
     _, labels, val, idx, lse = distill_case(T, V, 16, True, tau=tau, device=DEV)
     g = torch.Generator(device=DEV).manual_seed(0)
     h = torch.randn(T, D, device=DEV, generator=g).to(dtype).requires_grad_()
     W = (torch.randn(V, D, device=DEV, generator=g) * 0.1).to(dtype).requires_grad_()
     labels = labels if labelled else None
-    up = 2.0 ** 13
+    up = 2.0 ** (13 if labelled else 21)  # 7e-9 * 96^-1/2 at temperature 30 would be 7e-6 under 2^13, a subnormal
     (L.linear_distillation(h, W, labels, val, idx, lse, tau, alpha, chunk=64) * up).backward()
     hd, Wd = h.detach().double(), W.detach().double()
     wg = distill_oracle(hd @ Wd.t(), labels, val, idx, lse, tau, alpha)[1]
@@ -55,11 +59,21 @@ def test_head_gradient_over_a_large_vocabulary(labelled, alpha, tau, dtype):
     kind[idx.flatten()] = 1
     if labelled:
         kind[labels[labels >= 0]] = 2
-    bound = 1.25 * (2 / 3) ** 0.5 * halves(dtype)[0]
+    half, small = halves(dtype)
+    sub = small / 3 ** 0.5 / L._LinearDistillation._scale(dtype, labels, tau, alpha) * up / n
     off = {}
     for name, m in (("rest", kind == 0), ("entries", kind == 1), ("labels", kind == 2)):
         if m.any() and not (name == "entries" and alpha == 0):
-            off["W " + name] = ((W.grad.double() - want)[m].norm() / want[m].norm()).item()
+            flat = (sub * hd.norm(dim=0)).norm() * m.sum() ** 0.5 / want[m].norm()
+            off["W " + name] = ((W.grad.double() - want)[m].norm() / want[m].norm()).item(), \
+                1.25 * (2 / 3 * half ** 2 + flat.item() ** 2) ** 0.5
     wh = up * wg @ Wd / n
-    off["h"] = ((h.grad.double() - wh).norm() / wh.norm()).item()
-    assert all(v <= bound for v in off.values()), (off, bound)
+    flat = (sub * Wd.norm(dim=0)).norm() * T ** 0.5 / wh.norm()
+    off["h"] = ((h.grad.double() - wh).norm() / wh.norm()).item(), 1.25 * (2 / 3 * half ** 2 + flat.item() ** 2) ** 0.5
+    assert all(v <= bound for v, bound in off.values()), off
+
+
+@pytest.mark.parametrize("gdt", [None, torch.bfloat16])
+@pytest.mark.parametrize("tau,V,k", [(10.0, 5003, 4), (30.0, 20000, 16), (100.0, 20000, 64), (30.0, 128256, 16), (30.0, 128256, 256)])
+def test_high_temperature(tau, V, k, gdt):
+    check_high_temperature(tau, V, k, DEV, gdt)
