@@ -9,6 +9,7 @@ autograd reference)."""
 from __future__ import annotations
 
 import math
+from contextlib import contextmanager
 from typing import Optional, Tuple
 
 import torch
@@ -179,14 +180,28 @@ def _mm_fp32(a: torch.Tensor, b: torch.Tensor) -> torch.Tensor:
     return a.float() @ b.float()
 
 
+@contextmanager
+def _head(h: torch.Tensor, W: torch.Tensor):
+    """h and W in the type that F.linear would take them in, and autocast off for what is done with
+    them: it would round the products' fp32 results to its type."""
+    dev = h.device.type
+    if not torch.is_autocast_enabled(dev):
+        yield h, W
+        return
+    dtype = torch.get_autocast_dtype(dev)
+    h, W = h.to(dtype), W.to(dtype)
+    with torch.autocast(dev, enabled=False):
+        yield h, W
+
+
 @torch.no_grad()
 def linear_top_logits(h: torch.Tensor, W: torch.Tensor, k: int, temperature: float = 1.0,
                       chunk: int = 4096) -> TopLogits:
     """``top_logits`` of the LM head's h @ W^T, ``chunk`` tokens at a time, so
     that the [tokens, vocab] logits never exist at once. h: [..., dim]; the
     results are [..., k] and [...]."""
-    h2 = h.reshape(-1, h.shape[-1])
-    parts = [_fused.top_logits(_mm_fp32(c, W.t()), k, temperature) for c in h2.split(max(1, chunk))]
+    with _head(h.reshape(-1, h.shape[-1]), W) as (h2, W):
+        parts = [_fused.top_logits(_mm_fp32(c, W.t()), k, temperature) for c in h2.split(max(1, chunk))]
     values, indices, lse = (torch.cat(p) if len(p) > 1 else p[0] for p in zip(*parts))
     lead = h.shape[:-1]
     return TopLogits(values.view(*lead, k), indices.view(*lead, k), lse.view(lead))
@@ -267,4 +282,5 @@ def linear_distillation(h: torch.Tensor, W: torch.Tensor, labels: Optional[torch
     # of all rows at once: the chunks are slices, which would pass over a row too many
     _fused._check_distillation((h2.shape[0], W.shape[0]), *teacher)
     need = torch.is_grad_enabled() and (h.requires_grad or W.requires_grad)
-    return _LinearDistillation.apply(h2, W, *teacher, max(1, chunk), need)
+    with _head(h2, W) as (h2, W):
+        return _LinearDistillation.apply(h2, W, *teacher, max(1, chunk), need)

@@ -83,3 +83,21 @@ def test_vocabulary_masked_by_the_lowest_value(rest):
 @pytest.mark.parametrize("tau,V,k", [(10.0, 5003, 4), (30.0, 20000, 16), (100.0, 20000, 64)])
 def test_high_temperature(tau, V, k):
     check_high_temperature(tau, V, k, "cpu")
+
+
+# ------------------------------------------------------------------ autocast
+def test_autocast():
+    """As the call with its inputs in autocast's type: the fp32 products stay fp32, the gradients come back in the inputs' type."""
+    kw = linear_case()
+    kw["h"], kw["W"] = kw["h"].requires_grad_(), kw["W"].requires_grad_()
+    with torch.autocast("cpu", torch.bfloat16):
+        loss = L.linear_distillation(**kw)
+        top = L.linear_top_logits(kw["h"], kw["W"], 4)
+    got = torch.autograd.grad(loss, (kw["h"], kw["W"]))
+    low = dict(kw, h=kw["h"].detach().bfloat16().requires_grad_(), W=kw["W"].detach().bfloat16().requires_grad_())
+    want = L.linear_distillation(**low)
+    assert torch.equal(loss, want) and loss.dtype == torch.float32
+    for a, b in zip(got, torch.autograd.grad(want, (low["h"], low["W"]))):
+        assert a.dtype == torch.float32 and torch.equal(a, b.float())
+    for a, b in zip(top, L.linear_top_logits(low["h"], low["W"], 4)):
+        assert torch.equal(a, b)

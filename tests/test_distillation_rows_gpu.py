@@ -77,3 +77,23 @@ def test_head_gradient_over_a_large_vocabulary(labelled, alpha, tau, dtype):
 @pytest.mark.parametrize("tau,V,k", [(10.0, 5003, 4), (30.0, 20000, 16), (100.0, 20000, 64), (30.0, 128256, 16), (30.0, 128256, 256)])
 def test_high_temperature(tau, V, k, gdt):
     check_high_temperature(tau, V, k, DEV, gdt)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_autocast(dtype):
+    """As the call with its inputs in autocast's type, on an fp32 model's hidden states and head."""
+    T, V, D = 70, 2051, 64
+    _, labels, val, idx, lse = distill_case(T, V, 8, True, device=DEV)
+    g = torch.Generator(device=DEV).manual_seed(0)
+    h = torch.randn(T, D, device=DEV, generator=g).requires_grad_()
+    W = (torch.randn(V, D, device=DEV, generator=g) * 0.1).requires_grad_()
+    with torch.autocast("cuda", dtype):
+        loss = L.linear_distillation(h, W, labels, val, idx, lse, 1.0, 0.5, chunk=32)
+        top = L.linear_top_logits(h, W, 6)
+    got = torch.autograd.grad(loss, (h, W))
+    hl, Wl = h.detach().to(dtype).requires_grad_(), W.detach().to(dtype).requires_grad_()
+    want = L.linear_distillation(hl, Wl, labels, val, idx, lse, 1.0, 0.5, chunk=32)
+    assert torch.equal(loss, want)
+    for a, b in zip(got, torch.autograd.grad(want, (hl, Wl))):
+        assert a.dtype == torch.float32 and a.isfinite().all() and torch.equal(a, b.float())
+    assert all(torch.equal(a, b) for a, b in zip(top, L.linear_top_logits(hl, Wl, 6)))
