@@ -205,6 +205,20 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> window_attention_bwd(const at::Te
   return {dq, dk, dv};
 }
 
+// The op alone records no gradient (ops/fused.py wraps both passes): a call that would
+// drop one is an error.
+std::tuple<at::Tensor, at::Tensor, at::Tensor> window_attention_fwd_checked(const at::Tensor& q, const at::Tensor& k,
+                                                                            const at::Tensor& v, int64_t window,
+                                                                            int64_t sinks, bool backward) {
+  TORCH_CHECK(!at::GradMode::is_enabled() || !(q.requires_grad() || k.requires_grad() || v.requires_grad()),
+              "dion_b200 window_attention_fwd: this op records no gradient; dion_b200.ops.fused.window_attention does");
+  static const auto op = c10::Dispatcher::singleton()
+                             .findSchemaOrThrow("dion_b200::window_attention_fwd", "")
+                             .typed<decltype(window_attention_fwd)>();
+  at::AutoDispatchBelowADInplaceOrView below;
+  return op.call(q, k, v, window, sinks, backward);
+}
+
 }  // namespace bdion
 
 // A dispatcher op, so that selective activation checkpointing can name its
@@ -214,3 +228,4 @@ TORCH_LIBRARY(dion_b200, m) {
         "Tensor, Tensor)");
 }
 TORCH_LIBRARY_IMPL(dion_b200, CUDA, m) { m.impl("window_attention_fwd", &bdion::window_attention_fwd); }
+TORCH_LIBRARY_IMPL(dion_b200, Autograd, m) { m.impl("window_attention_fwd", &bdion::window_attention_fwd_checked); }

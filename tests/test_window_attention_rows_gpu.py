@@ -87,3 +87,12 @@ def test_non_finite_queries_and_gradients():
         _, dq, _, dv = run(q, k, v, do, window, sinks)
         keys = torch.tensor([bool(sees(s, window, sinks, t)[i]) for t in range(s)], device=DEV)
         assert dq[:, i].isnan().all() and dv[:, keys].isnan().all()
+
+
+def test_a_direct_call_of_the_op_does_not_drop_a_gradient():
+    q, k, v, _ = make(1, 40, 4, 2, 64)
+    with pytest.raises(RuntimeError, match="records no gradient"):
+        torch.ops.dion_b200.window_attention_fwd(q, k, v, 8, 1, False)
+    with torch.no_grad():
+        o = torch.ops.dion_b200.window_attention_fwd(q, k, v, 8, 1, False)[0]
+    assert torch.equal(o, L.window_attention(q, k, v, 8, 1).detach())
