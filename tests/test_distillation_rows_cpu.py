@@ -101,3 +101,16 @@ def test_autocast():
         assert a.dtype == torch.float32 and torch.equal(a, b.float())
     for a, b in zip(top, L.linear_top_logits(low["h"], low["W"], 4)):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("wanted", ["h", "W"])
+def test_one_gradient_wanted(wanted):
+    """A frozen head, or hidden states without a gradient: the other's is as with both."""
+    both = linear_case()
+    both["h"], both["W"] = both["h"].requires_grad_(), both["W"].requires_grad_()
+    want = torch.autograd.grad(L.linear_distillation(**both), both[wanted])[0]
+    one = dict(both, h=both["h"].detach(), W=both["W"].detach())
+    one[wanted] = one[wanted].requires_grad_()
+    loss = L.linear_distillation(**one)
+    loss.backward()
+    assert torch.equal(one[wanted].grad, want) and one["hW".replace(wanted, "")].grad is None

@@ -97,3 +97,17 @@ def test_autocast(dtype):
     for a, b in zip(got, torch.autograd.grad(want, (hl, Wl))):
         assert a.dtype == torch.float32 and a.isfinite().all() and torch.equal(a, b.float())
     assert all(torch.equal(a, b) for a, b in zip(top, L.linear_top_logits(hl, Wl, 6)))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("wanted", ["h", "W"])
+def test_one_gradient_wanted(wanted, dtype):
+    T, V, D = 70, 2056, 64
+    _, labels, val, idx, lse = distill_case(T, V, 8, True, device=DEV)
+    g = torch.Generator(device=DEV).manual_seed(0)
+    x = {"h": torch.randn(T, D, device=DEV, generator=g).to(dtype), "W": (torch.randn(V, D, device=DEV, generator=g) * 0.1).to(dtype)}
+    both = {n: t.clone().requires_grad_() for n, t in x.items()}
+    one = {n: t.clone().requires_grad_(n == wanted) for n, t in x.items()}
+    want, got = (torch.autograd.grad(L.linear_distillation(**a, labels=labels, top_values=val, top_indices=idx, top_lse=lse, alpha=0.5,
+                                                           chunk=32), a[wanted])[0] for a in (both, one))
+    assert torch.equal(want, got)
