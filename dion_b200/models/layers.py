@@ -274,7 +274,12 @@ def linear_distillation(h: torch.Tensor, W: torch.Tensor, labels: Optional[torch
     top logits (see :func:`dion_b200.ops.fused.distillation_fwd_bwd` for the
     loss). h: [..., dim], labels: [...] or None, top_values / top_indices:
     [..., k], top_lse: [...]. Rows whose label is outside [0, V) are left out
-    of the sum and of the mean; the loss is 0 if that leaves none."""
+    of the sum and of the mean; the loss is 0 if that leaves none.
+
+    The mean is over this call's rows. Where data parallelism averages gradients
+    over ranks that leave out unequally many, that is not the mean over all rows:
+    multiply each rank's loss by ranks * (its rows in the loss) / (those of all
+    ranks), which one all-reduce of the counts gives."""
     h2 = h.reshape(-1, h.shape[-1])
     flat = lambda t: None if t is None else t.reshape(-1)  # noqa: E731
     rows = lambda t: t.reshape(math.prod(t.shape[:-1]), t.shape[-1])  # noqa: E731

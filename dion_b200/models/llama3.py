@@ -319,4 +319,6 @@ class Transformer(nn.Module):
 
     def distillation_loss(self, tokens: torch.Tensor, labels: Optional[torch.Tensor], teacher: L.TopLogits,
                           temperature: float = 1.0, alpha: float = 1.0) -> torch.Tensor:
+        """Mean distillation loss over this rank's rows whose label takes part (see
+        :func:`~dion_b200.models.layers.linear_distillation`, also for ranks that leave out unequally many)."""
         return self(tokens, labels, teacher=teacher, temperature=temperature, alpha=alpha)

@@ -269,7 +269,7 @@ def _rows_enabled(x: torch.Tensor) -> bool:
 def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0) -> TopLogits:
     """The k largest logits of every row of [T, V] in falling order (equal ones
     by the lower index, a NaN above all), with the row's log-sum-exp at
-    ``temperature`` (1e-18 to 1e18). 1 <= k <= min(V, 1024)."""
+    ``temperature`` (1e-18 to 1e18). 1 <= k <= min(V, 1024); V up to 2^20 on CUDA."""
     if logits.dim() != 2:
         raise ValueError(f"top_logits: logits [T, V], got {tuple(logits.shape)}")
     T, V = logits.shape

@@ -114,3 +114,25 @@ def test_one_gradient_wanted(wanted):
     loss = L.linear_distillation(**one)
     loss.backward()
     assert torch.equal(one[wanted].grad, want) and one["hW".replace(wanted, "")].grad is None
+
+
+def test_unequal_rows_over_ranks():
+    """Two ranks' losses, each times ranks * (its rows) / (all rows) and averaged as data parallelism does, have the gradient
+    of the mean over all rows; the plain average has not."""
+    T = 12
+    kw = linear_case(T)
+    kw["labels"][:5] = -100
+    kw["labels"][5:] = torch.arange(T - 5)
+
+    def grad(rows, factor=1.0):
+        part = {n: t[rows] if torch.is_tensor(t) and n != "W" else t for n, t in kw.items()}
+        part["W"] = kw["W"].clone().requires_grad_()
+        return torch.autograd.grad(L.linear_distillation(**part) * factor, part["W"])[0]
+
+    halves = slice(0, 6), slice(6, T)
+    live = [int((kw["labels"][r] >= 0).sum()) for r in halves]
+    assert live == [1, 6]
+    whole = grad(slice(0, T))
+    scaled = sum(grad(r, 2 * n / sum(live)) for r, n in zip(halves, live)) / 2
+    torch.testing.assert_close(scaled, whole, rtol=1e-5, atol=1e-7)
+    assert not torch.allclose(sum(grad(r) for r in halves) / 2, whole, rtol=1e-2, atol=1e-4)
