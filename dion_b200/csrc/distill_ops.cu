@@ -658,16 +658,20 @@ __global__ void __launch_bounds__(kThreads, 2)
   }
   if (grad == nullptr) return;
 
-  // gradient. Outside the set: w_hard softmax(z) + w_soft q (1 - p_rest / q_rest), where
-  // 1 - p_rest / q_rest = (psum - q_set) / q_rest: at a high temperature the set holds
-  // little on either side, and the difference of two numbers near 1 would keep few bits
-  const float w_soft = a.grad_scale * a.alpha * a.tau * (psum + p_rest == 0.f ? 0.f : 1.f);
+  // gradient. In the set: w_hard softmax(z) + w_soft (mass q - p), mass = sum p + p_rest,
+  // which is not 1 where the entries hold more than all (columns that come twice), or less
+  // over the whole vocabulary. Outside: w_hard softmax(z) + w_soft q (1 - p_rest / q_rest)
+  // if there is a rest, where 1 - p_rest / q_rest = (psum - q_set) / q_rest: at a high
+  // temperature the set holds little on either side, and the difference of two numbers near
+  // 1 would keep few bits
+  const float w_soft = a.grad_scale * a.alpha * a.tau;
+  const float mass = p_rest > 0.f ? 1.f : psum;
   const float w_hard = hard ? a.grad_scale * (1.f - a.alpha) : 0.f;
   const float inv_B = 1.f / B, inv_F = both ? 1.f / F : inv_B;
   // factors of 2^(c (z - rm)), the first of them the teacher's part alone, and of 2^(log2e (z - rm))
   float f_soft = 0.f, f_rest = 0.f, f_full = 0.f;
   if (rest > 0.f || rest != rest) {
-    f_soft = w_soft * (p_rest > 0.f ? (psum - q_set) / rest : to_top * inv_B);
+    f_soft = w_soft * (p_rest > 0.f ? (psum - q_set) / rest : mass * to_top * inv_B);
     f_rest = f_soft + (both ? 0.f : w_hard * to_top * inv_B);
     f_full = both ? w_hard * to_top_full * inv_F : 0.f;
   }
@@ -719,7 +723,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     float p = 0.f;
     for (int e = j; e < (twice ? a.k : j + 1); ++e)
       if (s_i[e] == i && s_p[e] != -INFINITY) p += ex2(log_p(s_p[e]) * kLog2e);
-    float g = w_soft * (soft_at(s_z[j]) - p);
+    float g = w_soft * (mass * soft_at(s_z[j]) - p);
     if (hard) g += w_hard * (hard_at(s_z[j]) - (i == label ? 1.f : 0.f));
     put(gx + i, g);
   }

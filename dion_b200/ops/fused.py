@@ -350,8 +350,9 @@ def _distillation_ref(z, labels, top_values, top_indices, top_lse, tau, alpha, n
     logq = torch.log_softmax(relative(z) / tau, 1)
     kl = torch.where(p == 0, 0.0, p * (logp - logq.gather(1, at))).sum(1)
     q = logq.exp() if need_grad else None
+    # not 1 where columns come twice, or where the whole vocabulary is in the set and mass elsewhere
     mass = p.sum(1, keepdim=True)
-    soft = q
+    soft = torch.where(mass == 0, 0.0, mass * q) if need_grad else None
     if top_lse is not None:
         inside = torch.zeros_like(z).scatter_add(1, at, valid.to(z.dtype)) > 0
         p_rest = torch.where(inside.all(1, keepdim=True), 0.0, (1 - mass).clamp_min(0))
@@ -361,13 +362,12 @@ def _distillation_ref(z, labels, top_values, top_indices, top_lse, tau, alpha, n
         ratio = torch.where((mass < 0.5) & (q_set < 0.5), (-mass).log1p() - (-q_set).log1p(), p_rest.log() - rest)
         kl = kl + torch.where(p_rest > 0, p_rest * ratio, 0.0)[:, 0]
         if need_grad:
-            outside = torch.where(p_rest > 0, (mass - q_set) * (logq - rest).exp(), q)
-            soft = torch.where(inside | (rest == ninf), q, outside)
-        mass = mass + p_rest
+            outside = (mass - q_set) * (logq - rest).exp()
+            soft = torch.where(p_rest > 0, torch.where(inside | (rest == ninf), q, outside), soft)
     loss = alpha * tau * tau * kl if alpha > 0 else torch.zeros_like(kl)
     grad = None
     if need_grad:
-        grad = torch.where(mass == 0, 0.0, soft.scatter_add(1, at, -p)) * (alpha * tau)
+        grad = soft.scatter_add(1, at, -p) * (alpha * tau)
     if labels is not None:
         live = (labels >= 0) & (labels < V)
         y = labels.clamp(0, V - 1)[:, None]

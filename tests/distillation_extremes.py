@@ -82,3 +82,26 @@ def check_high_temperature(tau, V, k, device, gdt=None):
     tol = tol + (half + 2.0 ** -18) * wg.abs() + small
     tol = torch.where(out, tol, tol + tau * (logq.exp() * 2.0 ** -17).scatter_add(1, idx, lp.exp() * 2.0 ** -17))
     assert_within(grad, wg, tol, "grad")
+
+
+def check_other_masses(tau, alpha, device, dtype=torch.float32):
+    """A teacher's probabilities whose sum with the rest's is not 1: columns that come twice under a log-sum-exp of the whole
+    row (more than 1, nothing left for the rest), a log-sum-exp that is too small, entries over the student's whole
+    vocabulary with mass elsewhere. The gradient is that of the loss as it stands."""
+    z, labels, val, idx, lse = distill_case(9, 40, 40, True, dtype, tau=tau, seed=4, device=device)
+    order = torch.stack([torch.randperm(40, generator=torch.Generator().manual_seed(r)) for r in range(9)]).to(device)
+    val, idx = val.gather(1, order), idx.gather(1, order)
+    top = idx.clone()
+    top[0:3, 20:] = idx[0:3, :20]     # twenty columns, twice each
+    val[0:3, 20:] = val[0:3, :20]
+    lse[1] -= 1.0
+    lse[3] -= 0.5                     # all columns, a sum above 1
+    lse[4:7] += 0.7                   # all columns, a sum of 1/2
+    top[7, 5:] = -1                   # few columns, a sum above 1 for five of them
+    lse[7] = torch.logsumexp(val[7, :5] / tau, 0) - 0.3
+    labels = labels.clamp_min(0) if alpha < 1 else None
+    want, wg, tl, tg = distill_oracle(z, labels, val, top, lse, tau, alpha)
+    loss, grad = fused.distillation_fwd_bwd(z, labels, val, top, lse, tau, alpha)
+    assert abs(loss.item() - want.item()) <= tl.item(), (loss.item(), want.item(), tl.item())
+    half, small = halves(grad.dtype)
+    assert_within(grad, wg, half * wg.abs() + tg + small + 1e-30, "grad")

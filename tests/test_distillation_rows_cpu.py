@@ -5,7 +5,8 @@ import torch
 from dion_b200.models import layers as L
 from dion_b200.ops import fused
 
-from distillation_extremes import check_high_temperature, check_lowest, check_masked_vocabulary, check_offset
+from distillation_extremes import (check_high_temperature, check_lowest, check_masked_vocabulary, check_offset,
+                                    check_other_masses)
 from test_distillation_cpu import distill_case
 
 
@@ -136,3 +137,8 @@ def test_unequal_rows_over_ranks():
     scaled = sum(grad(r, 2 * n / sum(live)) for r, n in zip(halves, live)) / 2
     torch.testing.assert_close(scaled, whole, rtol=1e-5, atol=1e-7)
     assert not torch.allclose(sum(grad(r) for r in halves) / 2, whole, rtol=1e-2, atol=1e-4)
+
+
+@pytest.mark.parametrize("tau,alpha", [(1.0, 1.0), (2.0, 0.5), (1.5, 0.5)])
+def test_masses_that_do_not_sum_to_one(tau, alpha):
+    check_other_masses(tau, alpha, "cpu")

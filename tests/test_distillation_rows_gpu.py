@@ -4,7 +4,8 @@ import torch
 
 from dion_b200.models import layers as L
 
-from distillation_extremes import check_high_temperature, check_lowest, check_masked_vocabulary, check_offset
+from distillation_extremes import (check_high_temperature, check_lowest, check_masked_vocabulary, check_offset,
+                                    check_other_masses)
 from operator_oracles import distill_oracle, halves
 from test_distillation_cpu import distill_case
 from test_distillation_gpu import TYPES
@@ -111,3 +112,9 @@ def test_one_gradient_wanted(wanted, dtype):
     want, got = (torch.autograd.grad(L.linear_distillation(**a, labels=labels, top_values=val, top_indices=idx, top_lse=lse, alpha=0.5,
                                                            chunk=32), a[wanted])[0] for a in (both, one))
     assert torch.equal(want, got)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tau,alpha", [(1.0, 1.0), (2.0, 0.5), (1.5, 0.5), (1.0, 0.5)])
+def test_masses_that_do_not_sum_to_one(tau, alpha, dtype):
+    check_other_masses(tau, alpha, DEV, dtype)
