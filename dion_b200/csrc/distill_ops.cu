@@ -192,11 +192,16 @@ __device__ __forceinline__ uint32_t kth_key(const uint32_t (&key)[R], int k) {
 // second bound has thinned them out. Rows with too many candidates (equal
 // values; also checked: too few), and rows with a NaN or +inf, take the exact
 // threshold over the whole row bit by bit and keep the lowest indices of the equal ones.
-// 4096 x 128256 bf16, k = 64: 378 us, 2.8 TB/s (161 us at the copy rate); 1500 x
-// 50009 fp32, k = 200: 139 us. Bound by instructions and by the steps in which one
-// warp searches for a bound while the row's others wait; three rows to an SM (two in
-// fp32, whose groups take twice the registers) overlap these. Two full passes took 576 us, a
-// sample of half the size (twice the candidates) 601 us where this took 534.
+// 4096 x 128256 bf16, k = 64: 379 us, 2.8 TB/s (161 us at the copy rate); the same in
+// fp32 behind a head's product 514 us; 1500 x 50009 fp32, k = 200: 140 us. Bound by
+// instructions (70 % of the issue slots) and by the steps in which one warp searches for
+// a bound while the row's others wait; three rows to an SM (two in fp32, whose groups
+// take twice the registers) overlap these. Two full passes took 576 us, a sample of half
+// the size (twice the candidates) 601 us where this took 534.
+// Beyond 256 entries the sample is the whole row: k = 300 at 4096 x 128256 bf16 takes 563
+// us. Where the candidates' buffer then overflows, most of all in small vocabularies, the
+// rows take the exact way: 4096 x 4096 at k = 512 610 us, at k = 1024 1157 us, 4096 x
+// 32768 at k = 1024 1506 us, against 504 us for 1024 x 128256 at k = 1024.
 template <typename T, int G>
 __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 3 : 2)
     top_logits_kernel(const T* __restrict__ logits, int64_t ld, int V, int k, bool vec, int ns, float inv_tau,
@@ -431,11 +436,13 @@ enum HardMode { kHardNone, kHardSquare, kHardOther };
 // The entries' columns are marked in a bitmap, so that the sum over the rest
 // is taken directly (1 - sum q_j would cancel when the student is sure) and
 // keeps a maximum of its own. 4096 x 128256 bf16 at temperature 2 with labels:
-// 499 us, 4.2 TB/s of the bytes that have to move (322 us at the copy rate). Both
-// passes issue about as many instructions as the memory's time allows, and some of
-// the second reads miss L2. Holding a row in the registers of a cluster of four
-// blocks, so that it is read once, took 714 us at best: its blocks wait for one
-// another's sums with nothing else to do.
+// 495 us, 4.2 TB/s of the bytes that have to move (322 us at the copy rate); 512 us in
+// passes repeated for over a second (1822 MHz). fp32 logits: 2048 x 128256 with an fp32
+// gradient 493 us at 1725 MHz, 4096 x 128256 with a bf16 one 907 us within linear
+// distillation (1522 MHz). No unit is full (58 % of the issue slots and of DRAM): the
+// two passes of a row with sums between them, two rows to an SM, leave latency. Holding
+// a row in the registers of a cluster of four blocks, so that it is read once, took 714
+// us at best: its blocks wait for one another's sums with nothing else to do.
 template <typename T, typename TG, int MODE>
 __global__ void __launch_bounds__(kThreads, 2)
     distill_kernel(const T* __restrict__ logits, TG* __restrict__ grad, const DistillArgs a) {
@@ -797,7 +804,7 @@ void top_logits(const at::Tensor& logits, at::Tensor& values, at::Tensor& indice
   auto s = at::cuda::getCurrentCUDAStream();
   by_type(logits.scalar_type(), [&](auto tag) {
     using E = decltype(tag);
-    // rounds in the sample: about 256 columns reach its bound
+    // rounds in the sample: about 256 columns reach its bound, or more than k where k is larger
     const int rounds = (V / 8 + kThreads - 1) / kThreads;
     const int ns = std::max(1, std::min(rounds, (rounds * k + 255) / 256));
     auto launch = [&](auto g) {
@@ -805,7 +812,8 @@ void top_logits(const at::Tensor& logits, at::Tensor& values, at::Tensor& indice
           static_cast<const E*>(logits.data_ptr()), logits.stride(0), V, k, aligned8(logits), ns, (float)(1 / tau),
           (float)(kLog2e / tau), values.data_ptr<float>(), indices.data_ptr<int64_t>(), lse.data_ptr<float>());
     };
-    // at least twice as many groups as entries keeps the candidates near 1.4 k
+    // at least twice as many sets as entries, where the row has that many groups, keeps the
+    // candidates near 1.4 k
     if (k <= kThreads / 2)
       launch(std::integral_constant<int, 1>{});
     else

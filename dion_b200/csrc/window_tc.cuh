@@ -89,12 +89,16 @@ struct FwdCfg {
 // row per thread. S has two buffers, so the next step's scores are there when a
 // row is done with this one's, and P V runs under the next step's exponentials.
 //
-// Measured: 1 x 32763 positions, 8 heads of 128 on one key head, fp16, window 4096:
-// 486 us, 1.08 PFLOP/s (0.64 of the measured bf16 rate); 1 x 8192, 32 heads of 128,
-// window 2048: 244 us without and 260 us with o's remainder; 2 x 4096, 32 heads of
-// 64, window 1024: 127 us. Steps of 128 keys with one buffer of S: 309 us for the
-// second of these. At 128 the tensor cores bound it (a product of 128 x 64 x 16 from
-// shared memory takes about as long as one of 128 x 128 x 16), at 64 the rows' work.
+// Measured in passes repeated for over a second (SM clock beside it; the power cap
+// lowers it): 1 x 32763 positions, 8 heads of 128 on one key head, fp16, window 4096:
+// 566 us, 0.92 PFLOP/s at 1507 MHz (485 us in a run too short for the cap); 1 x 8192,
+// 32 heads of 128, window 2048, with o's remainder: 301 us at 1687 MHz (260); 2 x 4096,
+// 32 heads of 64, window 1024: 134 us at 1882 MHz (127). Steps of 128 keys with one
+// buffer of S: 309 us where these took 244, both without the remainder and in short
+// runs. At 128 a product of 128 x 64 x 16 from shared memory takes about as long as one
+// of 128 x 128 x 16, so S runs at half the tensor cores' rate; at 64 no unit is half
+// busy, and the chain from TMEM load to TMEM store bounds it with the few warps (17 %)
+// that two CTAs of four row warps are.
 //
 // A row's running maximum is the reference of its exponentials. It is moved
 // only when a step exceeds it by more than 2^8, so O in TMEM is rarely rescaled;
@@ -368,11 +372,13 @@ struct DqCfg {
 // The next step's S is computed as soon as the rows have read this one's, its dP
 // goes into the other buffer, so the rows work from step to step without waiting
 // for the sums. (Steps of 64 keys: a product of 128 x 64 x 16 takes as long from
-// shared memory as one of 128 x 128 x 16; 492 us where this takes 389, 1 x 8192, 32
-// heads of 128, window 2048. At 64 both take about 182 us at 2 x 4096, 32 heads,
-// window 1024.) The tensor cores bound it at 128: 24 products of 128 x 128 x 16 a step
-// at some 80 cycles. delta is taken here from O and dO and
-// kept, negated, for the dK / dV kernel (0 behind the last position).
+// shared memory as one of 128 x 128 x 16; 492 us where this took 389 in short runs, 1 x
+// 8192, 32 heads of 128, window 2048. At 64 both took about 182 us at 2 x 4096, 32
+// heads, window 1024.) In passes repeated for over a second: 450 us at 1687 MHz and 197
+// us at 1882 MHz. At 128 the tensor cores bound it, 24 products of 128 x 128 x 16 a step
+// at some 80 cycles; at 64 the chain S, rows, dQ, with 28 % of the warps. delta is taken
+// here from O and dO and kept, negated, for the dK / dV kernel (0 behind the last
+// position).
 template <typename T, int DP>
 __global__ void __launch_bounds__(576, 1)
     window_dq_tc(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
@@ -675,9 +681,10 @@ struct DkvCfg {
 // shared memory. Four threads share a key row, a quarter of the step's queries
 // each: a thread reads its 32 columns of dP^T and packs P^T and dS^T into them,
 // so S^T is free for the next step as soon as it has been read. 2 x 4096, 32 heads of
-// 64 on 8, window 1024: 191 us (216 with P^T on S^T, 273 in steps of 64 queries); 1 x
-// 8192, 32 heads of 128 on 8, window 2048: 521 us (508, 540). At 128 TMEM has room for
-// one buffer of dP^T, and the chain dP^T -> rows -> dV, dK -> next dP^T bounds it.
+// 64 on 8, window 1024, in short runs: 191 us (216 with P^T on S^T, 273 in steps of 64
+// queries); 1 x 8192, 32 heads of 128 on 8, window 2048: 521 us (508, 540). In passes
+// repeated for over a second: 201 us at 1882 MHz and 606 us at 1687 MHz. At 128 TMEM has
+// room for one buffer of dP^T, and the chain dP^T -> rows -> dV, dK -> next dP^T bounds it.
 template <typename T, int DP>
 __global__ void __launch_bounds__(576, 1)
     window_dkv_tc(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,

@@ -118,3 +118,15 @@ def test_one_gradient_wanted(wanted, dtype):
 @pytest.mark.parametrize("tau,alpha", [(1.0, 1.0), (2.0, 0.5), (1.5, 0.5), (1.0, 0.5)])
 def test_masses_that_do_not_sum_to_one(tau, alpha, dtype):
     check_other_masses(tau, alpha, DEV, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_without_rows(dtype):
+    _, labels, val, idx, lse = (t[:0] for t in distill_case(3, 24, 4, True, device=DEV))
+    h = torch.randn(0, 8, device=DEV).to(dtype).requires_grad_()
+    W = torch.randn(24, 8, device=DEV).to(dtype).requires_grad_()
+    loss = L.linear_distillation(h, W, labels, val, idx, lse, 1.0, 0.5)
+    gh, gW = torch.autograd.grad(loss, (h, W))
+    assert loss.item() == 0 and gh.shape == (0, 8) and not gW.any()
+    top = L.linear_top_logits(h.detach().view(2, 0, 8), W, 4)
+    assert top.values.shape == (2, 0, 4) and top.indices.shape == (2, 0, 4) and top.lse.shape == (2, 0)

@@ -26,10 +26,10 @@ def _train_body(kw, rank, world):
 
 
 @functools.lru_cache(None)
-def _alone():
-    (status, res), = spawn(functools.partial(_train_body, {}), world=1).values()
+def _alone(body):
+    (status, res), = spawn(functools.partial(body, {}), world=1).values()
     assert status == "ok", res
-    return torch.tensor(res)
+    return res
 
 
 @pytest.mark.parametrize("kw", [dict(tp=2, sequence_parallel=False), dict(tp=2, sequence_parallel=True),
@@ -38,7 +38,8 @@ def test_training_matches_one_process(kw):
     out = spawn(functools.partial(_train_body, kw), world=2)
     for status, res in out.values():
         assert status == "ok", res
-    assert torch.allclose(_alone(), torch.tensor(out[0][1]), rtol=2e-3, atol=2e-3), (_alone(), out[0][1])
+    want = torch.tensor(_alone(_train_body))
+    assert torch.allclose(want, torch.tensor(out[0][1]), rtol=2e-3, atol=2e-3), (want, out[0][1])
 
 
 def _distill_body(kw, rank, world):
@@ -63,11 +64,10 @@ def _distill_body(kw, rank, world):
 
 @pytest.mark.parametrize("kw", [dict(dp_shard=2, local_batch_size=2), dict(tp=2, sequence_parallel=False)])
 def test_distillation_matches_one_process(kw):
-    ref = spawn(functools.partial(_distill_body, {}), world=1)
     out = spawn(functools.partial(_distill_body, kw), world=2)
-    for status, res in list(ref.values()) + list(out.values()):
+    for status, res in out.values():
         assert status == "ok", res
-    (loss, grads, idx, lse), ranks = ref[0][1], [out[r][1] for r in range(2)]
+    (loss, grads, idx, lse), ranks = _alone(_distill_body), [out[r][1] for r in range(2)]
     cut = "dp_shard" in kw
     assert abs(sum(r[0] for r in ranks) / 2 - loss) < 1e-5 * loss
     for r, (_, g, i, z) in enumerate(ranks):
