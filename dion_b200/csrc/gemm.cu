@@ -36,6 +36,8 @@ CUtensorMap make_map(const void* base, bool fp32, int64_t cols, int64_t rows, in
   CUtensorMap m;
   const int esz = fp32 ? 4 : 2;
   cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)batch};
+  // the stride of a single row leads nowhere: a view of one row of a wider tensor may have any
+  if (rows <= 1) ld = (cols + 15) / 16 * 16;
   if (batch <= 1) bstride = ld * rows;
   cuuint64_t strides[2] = {(cuuint64_t)(ld * esz), (cuuint64_t)(bstride * esz)};
   cuuint32_t box[3] = {(cuuint32_t)(128 / esz), (cuuint32_t)box_rows, 1u};
