@@ -222,11 +222,13 @@ class _LinearDistillation(torch.autograd.Function):
         rounds to itself, where -(1 - alpha) would be off by the same part in every
         row. In fp16 a power of two on top: an entry of a 128k vocabulary is 8e-6 on
         average, among the subnormals (spacing 6e-8), while no entry exceeds
-        (1 - alpha) + alpha * temperature; that bound is brought to 2^14 ... 2^15."""
+        (1 - alpha) + alpha * temperature times the teacher's mass; with a mass of 1 that
+        bound is brought to 2^13 ... 2^14, so that one of 3 (columns that come twice under
+        a log-sum-exp of the row) stays finite as well."""
         hard = 1.0 - alpha if labels is not None and alpha < 1 else 0.0
         scale = 1.0 / hard if hard else 1.0
         if dtype == torch.float16:
-            scale *= 2.0 ** (15 - math.ceil(math.log2((hard + alpha * temperature) * scale)))
+            scale *= 2.0 ** (14 - math.ceil(math.log2((hard + alpha * temperature) * scale)))
         return scale
 
     @staticmethod

@@ -41,8 +41,8 @@ def test_head_gradient_over_a_large_vocabulary(labelled, alpha, tau, dtype):
     of nearly 1 - alpha. In the mean square over such rows, two roundings (the logits' gradient, the result), each
     half / sqrt(3) of its value, and a quarter more for all that is fp32. (The loss is scaled as fp16 wants, so that
     the result itself is not among the subnormals.) In fp16 an entry of the logits' gradient that is a subnormal under
-    its factor, 2^14 / temperature at least, is off by up to 2^-25 whatever its size, 2^-25 / sqrt(3) in the mean
-    square, so each of the head's entries by that / factor * sqrt(sum h^2): what is 2^-39 of the largest possible
+    its factor, 2^13 / temperature at least, is off by up to 2^-25 whatever its size, 2^-25 / sqrt(3) in the mean
+    square, so each of the head's entries by that / factor * sqrt(sum h^2): what is 2^-38 of the largest possible
     entry (at temperature 30 without labels, the rows in question are) keeps fewer bits."""
     T, V, D = 96, 128256, 64
     _, labels, val, idx, lse = distill_case(T, V, 16, True, tau=tau, device=DEV)
